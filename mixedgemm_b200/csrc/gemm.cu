@@ -25,8 +25,6 @@
 //                                     128-row operand, tile stored transposed
 //   mixed_gemm_kernel<128 | 256>      everything else; with 34..74 tiles and a long K several CTAs
 //                                     per tile, partial sums through the caller's workspace
-#include <cuda.h>
-#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -37,9 +35,16 @@
 #include <random>
 
 #include "mg_common.h"
+#include "mg_wait.cuh"
 #include "ptx_sm100.cuh"
+#include "tensor_map.h"
 
 namespace {
+
+using mg::get_encoder;
+using mg::make_map;
+using mg::wait_parity;
+using mg::wait_parity_cluster;
 
 constexpr int BM = 128;
 constexpr int kThreads = 192;
@@ -74,50 +79,6 @@ struct GemmParams {
   unsigned long long sp_token;      // 56 bits, unique per launch: a word with another token counts as 0
   float* sp_partials;  // [split][tile][column group of 4][sp_rows][4]
 };
-
-// Bounded mbarrier wait: true once the phase has completed.  When the limit expires the lane
-// records `code`, raises the CTA's stop flag and returns false; from then on every wait of the CTA
-// that does not find its phase complete at the first probe returns false at once.  A role whose
-// wait failed issues nothing more (no copies, no MMAs, no arrivals) and leaves its loops; the
-// kernel then ends normally, with nothing stored.
-__device__ __forceinline__ bool wait_parity(uint32_t bar, uint32_t parity, volatile int* stop, int* status,
-                                            long long limit, int code) {
-  if (ptx::mbar_try_wait(bar, parity)) return true;
-  long long t0 = 0;
-  for (uint32_t spin = 0;; ++spin) {
-    if (ptx::mbar_try_wait(bar, parity)) return true;
-    if ((spin & 63u) == 0) {
-      if (*stop) return false;
-      const long long now = clock64();
-      if (spin == 0) t0 = now;
-      if (now - t0 > limit) {
-        *stop = 1;
-        atomicOr(status, code);
-        return false;
-      }
-    }
-  }
-}
-
-// The same for a barrier whose phase is completed by other CTAs of the cluster.
-__device__ __forceinline__ bool wait_parity_cluster(uint32_t bar, uint32_t parity, volatile int* stop, int* status,
-                                                    long long limit, int code) {
-  if (ptx::mbar_try_wait_cluster(bar, parity)) return true;
-  long long t0 = 0;
-  for (uint32_t spin = 0;; ++spin) {
-    if (ptx::mbar_try_wait_cluster(bar, parity)) return true;
-    if ((spin & 63u) == 0) {
-      if (*stop) return false;
-      const long long now = clock64();
-      if (spin == 0) t0 = now;
-      if (now - t0 > limit) {
-        *stop = 1;
-        atomicOr(status, code);
-        return false;
-      }
-    }
-  }
-}
 
 // Tile order: row blocks in groups of eight, all column blocks of a group before the next group.
 // The CTAs (or clusters) running at one time then share about eight A tiles and nine B tiles instead
@@ -1036,40 +997,6 @@ __global__ void repack_rows_kernel(const RepackJobs jobs) {
 }
 
 // ---------------------------------------------------------------- host side
-PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
-std::once_flag g_encode_once;
-
-int get_encoder(PFN_cuTensorMapEncodeTiled_v12000* out) {
-  std::call_once(g_encode_once, [] {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-  });
-  *out = g_encode;
-  return g_encode ? MG_OK : MG_ERR_CUDA;
-}
-
-// 2-D K-major operand: `kdim` elements of type `dt` per row, `rows` rows, `pitch` bytes.
-int make_map(CUtensorMap* m, CUtensorMapDataType dt, const void* ptr, uint64_t kdim, uint64_t rows,
-             uint64_t pitch, uint32_t box_k, uint32_t box_rows) {
-  PFN_cuTensorMapEncodeTiled_v12000 enc;
-  if (get_encoder(&enc) != MG_OK) return MG_ERR_CUDA;
-  cuuint64_t dims[2] = {kdim, rows};
-  cuuint64_t strides[1] = {pitch};
-  cuuint32_t box[2] = {box_k, box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(m, dt, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    mg::note_cuda_error(cudaErrorInvalidValue);
-    return MG_ERR_CUDA;
-  }
-  return MG_OK;
-}
-
 // 3-D K-major operand stored in row shards: `kdim` elements per row, `shard_rows` rows `pitch` bytes
 // apart per shard, `nshards` shards `shard_stride` bytes apart.  One shard describes a plain 2-D operand.
 int make_map3(CUtensorMap* m, CUtensorMapDataType dt, const void* ptr, uint64_t kdim, uint64_t shard_rows,
