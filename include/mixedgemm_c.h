@@ -396,6 +396,50 @@ int mg_matmul_static_ws(const uint8_t* AN, const uint8_t* BN, const uint8_t* AS,
                         const uint8_t* SFAS, const uint8_t* SFBS, const uint8_t* SFAO, const uint8_t* SFBO,
                         void* stream);
 
+/*
+ * 8-bit integers with a scale for each row.  No counterpart in the reference: the form for layers
+ * that 4-bit weights hurt, and the norm that stands in front of either form.
+ *
+ * Element types of activations and results. */
+enum { MG_BF16 = 0, MG_FP16 = 1, MG_FP32 = 2 };
+/* Longest row: the 32-bit sum of K products of magnitude 2^14 stays in range. */
+#define MG_INT8_MAX_K 131071
+
+/*
+ * Q[r,k] = rint(X[r,k] * (127 / a_r)), scale[r] = a_r / 127, a_r = max(max_k |X[r,k]|, 2^-100), in fp32.
+ *   X      [M,K] of `dtype`, rows `ldx` elements apart (tokens of an activation, channels of a weight)
+ *   Q      [M,K] int8, rows `ldq` bytes apart; bytes beyond K are left alone
+ *   scale  [M] fp32
+ * A row that holds a NaN or an infinity gets the scale NaN and codes 0.  Any alignment of X and Q is
+ * taken; rows that all start on 16-byte boundaries (Q: 8) with K a multiple of 8 (fp32: 4) take the
+ * vector form.  M may be 0.
+ */
+int mg_quantize_int8(const void* X, int dtype, int M, int K, size_t ldx, int8_t* Q, size_t ldq, float* scale,
+                     void* stream);
+
+/*
+ * Root-mean-square norm with the residual's addition, quantised as above:
+ *   u = X + R rounded to `dtype` (written to U; R and U are both NULL when there is no residual)
+ *   h = u * W / sqrt(mean_k u^2 + eps) in fp32;   Q, scale = the 8-bit form of h
+ *   W [K] of `dtype`.  U may be R or X itself.  A row whose sum of squares is not a finite fp32 number
+ *   gets the scale NaN and codes 0.
+ */
+int mg_rms_norm_int8(const void* X, const void* R, const void* W, float eps, int dtype, int M, int K, size_t ldx,
+                     size_t ldr, void* U, size_t ldu, int8_t* Q, size_t ldq, float* scale, void* stream);
+
+/*
+ * D[m,n] = (sum_k A[m,k] B[n,k]) * scale_a[m] * scale_b[n] + bias[n], the sum exact in 32-bit integers,
+ * the rest in fp32, rounded once to `dtype`.
+ *   A [M,K], B [N,K] int8, rows lda / ldb bytes apart: base and pitch multiples of 16 bytes, bytes
+ *          beyond K never read into the sum (K itself may be any value up to MG_INT8_MAX_K)
+ *   scale_a [M], scale_b [N] fp32;  bias [N] fp32 or NULL
+ *   D      [M,N] of `dtype`, rows ldd elements apart, any alignment of its type
+ * No workspace.  M, N may be 0.
+ */
+int mg_matmul_int8(const int8_t* A, size_t lda, const int8_t* B, size_t ldb, const float* scale_a,
+                   const float* scale_b, const float* bias, int M, int N, int K, void* D, int dtype, size_t ldd,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

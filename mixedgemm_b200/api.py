@@ -387,6 +387,135 @@ def matmul_multi(problems, flags=None):
     return outs
 
 
+# ----------------------------------------------------------------- 8-bit integers, a scale per row
+
+_ELEMENT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # MG_BF16, MG_FP16, MG_FP32
+
+
+def _on(dev, fn, *args):
+    """fn(*args, stream) with `dev` current; the usual case, `dev` being current already, costs nothing."""
+    if torch.cuda.current_device() == dev.index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    with torch.cuda.device(dev):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+
+
+def _rows(t, what, name, dev=None, like=None, dtype=None):
+    """Row pitch (elements) of a 2-D CUDA tensor whose rows are dense and do not overlap."""
+    if not t.is_cuda or t.dim() != 2 or (dev is not None and t.device != dev):
+        raise RuntimeError("%s: %s must be a 2-D CUDA tensor%s" % (what, name, "" if dev is None else " on the others' device"))
+    if like is not None and t.shape != like:
+        raise RuntimeError("%s: %s has shape %s where %s is expected" % (what, name, tuple(t.shape), tuple(like)))
+    if dtype is not None and t.dtype != dtype:
+        raise RuntimeError("%s: %s must be %s, not %s" % (what, name, dtype, t.dtype))
+    M, K = t.shape
+    s0, s1 = t.stride()
+    if (s1 != 1 and K > 1) or (s0 < K and M > 1):
+        raise RuntimeError("%s: the rows of %s must have unit stride and must not overlap (strides %s)" % (what, name, (s0, s1)))
+    return s0 if M > 1 else K
+
+
+def _vector(t, what, name, n, dev, dtype):
+    if not t.is_cuda or t.device != dev or t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        raise RuntimeError("%s: %s must be a contiguous %s tensor of %d elements on the others' device" % (what, name, dtype, n))
+    return t
+
+
+def _int8_outputs(M, K, dev, out, what):
+    """(codes, row pitch, scale): the caller's, or new ones whose rows matmul_int8 can read in place."""
+    if out is None:
+        pitch = (K + 15) // 16 * 16
+        return (torch.empty_strided((M, K), (pitch, 1), dtype=torch.int8, device=dev), pitch,
+                torch.empty(M, dtype=torch.float32, device=dev))
+    q, scale = out
+    return q, _rows(q, what, "the codes", dev, (M, K), torch.int8), _vector(scale, what, "the scale", M, dev, torch.float32)
+
+
+def quantize_int8(X, out=None):
+    """Rows of X [M,K] (bf16, fp16 or fp32; tokens of an activation or output channels of a weight) in
+    8 bits: returns (codes int8 [M,K], scale fp32 [M]) with X ~ codes * scale[:, None], scale = largest
+    magnitude of the row / 127, codes rounded to nearest even.  The rows of X may be any distance
+    apart; those of the codes start on 16-byte boundaries, as matmul_int8 needs them.  A row with a
+    value that is not finite gets the scale NaN and codes 0.  `out` = (codes, scale) to write into."""
+    ldx = _rows(X, "quantize_int8", "X")
+    if X.dtype not in _ELEMENT:
+        raise RuntimeError("quantize_int8: X must be bfloat16, float16 or float32, not %s" % X.dtype)
+    M, K = X.shape
+    q, ldq, scale = _int8_outputs(M, K, X.device, out, "quantize_int8")
+    st = _on(X.device, _capi.load().mg_quantize_int8, X.data_ptr(), _ELEMENT[X.dtype], M, K, ldx, q.data_ptr(), ldq,
+             scale.data_ptr())
+    if st:
+        _capi.check(st, "quantize_int8")
+    return q, scale
+
+
+def _norm_inputs(X, weight, residual, residual_out, what):
+    """Checks of the fused norms; returns (ldx, ldr, residual_out, ldu)."""
+    ldx = _rows(X, what, "X")
+    _vector(weight, what, "the norm's weight", X.size(1), X.device, X.dtype)
+    if residual is None:
+        if residual_out is not None:
+            raise RuntimeError("%s: residual_out without a residual" % what)
+        return ldx, 0, None, 0
+    ldr = _rows(residual, what, "the residual", X.device, X.shape, X.dtype)
+    if residual_out is None:
+        residual_out = torch.empty(X.shape, dtype=X.dtype, device=X.device)
+        return ldx, ldr, residual_out, X.size(1)
+    return ldx, ldr, residual_out, _rows(residual_out, what, "residual_out", X.device, X.shape, X.dtype)
+
+
+def rms_norm_int8(X, weight, eps=1e-6, residual=None, residual_out=None, out=None):
+    """quantize_int8 of the root-mean-square norm of X [M,K] (+ residual), in one launch:
+    u = X + residual (rounded to X's type), h = u * weight / sqrt(mean(u^2) + eps) in fp32.
+    Returns (codes, scale), with a residual (codes, scale, u): u is the stream that goes on.
+    weight [K] and residual [M,K] have X's type; residual_out may be `residual` (or X) itself, to
+    update the stream in place.  A row whose sum of squares is not a finite fp32 number gets the
+    scale NaN and codes 0."""
+    ldx, ldr, u, ldu = _norm_inputs(X, weight, residual, residual_out, "rms_norm_int8")
+    if X.dtype not in _ELEMENT:
+        raise RuntimeError("rms_norm_int8: X must be bfloat16, float16 or float32, not %s" % X.dtype)
+    M, K = X.shape
+    q, ldq, scale = _int8_outputs(M, K, X.device, out, "rms_norm_int8")
+    st = _on(X.device, _capi.load().mg_rms_norm_int8, X.data_ptr(), None if u is None else residual.data_ptr(),
+             weight.data_ptr(), eps, _ELEMENT[X.dtype], M, K, ldx, ldr, None if u is None else u.data_ptr(), ldu,
+             q.data_ptr(), ldq, scale.data_ptr())
+    if st:
+        _capi.check(st, "rms_norm_int8")
+    return (q, scale) if u is None else (q, scale, u)
+
+
+def matmul_int8(A, B, scale_a, scale_b, bias=None, out=None, out_dtype=None):
+    """A [M,K] int8 (tokens) times B [N,K] int8 (channels), both with a scale per row:
+    (A @ B^T, exact in 32-bit integers) * scale_a[:, None] * scale_b[None, :] + bias, rounded once to
+    `out_dtype` (bfloat16 unless given; float16 or float32).  scale_a [M], scale_b [N] and bias [N]
+    are fp32.  Rows of A and B start on 16-byte boundaries (those of quantize_int8 do); K is at most
+    131071.  `out` [M,N] receives the result instead of a new tensor; its rows may be any distance apart."""
+    lda = _rows(A, "matmul_int8", "A", dtype=torch.int8)
+    dev = A.device
+    ldb = _rows(B, "matmul_int8", "B", dev, dtype=torch.int8)
+    M, K = A.shape
+    N = B.size(0)
+    if B.size(1) != K:
+        raise RuntimeError("matmul_int8: A has rows of %d elements, B of %d" % (K, B.size(1)))
+    _vector(scale_a, "matmul_int8", "scale_a", M, dev, torch.float32)
+    _vector(scale_b, "matmul_int8", "scale_b", N, dev, torch.float32)
+    if bias is not None:
+        _vector(bias, "matmul_int8", "the bias", N, dev, torch.float32)
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype or torch.bfloat16, device=dev)
+        ldd = N
+    else:
+        ldd = _rows(out, "matmul_int8", "out", dev, (M, N), out_dtype)
+    if out.dtype not in _ELEMENT:
+        raise RuntimeError("matmul_int8: the result must be bfloat16, float16 or float32, not %s" % out.dtype)
+    st = _on(dev, _capi.load().mg_matmul_int8, A.data_ptr(), lda, B.data_ptr(), ldb, scale_a.data_ptr(),
+             scale_b.data_ptr(), None if bias is None else bias.data_ptr(), M, N, K, out.data_ptr(),
+             _ELEMENT[out.dtype], ldd)
+    if st:
+        _capi.check(st, "matmul_int8")
+    return out
+
+
 def set_option(name, value):
     """mg_set_option: choose between kernels / turn a mode off at run time (names in mixedgemm_c.h)."""
     _capi.check(_capi.load().mg_set_option(name.encode(), int(value)), "set_option(%s)" % name)

@@ -1,0 +1,345 @@
+// Product of 8-bit integers with a scale per token and per channel, for sm_100a:
+//
+//   D[m,n] = (sum_k A[m,k] B[n,k]) * sa[m] * sb[n] + bias[n]
+//
+// The sum runs on the tensor cores (tcgen05.mma kind::i8) in 32-bit integers held in tensor memory,
+// so it is exact and does not depend on the order or on how K is split.  The channels are the MMA's
+// 128-row operand and the tokens its column operand: a thread of the epilogue then owns one channel
+// (its scale and bias are two registers), a warp stores 32 consecutive channels of one token, and no
+// alignment of D is needed; a tile carries only as many tokens as there are.  Rows beyond M or N and
+// bytes beyond K are filled with zeros by the tensor-map loads.
+//
+//   warp 0      producer: one 128-byte slice of K per stage for both operands (tiled tensor maps,
+//               128-byte swizzle)
+//   warp 1      MMA issuer: four K = 32 instructions per stage; owns the tensor memory
+//   warps 2-5   epilogue
+//
+// All waits are bounded (see mg_wait.cuh); a kernel that gives up stores nothing.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "mg_common.h"
+#include "mg_wait.cuh"
+#include "ptx_sm100.cuh"
+#include "tensor_map.h"
+
+namespace {
+
+using mg::wait_parity;
+
+constexpr int kRows = 128;      // channels of a CTA's tile
+constexpr int kThreads = 192;
+constexpr int kMaxSplit = 8;
+
+struct Int8Params {
+  int M, N;
+  int stages;  // 128-byte slices of K
+  const float* sa;
+  const float* sb;
+  const float* bias;
+  void* D;
+  size_t ldd;
+  int* status;
+  long long wait_cycles;
+};
+
+// Instruction descriptor: 32-bit integer accumulator, signed 8-bit operands, both K-major.
+template <int MMA_M, int MMA_N>
+constexpr uint32_t kIdescI8 =
+    (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(MMA_N >> 3) << 17) | ((uint32_t)(MMA_M >> 4) << 24);
+
+template <typename T>
+__device__ __forceinline__ T round_to(float f);
+template <>
+__device__ __forceinline__ __nv_bfloat16 round_to(float f) {
+  return __float2bfloat16_rn(f);
+}
+template <>
+__device__ __forceinline__ __half round_to(float f) {
+  return __float2half_rn(f);
+}
+template <>
+__device__ __forceinline__ float round_to(float f) {
+  return f;
+}
+
+// A tile of 128 channels x BT tokens per cluster; the CTAs of the cluster (gridDim.z of them, along z)
+// share its K slices and add their sums through distributed shared memory.
+template <int BT>
+struct SmallCfg {
+  static constexpr int STAGES = BT == 32 ? 5 : BT == 64 ? 4 : 4;
+  static constexpr uint32_t W_BYTES = kRows * 128;
+  static constexpr uint32_t T_BYTES = BT * 128;
+  static constexpr uint32_t STAGE_BYTES = W_BYTES + T_BYTES;
+  // sums received from the other CTAs: this CTA's BT / splits columns from splits - 1 senders
+  static constexpr uint32_t recv_bytes(int splits) { return (uint32_t)(splits - 1) * kRows * (BT / splits) * 4; }
+  static constexpr size_t smem(int splits) { return 1024 + (size_t)STAGES * STAGE_BYTES + 256 + recv_bytes(splits); }
+};
+
+template <int BT, typename T>
+__global__ void __launch_bounds__(kThreads) int8_gemm_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tmW,
+                                                             const __grid_constant__ CUtensorMap tmT) {
+  using C = SmallCfg<BT>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = ptx::smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  const uint32_t bar0 = base + C::STAGES * C::STAGE_BYTES;
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (C::STAGES + s); };
+  const uint32_t done_bar = bar0 + 8u * (2 * C::STAGES);
+  volatile uint32_t* tmem_holder =
+      reinterpret_cast<volatile uint32_t*>(gbase + C::STAGES * C::STAGE_BYTES + 8 * (2 * C::STAGES + 1));
+  volatile int* stop = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  const uint32_t recv = bar0 + 256u;  // [sender][column / 4][channel][4] sums
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int splits = gridDim.z, rank = blockIdx.z;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      ptx::mbar_init(full_bar(s), 1);
+      ptx::mbar_init(empty_bar(s), 1);
+    }
+    ptx::mbar_init(done_bar, 1);
+    *stop = 0;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tmap(&tmW);
+    ptx::prefetch_tmap(&tmT);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t*>(tmem_holder)), BT);
+    ptx::tmem_relinquish();
+  }
+  ptx::grid_dep_launch_dependents();
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (splits > 1) ptx::cluster_sync();  // every CTA of the cluster runs before anyone stores into it
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  ptx::grid_dep_wait();  // the prologue above touched no global memory
+
+  const int n0 = blockIdx.x * kRows, m0 = blockIdx.y * BT;
+  const int s0 = (int)((long long)p.stages * rank / splits), s1 = (int)((long long)p.stages * (rank + 1) / splits);
+
+  if (warp == 0) {
+    const bool leader = ptx::elect_one();
+    int slot = 0;
+    uint32_t phase = 0;
+    for (int s = s0; s < s1; ++s) {
+      if (!wait_parity(empty_bar(slot), phase ^ 1u, stop, p.status, p.wait_cycles, 1)) break;
+      if (leader) {
+        const uint32_t sbase = base + slot * C::STAGE_BYTES, fb = full_bar(slot);
+        ptx::mbar_expect_tx(fb, C::STAGE_BYTES);
+        ptx::tma_load_2d(sbase, &tmW, s * 128, n0, fb);
+        ptx::tma_load_2d(sbase + C::W_BYTES, &tmT, s * 128, m0, fb);
+      }
+      if (++slot == C::STAGES) { slot = 0; phase ^= 1u; }
+    }
+  } else if (warp == 1) {
+    const bool leader = ptx::elect_one();
+    constexpr uint32_t kIdesc = kIdescI8<kRows, BT>;
+    int slot = 0;
+    uint32_t phase = 0, accumulate = 0;
+    bool live = true;
+    for (int s = s0; s < s1; ++s) {
+      if (!wait_parity(full_bar(slot), phase, stop, p.status, p.wait_cycles, 2)) { live = false; break; }
+      ptx::tc_fence_after();
+      const uint32_t sbase = base + slot * C::STAGE_BYTES;
+      const uint32_t w_lo = ptx::desc_lo(sbase), t_lo = ptx::desc_lo(sbase + C::W_BYTES);
+      if (leader) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          ptx::mma_i8(tmem, w_lo + j * 2, t_lo + j * 2, ptx::kDescHiSw128, kIdesc, accumulate);
+          accumulate = 1;
+        }
+        ptx::tc_commit(empty_bar(slot));
+      }
+      if (++slot == C::STAGES) { slot = 0; phase ^= 1u; }
+    }
+    if (leader && live) ptx::tc_commit(done_bar);
+  } else {
+    const int quad = warp & 3;  // tensor-memory lanes this warp may read
+    const int ch = quad * 32 + lane, n = n0 + ch;
+    const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16);
+    const bool real = n < p.N;
+    const float sb = real ? p.sb[n] : 0.f;
+    const float bias = real && p.bias ? p.bias[n] : 0.f;
+    T* out = static_cast<T*>(p.D) + n;
+    auto emit = [&](int col, int sum) {  // every lane of the warp calls it with the same column
+      const int m = m0 + col;
+      if (m < p.M && real) out[(size_t)m * p.ldd] = round_to<T>(__fmaf_rn(__fmul_rn((float)sum, p.sa[m]), sb, bias));
+    };
+    const bool ok = wait_parity(done_bar, 0, stop, p.status, p.wait_cycles, 8);
+    __syncwarp();
+    ptx::tc_fence_after();
+    if (splits == 1) {
+      const bool store = ok && !*stop;
+#pragma unroll 1
+      for (int c = 0; c < BT; c += 32) {
+        uint32_t r[32];
+        ptx::tmem_ld_32x32(taddr + c, r);
+        ptx::tmem_ld_wait();
+        if (store) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) emit(c + i, (int)r[i]);
+        }
+      }
+    } else {
+      // Column group g of this tile (BT / splits columns) is finished by CTA g: the others send it
+      // theirs, 16 bytes (four columns of a channel) at a time.
+      const int cols = BT / splits;
+      const uint32_t per_sender = (uint32_t)kRows * cols * 4;
+#pragma unroll 1
+      for (int c = 0; c < BT; c += 32) {
+        uint32_t r[32];
+        ptx::tmem_ld_32x32(taddr + c, r);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int v = 0; v < 8; ++v) {
+          const int col = c + v * 4, g = col / cols;
+          if (g != rank) {
+            const uint32_t dst = recv + (uint32_t)(rank - (rank > g)) * per_sender +
+                                 (uint32_t)((col - g * cols) >> 2) * (kRows * 16u) + (uint32_t)ch * 16u;
+            ptx::st_cluster_v4(ptx::map_to_cta(dst, (uint32_t)g), r[v * 4], r[v * 4 + 1], r[v * 4 + 2], r[v * 4 + 3]);
+          }
+        }
+      }
+    }
+  }
+
+  if (splits > 1) {
+    // every wait above is bounded, so every thread of the cluster arrives here; a CTA that gave up
+    // tells the others first, so that nobody adds sums that were never sent
+    __syncthreads();
+    if (threadIdx.x == 0 && *stop)
+      for (int g = 0; g < splits; ++g) ptx::st_cluster_u32(ptx::map_to_cta(ptx::smem_u32(const_cast<int*>(stop)), (uint32_t)g), 1u);
+    ptx::cluster_sync();
+    if (warp >= 2 && !*stop) {
+      const int quad = warp & 3, ch = quad * 32 + lane, n = n0 + ch;
+      const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16);
+      const bool real = n < p.N;
+      const float sb = real ? p.sb[n] : 0.f;
+      const float bias = real && p.bias ? p.bias[n] : 0.f;
+      T* out = static_cast<T*>(p.D) + n;
+      const int cols = BT / splits;
+      const uint32_t per_sender = (uint32_t)kRows * cols * 4;
+      for (int c = 0; c < cols; c += 4) {
+        uint32_t r[4];
+        ptx::tmem_ld_32x4(taddr + rank * cols + c, r);
+        ptx::tmem_ld_wait();
+        int sum[4] = {(int)r[0], (int)r[1], (int)r[2], (int)r[3]};
+        for (int s = 0; s < splits - 1; ++s) {
+          const uint4 a = ptx::lds_v4(recv + (uint32_t)s * per_sender + (uint32_t)(c >> 2) * (kRows * 16u) +
+                                         (uint32_t)ch * 16u);
+          sum[0] += (int)a.x;
+          sum[1] += (int)a.y;
+          sum[2] += (int)a.z;
+          sum[3] += (int)a.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int m = m0 + rank * cols + c + i;
+          if (m < p.M && real)
+            out[(size_t)m * p.ldd] = round_to<T>(__fmaf_rn(__fmul_rn((float)sum[i], p.sa[m]), sb, bias));
+        }
+      }
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  if (*stop) {
+    // give copies and MMAs that are still in flight time to land before the CTA goes away
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 1) ptx::tmem_dealloc(tmem, BT);
+}
+
+template <int BT, typename T>
+int launch_small(const Int8Params& p, const CUtensorMap& w, const CUtensorMap& t, int splits, cudaStream_t st) {
+  using C = SmallCfg<BT>;
+  auto kern = int8_gemm_kernel<BT, T>;
+  const size_t smem = C::smem(splits);
+  MG_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::smem(kMaxSplit)));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((p.N + kRows - 1) / kRows, (p.M + BT - 1) / BT, splits);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = splits;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = mg::pdl_enabled() ? 2 : 1;
+  MG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, w, t));
+  return MG_OK;
+}
+
+template <typename T>
+int launch_int8(const Int8Params& p, const int8_t* A, size_t lda, const int8_t* B, size_t ldb, int K, int sms,
+                cudaStream_t st) {
+  const mg::Options opt = mg::options();
+  int bt = p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
+  if (opt.int8_tokens == 32 || opt.int8_tokens == 64 || opt.int8_tokens == 128) bt = opt.int8_tokens;
+  const int tiles = ((p.N + kRows - 1) / kRows) * ((p.M + bt - 1) / bt);
+  int splits = 1;
+  while (splits < kMaxSplit && tiles * splits * 2 <= sms && p.stages >= splits * 4) splits *= 2;
+  if (opt.int8_split > 0) splits = opt.int8_split >= 8 ? 8 : opt.int8_split >= 4 ? 4 : opt.int8_split >= 2 ? 2 : 1;
+  while (splits > p.stages) splits /= 2;
+  if ((p.M + bt - 1) / bt > 65535) return MG_ERR_SHAPE;
+  CUtensorMap w, t;
+  int rc;
+  if ((rc = mg::make_map(&w, CU_TENSOR_MAP_DATA_TYPE_UINT8, B, K, p.N, ldb, 128, kRows))) return rc;
+  if ((rc = mg::make_map(&t, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, K, p.M, lda, 128, bt))) return rc;
+  if (bt == 32) return launch_small<32, T>(p, w, t, splits, st);
+  if (bt == 64) return launch_small<64, T>(p, w, t, splits, st);
+  return launch_small<128, T>(p, w, t, splits, st);
+}
+
+}  // namespace
+
+extern "C" int mg_matmul_int8(const int8_t* A, size_t lda, const int8_t* B, size_t ldb, const float* scale_a,
+                              const float* scale_b, const float* bias, int M, int N, int K, void* D, int dtype,
+                              size_t ldd, void* stream) {
+  if (M < 0 || N < 0 || K <= 0 || K > MG_INT8_MAX_K || dtype < 0 || dtype > 2) return MG_ERR_SHAPE;
+  // one row has no pitch: any value stands for the smallest that a tensor map takes
+  const size_t dense = ((size_t)K + 15) / 16 * 16;
+  if (M <= 1) lda = dense;
+  if (N <= 1) ldb = dense;
+  if (M <= 1) ldd = (size_t)N;
+  if (lda < (size_t)K || ldb < (size_t)K || ldd < (size_t)N) return MG_ERR_SHAPE;
+  if (lda % 16 || ldb % 16) return MG_ERR_ALIGN;
+  if (lda >= (1ull << 40) || ldb >= (1ull << 40)) return MG_ERR_SHAPE;
+  if (M == 0 || N == 0) return MG_OK;
+  if (!A || !B || !scale_a || !scale_b || !D) return MG_ERR_NULL;
+  if (!mg::aligned(A, 16) || !mg::aligned(B, 16) || !mg::aligned(scale_a, 4) || !mg::aligned(scale_b, 4) ||
+      !mg::aligned(bias, 4) || !mg::aligned(D, dtype == MG_FP32 ? 4 : 2))
+    return MG_ERR_ALIGN;
+  mg::DeviceInfo di;
+  int rc = mg::device_info(&di);
+  if (rc != MG_OK) return rc;
+  Int8Params p{};
+  p.M = M;
+  p.N = N;
+  p.stages = (K + 127) / 128;
+  p.sa = scale_a;
+  p.sb = scale_b;
+  p.bias = bias;
+  p.D = D;
+  p.ldd = ldd;
+  p.wait_cycles = mg::wait_limit_cycles();
+  if ((rc = mg::device_status_word(&p.status)) != MG_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == MG_BF16) return launch_int8<__nv_bfloat16>(p, A, lda, B, ldb, K, di.sm_count, st);
+  if (dtype == MG_FP16) return launch_int8<__half>(p, A, lda, B, ldb, K, di.sm_count, st);
+  return launch_int8<float>(p, A, lda, B, ldb, K, di.sm_count, st);
+}

@@ -46,6 +46,8 @@ struct Options {
   int fault_skip_load;  // FAULT_SKIP_LOAD: n > 0 makes the GEMM's first CTA withhold its n-th stage load
                         // (host-side fault injection for the bounded-wait test; the kernel then gives up
                         // after the wait limit and returns normally)
+  int int8_tokens;      // INT8_TOKENS: 32 / 64 / 128 / 256 forces the token tile of the 8-bit product
+  int int8_split;       // INT8_SPLIT: 1 / 2 / 4 / 8 forces the number of CTAs that share a tile's K
 };
 Options options();
 

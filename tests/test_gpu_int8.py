@@ -1,0 +1,373 @@
+"""8-bit operators on the GPU against their definitions in 64 bits.
+
+Tolerances, derived:
+  quantize_int8   every step is one correctly rounded fp32 operation, so codes and scales are equal to
+                  the same steps done by numpy in fp32.
+  rms_norm_int8   all terms of the sum of squares are positive; a thread adds at most 128 of them one
+                  after the other and ten tree levels follow: 138 roundings of 2^-24, half of that
+                  after the square root.  rsqrtf is off by 2^-22, and w u, v, 127/a, their products
+                  and a/127 add at most ten roundings: 69 + 4 + 10 < 96 units of 2^-24 = EPS_NORM.
+                  A code is then off by at most half a step plus twice 127 EPS_NORM; the scale by EPS_NORM.
+                  u is one fp32 addition and one rounding: equal to the same done by torch.
+  matmul_int8     the sum S is exact.  float(S), times sa, and the fused multiply-add with sb and the
+                  bias are three roundings: 2^-24 (2 |S sa sb| + |y|) up to second-order terms, and
+                  the result type adds eps / 2 |y|, or, below its smallest normal number, half of its
+                  smallest step: fp16 has 2^-24 between all values under 2^-14, so 2^-25 there (a sum
+                  that nearly cancels the bias lands in that range, where eps / 2 |y| is less than that).
+"""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+EPS_NORM = 96 * 2.0 ** -24
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+TINY = 2.0 ** -100
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def tokens(M, K, dtype, seed=0):
+    """Tokens of different loudness, a few loud channels; on the CPU."""
+    g = gen(seed)
+    x = torch.randn(M, K, generator=g) * torch.exp2(torch.randn(M, 1, generator=g))
+    x[:, ::37] *= 20
+    return x.to(dtype)
+
+
+def pitched(t, pitch, fill):
+    """A CUDA copy of t whose rows are `pitch` elements apart, `fill` in between; and the whole buffer."""
+    buf = torch.full((t.shape[0], pitch), fill, dtype=t.dtype, device="cuda")
+    buf[:, :t.shape[1]] = t.cuda()
+    return buf[:, :t.shape[1]], buf
+
+
+def want_codes(x):
+    """The definition, every step one fp32 operation (numpy rounds as IEEE 754 asks)."""
+    f = x.float().numpy()
+    a = np.maximum(np.abs(f).max(1, keepdims=True), np.float32(TINY))
+    q = np.rint(f * (np.float32(127) / a))
+    return q.astype(np.int8), (a / np.float32(127))[:, 0]
+
+
+# ------------------------------------------------------------------------------------- quantize_int8
+
+# a warp's row, several warps' row, one row for a whole CTA, rows that are read twice; odd lengths
+LENGTHS = [1, 2, 7, 8, 31, 64, 65, 500, 512, 1000, 1024, 1032, 1931, 4096, 8192, 14336, 16385, 32768, 40000, 131071]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K", LENGTHS)
+def test_quantise_equals_its_definition(K, dtype):
+    import mixedgemm_b200 as mg
+    for M in (1, 3, 300 if K <= 4096 else 5):
+        x = tokens(M, K, dtype, seed=K + M)
+        q, s = mg.quantize_int8(x.cuda())
+        wq, ws = want_codes(x)
+        assert q.shape == (M, K) and q.stride(0) % 16 == 0 and q.dtype == torch.int8
+        assert np.array_equal(s.cpu().numpy(), ws)
+        assert np.array_equal(q.cpu().numpy(), wq)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K, pitch, lead", [(64, 72, 0), (64, 71, 0), (64, 80, 3), (1000, 1001, 1), (1032, 1040, 8), (4096, 4097, 5)])
+def test_quantise_strided_rows_and_untouched_padding(K, pitch, lead, dtype):
+    import mixedgemm_b200 as mg
+    M = 9
+    x = tokens(M, K, dtype, seed=K)
+    flat = torch.full((lead + M * pitch,), float("nan"), dtype=dtype, device="cuda")  # padding must not be read
+    view = flat[lead:].view(M, pitch)[:, :K]
+    view.copy_(x.cuda())
+    buf = torch.full((M, K + 5), 77, dtype=torch.int8, device="cuda")  # rows at odd addresses
+    s = torch.empty(M, device="cuda")
+    q, s2 = mg.quantize_int8(view, out=(buf[:, :K], s))
+    wq, ws = want_codes(x)
+    assert s2 is s and np.array_equal(q.cpu().numpy(), wq) and np.array_equal(s.cpu().numpy(), ws)
+    assert bool((buf[:, K:] == 77).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K", [40, 65, 4096])
+def test_quantise_rows_without_a_scale(K, dtype):
+    """Zeros, values below the floor, NaN and infinities: only the row that holds them is affected."""
+    import mixedgemm_b200 as mg
+    x = tokens(7, K, dtype, seed=1)
+    x[0] = 0
+    x[1, K // 2] = float("nan")
+    x[2, K - 1] = float("-inf")
+    x[3, 0], x[3, 1] = float("inf"), float("nan")
+    x[4] = torch.finfo(dtype).tiny if dtype != torch.float16 else 2.0 ** -24
+    x[5] = -x[5].abs().amax()
+    q, s = (t.cpu() for t in mg.quantize_int8(x.cuda()))
+    good = [0, 4, 5, 6]
+    wq, ws = want_codes(x[good])
+    assert np.array_equal(q[good].numpy(), wq) and np.array_equal(s[good].numpy(), ws)
+    assert (q[0] == 0).all() and s[0] == np.float32(TINY) / np.float32(127)
+    assert (q[5] == -127).all()
+    for r in (1, 2, 3):
+        assert (q[r] == 0).all() and torch.isnan(s[r])
+
+
+# ------------------------------------------------------------------------------------- rms_norm_int8
+
+def check_norm(got, x, w, r, eps):
+    q, s, u = [t.cpu() for t in got] + ([None] if r is None else [])
+    f = x
+    if r is not None:
+        f = (x.float() + r.float()).to(x.dtype)
+        assert torch.equal(u, f)
+    f = f.double()
+    h = f * w.double() / torch.sqrt(f.pow(2).mean(1, keepdim=True) + eps)
+    a = h.abs().amax(1, keepdim=True).clamp_min(TINY)
+    t = h * 127 / a
+    assert ((s.double() - a[:, 0] / 127).abs() <= EPS_NORM * a[:, 0] / 127).all()
+    assert float((q.double() - t).abs().max()) <= 0.5 + 2 * 127 * EPS_NORM
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K", LENGTHS)
+def test_norm_against_64_bits(K, dtype):
+    import mixedgemm_b200 as mg
+    for M, residual in ((1, True), (3, False), (200 if K <= 4096 else 4, True)):
+        x, r = tokens(M, K, dtype, seed=K), tokens(M, K, dtype, seed=K + 1) if residual else None
+        w = (1 + 0.2 * torch.randn(K, generator=gen(3))).to(dtype)
+        got = mg.rms_norm_int8(x.cuda(), w.cuda(), eps=1e-5, residual=r.cuda() if residual else None)
+        assert len(got) == 2 + residual
+        check_norm(got, x, w, r, 1e-5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K, px, pr", [(64, 72, 80), (65, 67, 70), (1000, 1000, 1003), (1032, 1040, 1032), (4096, 4100, 4104)])
+def test_norm_strided_and_in_place(K, px, pr, dtype):
+    import mixedgemm_b200 as mg
+    M = 11
+    x, r = tokens(M, K, dtype, seed=5), tokens(M, K, dtype, seed=6)
+    w = (1 + 0.2 * torch.randn(K, generator=gen(4))).to(dtype)
+    xv, xb = pitched(x, px, float("nan"))
+    rv, rb = pitched(r, pr, float("nan"))
+    got = mg.rms_norm_int8(xv, w.cuda(), eps=1e-6, residual=rv, residual_out=rv)  # the stream in place
+    assert got[2] is rv
+    check_norm(got, x, w, r, 1e-6)
+    assert bool(torch.isnan(rb[:, K:].float()).all()) and torch.equal(xv.cpu(), x)
+    rv.copy_(r.cuda())
+    got = mg.rms_norm_int8(xv, w.cuda(), eps=1e-6, residual=rv, residual_out=xv)  # or over x
+    check_norm(got, x, w, r, 1e-6)
+    assert torch.equal(rv.cpu(), r) and bool(torch.isnan(xb[:, K:].float()).all())
+
+
+def test_norm_in_place_on_rows_that_are_read_twice():
+    import mixedgemm_b200 as mg
+    M, K = 2, 131071
+    x, r = tokens(M, K, torch.bfloat16, seed=5), tokens(M, K, torch.bfloat16, seed=6)
+    w = torch.ones(K, dtype=torch.bfloat16)
+    rd = r.cuda()
+    check_norm(mg.rms_norm_int8(x.cuda(), w.cuda(), eps=1e-6, residual=rd, residual_out=rd), x, w, r, 1e-6)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K", [40, 65, 4096])
+def test_norm_rows_without_a_scale(K, dtype):
+    import mixedgemm_b200 as mg
+    x = tokens(6, K, dtype, seed=2)
+    w = (1 + 0.2 * torch.randn(K, generator=gen(5))).to(dtype)
+    x[0] = 0
+    x[1, 3] = float("nan")
+    x[2, K - 1] = float("inf")
+    if dtype != torch.float16:
+        x[3] = 1e20  # the sum of squares leaves fp32
+    q, s = (t.cpu() for t in mg.rms_norm_int8(x.cuda(), w.cuda(), eps=1e-5))
+    assert (q[0] == 0).all() and s[0] == np.float32(TINY) / np.float32(127)
+    for row in (1, 2) + ((3,) if dtype != torch.float16 else ()):
+        assert (q[row] == 0).all() and torch.isnan(s[row])
+    check_norm((q[4:], s[4:]), x[4:], w, None, 1e-5)
+
+
+# --------------------------------------------------------------------------------------- matmul_int8
+
+def codes(rows, K, seed, lo=-128):
+    q = torch.randint(lo, 128, (rows, K), generator=gen(seed), dtype=torch.int16).to(torch.int8)
+    buf = torch.full((rows, (K + 15) // 16 * 16), 99, dtype=torch.int8, device="cuda")  # padding must not count
+    buf[:, :K] = q.cuda()
+    return q, buf[:, :K]
+
+
+def check_product(y, a, b, sa, sb, bias):
+    S = (a.double() @ b.double().t())  # whole numbers below 2^31: exact
+    t = S * sa.double()[:, None] * sb.double()[None, :]
+    want = t if bias is None else t + bias.double()
+    y = y.cpu()
+    tol = 2.0 ** -24 * (2 * t.abs() + want.abs()) * (1 + 2.0 ** -20)
+    if y.dtype != torch.float32:
+        half_step = torch.finfo(y.dtype).eps / 2 * want.abs() * (1 + 2.0 ** -10)
+        tol = tol + half_step.clamp_min(torch.finfo(y.dtype).smallest_normal * torch.finfo(y.dtype).eps / 2)
+    bad = (y.double() - want).abs() > tol
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[0].tolist())
+
+
+def run_product(M, N, K, dtype, with_bias, seed=0):
+    import mixedgemm_b200 as mg
+    a, av = codes(M, K, seed)
+    b, bv = codes(N, K, seed + 1)
+    g = gen(seed + 2)
+    sa, sb = torch.rand(M, generator=g) * 0.01 + 1e-3, torch.rand(N, generator=g) * 0.01 + 1e-3
+    bias = torch.randn(N, generator=g) if with_bias else None
+    y = mg.matmul_int8(av, bv, sa.cuda(), sb.cuda(), bias=None if bias is None else bias.cuda(), out_dtype=dtype)
+    assert y.shape == (M, N) and y.dtype == dtype
+    check_product(y, a, b, sa, sb, bias)
+    assert mg.device_status() == 0
+
+
+SHAPES = [(1, 1, 1), (1, 128, 128), (1, 4096, 4096), (3, 7, 16), (5, 129, 31), (32, 128, 129), (33, 300, 1000), (64, 256, 4096),
+          (65, 127, 640), (127, 130, 2048), (128, 1024, 512), (129, 1, 257), (200, 333, 1931), (300, 513, 768),
+          (513, 1000, 384), (777, 2049, 1200)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M, N, K", SHAPES)
+def test_product_against_64_bits(M, N, K, dtype):
+    run_product(M, N, K, dtype, with_bias=(M + N) % 2 == 0, seed=M + N + K)
+
+
+@pytest.mark.parametrize("tile", [32, 64, 128])
+@pytest.mark.parametrize("split", [1, 2, 4, 8])
+def test_product_of_every_tile_and_split(tile, split, mgopt):
+    mgopt.set("INT8_TOKENS", tile)
+    mgopt.set("INT8_SPLIT", split)
+    for M, N, K in ((1, 130, 1024), (37, 300, 1931), (140, 257, 4096), (300, 640, 128)):
+        run_product(M, N, K, torch.float32, with_bias=True, seed=tile + split)
+
+
+def test_product_does_not_depend_on_tile_or_split(mgopt):
+    """The sum is exact, so every form gives the same bytes."""
+    import mixedgemm_b200 as mg
+    _, av = codes(100, 2000, 1)
+    _, bv = codes(400, 2000, 2)
+    sa, sb = torch.rand(100, device="cuda"), torch.rand(400, device="cuda")
+    ref = mg.matmul_int8(av, bv, sa, sb)
+    for tile in (32, 64, 128):
+        for split in (1, 2, 4, 8):
+            mgopt.set("INT8_TOKENS", tile)
+            mgopt.set("INT8_SPLIT", split)
+            assert torch.equal(mg.matmul_int8(av, bv, sa, sb), ref)
+
+
+def test_product_of_the_longest_row_does_not_overflow():
+    import mixedgemm_b200 as mg
+    K = 131071
+    a, av = torch.full((3, K), -128, dtype=torch.int8), None
+    a[1] = 127
+    av, _ = pitched(a, 131072, 99)
+    one = torch.ones(3, device="cuda")
+    y = mg.matmul_int8(av, av, one, one, out_dtype=torch.float32)
+    check_product(y, a, a, one.cpu(), one.cpu(), None)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M, N", [(40, 130), (300, 257)])
+def test_product_into_a_view_leaves_the_rest(M, N, dtype):
+    import mixedgemm_b200 as mg
+    K = 200
+    a, av = codes(M, K, 1)
+    b, bv = codes(N, K, 2)
+    sa, sb = torch.rand(M) * 0.01, torch.rand(N) * 0.01
+    flat = torch.full((1 + (M + 1) * (N + 3),), 7.0, dtype=dtype, device="cuda")  # odd base, odd pitch
+    buf = flat[1:].view(M + 1, N + 3)
+    out = buf[:M, :N]
+    assert mg.matmul_int8(av, bv, sa.cuda(), sb.cuda(), out=out) is out
+    check_product(out, a, b, sa, sb, None)
+    assert bool((buf[:, N:] == 7).all()) and bool((buf[M:] == 7).all()) and flat[0] == 7
+
+
+def test_product_of_nothing():
+    import mixedgemm_b200 as mg
+    q = lambda r: torch.zeros(r, 32, dtype=torch.int8, device="cuda")
+    s = lambda r: torch.ones(r, device="cuda")
+    assert mg.matmul_int8(q(0), q(5), s(0), s(5)).shape == (0, 5)
+    assert mg.matmul_int8(q(4), q(0), s(4), s(0)).shape == (4, 0)
+    assert mg.quantize_int8(torch.zeros(0, 32, device="cuda"))[0].shape == (0, 32)
+    x = torch.zeros(0, 32, device="cuda")
+    assert mg.rms_norm_int8(x, torch.ones(32, device="cuda"), residual=x)[2].shape == (0, 32)
+
+
+def test_a_bad_token_spoils_its_own_row_only():
+    import mixedgemm_b200 as mg
+    x = tokens(40, 256, torch.bfloat16)
+    x[17, 5] = float("nan")
+    q, s = mg.quantize_int8(x.cuda())
+    b, bv = codes(130, 256, 2)
+    sb = torch.rand(130) * 0.01
+    y = mg.matmul_int8(q, bv, s, sb.cuda())
+    assert bool(torch.isnan(y[17]).all())
+    keep = [i for i in range(40) if i != 17]
+    check_product(y[keep], q[keep].cpu(), b, s[keep].cpu(), sb, None)
+
+
+def test_refusals():
+    import mixedgemm_b200 as mg
+    x = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
+    w, q = torch.ones(64, dtype=torch.bfloat16, device="cuda"), torch.zeros(4, 64, dtype=torch.int8, device="cuda")
+    s = torch.ones(4, device="cuda")
+    bad = [
+        lambda: mg.quantize_int8(x.double()), lambda: mg.quantize_int8(x[0]), lambda: mg.quantize_int8(x.t()),
+        lambda: mg.quantize_int8(x[:1].expand(4, 64)), lambda: mg.quantize_int8(x[:, ::2]),
+        lambda: mg.quantize_int8(x, out=(q[:3], s)), lambda: mg.quantize_int8(x, out=(q, s[:3])),
+        lambda: mg.quantize_int8(x, out=(q.int(), s)), lambda: mg.quantize_int8(torch.zeros(2, 0, device="cuda")),
+        lambda: mg.rms_norm_int8(x, w.float()), lambda: mg.rms_norm_int8(x, w[:32]), lambda: mg.rms_norm_int8(x, w, eps=-1.0),
+        lambda: mg.rms_norm_int8(x, w, residual=x[:2]), lambda: mg.rms_norm_int8(x, w, residual=x.float()),
+        lambda: mg.rms_norm_int8(x, w, residual_out=x), lambda: mg.rms_norm_int8(x, w, residual=x, residual_out=x[:1].expand(4, 64)),
+        lambda: mg.matmul_int8(q, q[:, :32], s, s), lambda: mg.matmul_int8(q, q, s[:3], s), lambda: mg.matmul_int8(q, q, s, s.half()),
+        lambda: mg.matmul_int8(q, q, s, s, bias=s.bfloat16()), lambda: mg.matmul_int8(q.view(torch.uint8), q, s, s),
+        lambda: mg.matmul_int8(q, q, s, s, out_dtype=torch.float64), lambda: mg.matmul_int8(q, q, s, s, out=x[:, :4].t()),
+        lambda: mg.matmul_int8(q[:, :40].contiguous(), q[:, :40], s, s), lambda: mg.matmul_int8(q[:, 1:33], q[:, :32], s, s),
+        lambda: mg.matmul_int8(q, q, s, s, out=x[:, :4], out_dtype=torch.float16),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail("case %d was not refused" % i)
+    torch.cuda.synchronize()
+
+
+def test_norm_then_product_on_a_side_stream_and_in_two_graphs():
+    """The operators as a layer runs them, on another stream, and captured twice on one stream and
+    replayed at the same time on two: no call keeps anything from one to the next."""
+    import mixedgemm_b200 as mg
+    M, N, K = 24, 600, 4096
+    w = (1 + 0.2 * torch.randn(K, generator=gen(4))).to(torch.bfloat16).cuda()
+    bq, sb = mg.quantize_int8((torch.randn(N, K, generator=gen(5)) * 0.02).cuda())
+
+    def layer(x, r):
+        q, s, u = mg.rms_norm_int8(x, w, residual=r)
+        return mg.matmul_int8(q, bq, s, sb), u
+
+    xs = [tokens(M, K, torch.bfloat16, seed=i).cuda() for i in range(4)]
+    want = [layer(xs[i], xs[3 - i]) for i in range(4)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = layer(xs[0], xs[3])
+    side.synchronize()
+    assert torch.equal(got[0], want[0][0]) and torch.equal(got[1], want[0][1])
+    ins = [[xs[0].clone(), xs[3].clone()], [xs[1].clone(), xs[2].clone()]]
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(layer(*ins[i]))
+        graphs.append(g)
+    ins[0][0].copy_(xs[2]), ins[0][1].copy_(xs[1])
+    ins[1][0].copy_(xs[3]), ins[1][1].copy_(xs[0])
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        with torch.cuda.stream(side):
+            graphs[0].replay()
+        with torch.cuda.stream(other):
+            graphs[1].replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(outs[i][0], want[2 + i][0]) and torch.equal(outs[i][1], want[2 + i][1])
+    assert mg.device_status() == 0

@@ -1,0 +1,72 @@
+"""8-bit operators: what is refused, checked without a GPU (the C entry points answer shape, null and
+alignment errors before any CUDA call; the Python layer refuses tensors that are not on a GPU)."""
+import pytest
+import torch
+
+OK, SHAPE, NULL, ALIGN = 0, 1, 2, 3
+P = 4096        # stands for an aligned device pointer: never dereferenced, the call is refused first
+MAX_K = 131071
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from mixedgemm_b200 import build, _capi
+    build.build_lib()
+    return _capi.load()
+
+
+def quantise(lib, X=P, dtype=0, M=4, K=64, ldx=64, Q=P, ldq=64, S=P):
+    return lib.mg_quantize_int8(X, dtype, M, K, ldx, Q, ldq, S, None)
+
+
+@pytest.mark.parametrize("want, args", [
+    (OK, dict(M=0, X=None, Q=None, S=None)),
+    (SHAPE, dict(M=-1)), (SHAPE, dict(K=0)), (SHAPE, dict(K=MAX_K + 1, ldx=1 << 20, ldq=1 << 20)),
+    (SHAPE, dict(dtype=3)), (SHAPE, dict(dtype=-1)), (SHAPE, dict(ldx=63)), (SHAPE, dict(ldq=63)),
+    (NULL, dict(X=None)), (NULL, dict(Q=None)), (NULL, dict(S=None)),
+    (ALIGN, dict(X=P + 1)), (ALIGN, dict(dtype=2, X=P + 2)), (ALIGN, dict(S=P + 2)),
+])
+def test_quantise_refusals(lib, want, args):
+    assert quantise(lib, **args) == want
+
+
+def norm(lib, X=P, R=None, W=P, eps=1e-6, dtype=0, M=4, K=64, ldx=64, ldr=0, U=None, ldu=0, Q=P, ldq=64, S=P):
+    return lib.mg_rms_norm_int8(X, R, W, eps, dtype, M, K, ldx, ldr, U, ldu, Q, ldq, S, None)
+
+
+@pytest.mark.parametrize("want, args", [
+    (OK, dict(M=0, X=None, W=None, Q=None, S=None)),
+    (SHAPE, dict(M=-1)), (SHAPE, dict(K=0)), (SHAPE, dict(K=MAX_K + 1, ldx=1 << 20, ldq=1 << 20)), (SHAPE, dict(dtype=3)),
+    (SHAPE, dict(eps=-1e-6)), (SHAPE, dict(eps=float("nan"))), (SHAPE, dict(eps=float("inf"))),
+    (SHAPE, dict(R=P, U=P, ldr=63, ldu=64)), (SHAPE, dict(R=P, U=P, ldr=64, ldu=63)),
+    (NULL, dict(W=None)), (NULL, dict(R=P, ldr=64, ldu=64)), (NULL, dict(U=P, ldu=64)),
+    (ALIGN, dict(W=P + 1)), (ALIGN, dict(R=P + 1, U=P, ldr=64, ldu=64)), (ALIGN, dict(R=P, U=P + 1, ldr=64, ldu=64)),
+])
+def test_norm_refusals(lib, want, args):
+    assert norm(lib, **args) == want
+
+
+def product(lib, A=P, lda=64, B=P, ldb=64, sa=P, sb=P, bias=None, M=4, N=8, K=64, D=P, dtype=0, ldd=8):
+    return lib.mg_matmul_int8(A, lda, B, ldb, sa, sb, bias, M, N, K, D, dtype, ldd, None)
+
+
+@pytest.mark.parametrize("want, args", [
+    (OK, dict(M=0, A=None, D=None)), (OK, dict(N=0, B=None, D=None)),
+    (SHAPE, dict(M=-1)), (SHAPE, dict(N=-1)), (SHAPE, dict(K=0)), (SHAPE, dict(K=MAX_K + 1, lda=1 << 20, ldb=1 << 20)),
+    (SHAPE, dict(dtype=3)), (SHAPE, dict(lda=48)), (SHAPE, dict(ldb=48)), (SHAPE, dict(ldd=7)),
+    (SHAPE, dict(lda=1 << 40)), (SHAPE, dict(ldb=1 << 40)),
+    (ALIGN, dict(lda=72)), (ALIGN, dict(ldb=65)), (ALIGN, dict(A=P + 8)), (ALIGN, dict(B=P + 1)), (ALIGN, dict(sa=P + 2)),
+    (ALIGN, dict(sb=P + 1)), (ALIGN, dict(bias=P + 2)), (ALIGN, dict(D=P + 1)), (ALIGN, dict(D=P + 2, dtype=2)),
+    (NULL, dict(A=None)), (NULL, dict(B=None)), (NULL, dict(sa=None)), (NULL, dict(sb=None)), (NULL, dict(D=None)),
+])
+def test_product_refusals(lib, want, args):
+    assert product(lib, **args) == want
+
+
+def test_python_layer_refuses_tensors_off_the_gpu(lib):
+    import mixedgemm_b200 as mg
+    x, q, s = torch.zeros(2, 32), torch.zeros(2, 32, dtype=torch.int8), torch.ones(2)
+    for call in (lambda: mg.quantize_int8(x), lambda: mg.rms_norm_int8(x, torch.ones(32)),
+                 lambda: mg.matmul_int8(q, q, s, s)):
+        with pytest.raises(RuntimeError, match="CUDA tensor"):
+            call()
