@@ -428,6 +428,19 @@ int mg_rms_norm_int8(const void* X, const void* R, const void* W, float eps, int
                      size_t ldr, void* U, size_t ldu, int8_t* Q, size_t ldq, float* scale, void* stream);
 
 /*
+ * The same norm in front of the MX split: u = bf16(X + R) as above, h = bf16(u * W / sqrt(mean_k u^2 + eps)),
+ * then what mg_reorder_quantize_pitched writes for h, byte for byte.
+ *   X, R, U [M,K] bf16, rows ldx / ldr / ldu elements apart (multiples of 8), W [K] bf16, all 16-byte aligned;
+ *   R and U both NULL without a residual, U may be R or X itself; idx ... SF8 as in mg_reorder_quantize_pitched.
+ * A row whose sum of squares is not a finite fp32 number, or that holds an h that is not finite, gets
+ * scale bytes 255 (NaN), so that its row of a product is NaN.
+ */
+int mg_rms_norm_reorder_quantize(const void* X, size_t ldx, const void* R, size_t ldr, const void* W, float eps,
+                                 void* U, size_t ldu, int M, int K, const int16_t* idx, int KN, int KS, int KO,
+                                 uint8_t* C4, uint8_t* C6, uint8_t* C8, const size_t* pitches, uint8_t* SF4,
+                                 uint8_t* SF6, uint8_t* SF8, void* stream);
+
+/*
  * D[m,n] = (sum_k A[m,k] B[n,k]) * scale_a[m] * scale_b[n] + bias[n], the sum exact in 32-bit integers,
  * the rest in fp32, rounded once to `dtype`.
  *   A [M,K], B [N,K] int8, rows lda / ldb bytes apart: base and pitch multiples of 16 bytes, bytes

@@ -62,6 +62,8 @@ PROTOTYPES = {
     "mg_matmul_fp8": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "mg_quantize_int8": (_i, [_vp, _i, _i, _i, _sz, _vp, _sz, _vp, _vp]),
     "mg_rms_norm_int8": (_i, [_vp, _vp, _vp, ctypes.c_float, _i, _i, _i, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp]),
+    "mg_rms_norm_reorder_quantize": (_i, [_vp, _sz, _vp, _sz, _vp, ctypes.c_float, _vp, _sz, _i, _i, _vp, _i, _i, _i] +
+                                     [_vp] * 4 + [_vp] * 3 + [_vp]),
     "mg_matmul_int8": (_i, [_vp, _sz, _vp, _sz, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _sz, _vp]),
 }
 

@@ -484,6 +484,42 @@ def rms_norm_int8(X, weight, eps=1e-6, residual=None, residual_out=None, out=Non
     return (q, scale) if u is None else (q, scale, u)
 
 
+def rms_norm_reorder_quantize_x(X, weight, reorder_index, KN, KS, KO, eps=1e-6, residual=None, residual_out=None,
+                                out=None):
+    """reorder_quantize_x of the root-mean-square norm of X [M,K] bf16 (+ residual), in one launch:
+    u = bf16(X + residual), h = bf16(u * weight / sqrt(mean(u^2) + eps)).  Returns the six tensors that
+    reorder_quantize_x(h, ...) returns, byte for byte, and with a residual u as a seventh.  residual_out
+    may be `residual` (or X) itself; `out` the six buffers of alloc_quantized_x().  Rows start on
+    16-byte boundaries.  A row with a sum of squares or an h that is not finite gets NaN scales."""
+    what = "rms_norm_reorder_quantize_x"
+    ldx, ldr, u, ldu = _norm_inputs(X, weight, residual, residual_out, what)
+    M, K = X.shape
+    if X.dtype != torch.bfloat16:
+        raise RuntimeError("%s: X must be bfloat16, not %s" % (what, X.dtype))
+    if K != KN + KS + KO:
+        raise RuntimeError("%s: K = %d does not match KN+KS+KO" % (what, K))
+    dev = X.device
+    _vector(reorder_index, what, "reorder_index", K, dev, torch.int16)
+    if out is None:
+        out = alloc_quantized_x(M, KN, KS, KO, dev)
+    else:
+        lib = _capi.load()
+        _check_codes(out[:3], what)
+        for t, n in zip(out[:3], (KN // 2, KS // 4 * 3, KO)):
+            if tuple(t.shape) != (M, n) or t.device != dev:
+                raise RuntimeError("%s: a code buffer has shape %s where %s is expected" % (what, tuple(t.shape), (M, n)))
+        for t, k in zip(out[3:], (KN, KS, KO)):
+            if t.numel() < lib.mg_sf_bytes(M, k) or t.device != dev or t.dtype != torch.uint8 or not t.is_contiguous():
+                raise RuntimeError("%s: a scale buffer is too small or on another device" % what)
+    XN, XS, XO, s4, s6, s8 = out
+    st = _on(dev, _capi.load().mg_rms_norm_reorder_quantize, X.data_ptr(), ldx, None if u is None else residual.data_ptr(),
+             ldr, weight.data_ptr(), eps, None if u is None else u.data_ptr(), ldu, M, K, reorder_index.data_ptr(), KN, KS,
+             KO, _ptr(XN), _ptr(XS), _ptr(XO), _pitches((XN, XS, XO)), _ptr(s4), _ptr(s6), _ptr(s8))
+    if st:
+        _capi.check(st, what)
+    return tuple(out) if u is None else tuple(out) + (u,)
+
+
 def matmul_int8(A, B, scale_a, scale_b, bias=None, out=None, out_dtype=None):
     """A [M,K] int8 (tokens) times B [N,K] int8 (channels), both with a scale per row:
     (A @ B^T, exact in 32-bit integers) * scale_a[:, None] * scale_b[None, :] + bias, rounded once to

@@ -117,9 +117,10 @@ __device__ __forceinline__ float scale_round(float x, float rs) {
   return __uint_as_float(__float_as_uint(r) | (__float_as_uint(x) & 0x80000000u));
 }
 
-// One (row, group): gather, scale, quantise, pack, store.
+// One (row, group): gather, scale, quantise, pack, store.  nan_row: the scale is NaN, whatever the values.
 template <bool WEIGHTS>
-__device__ __forceinline__ void quantise_group(const ReorderParams& p, const RowCtx& rc, uint32_t idx2_addr, int g) {
+__device__ __forceinline__ void quantise_group(const ReorderParams& p, const RowCtx& rc, uint32_t idx2_addr, int g,
+                                               bool nan_row = false) {
   float x[32];
   float maxv = 0.f;
 #pragma unroll
@@ -142,7 +143,7 @@ __device__ __forceinline__ void quantise_group(const ReorderParams& p, const Row
   const SegOut so = seg == 0 ? p.seg[0] : (seg == 1 ? p.seg[1] : p.seg[2]);
 
   const int sf = scale_byte(maxv, fmt);
-  so.sf[rc.sf_row + (gs & 3) + (size_t)(gs >> 2) * 512 + (size_t)rc.row_blk * 512 * so.katoms] = (uint8_t)sf;
+  so.sf[rc.sf_row + (gs & 3) + (size_t)(gs >> 2) * 512 + (size_t)rc.row_blk * 512 * so.katoms] = (uint8_t)(nan_row ? 255 : sf);
   const float rs = __uint_as_float(((unsigned)(254 - sf) << 23) | 0x800u);  // 2^(127-sf) * (1 + 2^-12)
 
 #pragma unroll
@@ -353,6 +354,143 @@ __global__ void __launch_bounds__(kThreads, 1) reorder_quantize_multi_kernel(con
   }
 }
 
+// ---------------------------------------------------------------- behind a root-mean-square norm
+// u = bf16(x + r), h = bf16((u w) rsqrt(mean u^2 + eps)), then the codes and scales of h as above.
+//
+// A CTA takes R rows at a time.  kNormWarps / R warps share a row: they read it (and the residual)
+// once in 16-byte vectors, write u to the stream and to shared memory, add up u^2, and turn u into h
+// in place; then all threads quantise the R rows of the tile with the lanes of a warp walking the
+// rows of a group, as in the kernel above.  A row with a sum or a value that is not finite gets NaN
+// scales.  The phases of one CTA alternate; what overlaps loads with
+// arithmetic is that several CTAs share an SM.  The index stays in shared memory for the life of the CTA.
+// Bound: bytes (2 read + 0.63 written per element, 6 + 0.63 with a residual).
+constexpr int kNormWarps = 8;
+constexpr int kNormThreads = kNormWarps * 32;
+
+struct NormParams {
+  ReorderParams q;
+  const uint16_t* R;  // residual, or null
+  uint16_t* U;        // the stream after the addition (with R only)
+  const uint16_t* W;
+  size_t px, pr, pu;  // row pitches in elements
+  float eps;
+};
+
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int R>
+__global__ void __launch_bounds__(kNormThreads) norm_reorder_kernel(const __grid_constant__ NormParams np) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float s_sum[kNormWarps];
+  __shared__ int s_bad[R];
+  constexpr int kWarpsPerRow = kNormWarps / R;
+  const ReorderParams& p = np.q;
+  const int K = p.K, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int pitch = 2 * K + kRowSkew;
+  uint16_t* idx2 = reinterpret_cast<uint16_t*>(smem);
+  uint8_t* tile = smem + 2 * K;  // K is a multiple of 32
+  ptx::grid_dep_launch_dependents();
+  ptx::grid_dep_wait();
+  for (int i = tid; i < K; i += kNormThreads) {
+    const unsigned v = (uint16_t)p.idx[i];
+    idx2[i] = (uint16_t)(min(v, (unsigned)(K - 1)) * 2);
+  }
+  const uint32_t idx2_addr = ptx::smem_u32(idx2);
+  const int nv = K >> 3, G = K >> 5;
+  const int my_row = warp / kWarpsPerRow, my_lane = (warp % kWarpsPerRow) * 32 + lane;
+  constexpr int kLanes = kWarpsPerRow * 32;
+  const int r = tid % R, g0 = tid / R;
+
+  const unsigned rows = (unsigned)p.rows;
+  for (unsigned row0 = blockIdx.x * R; row0 < rows; row0 += gridDim.x * R) {
+    const unsigned row = row0 + my_row;
+    uint4* srow = reinterpret_cast<uint4*>(tile + (size_t)my_row * pitch);
+    float sum = 0.f;
+    if (my_lane == 0) s_bad[my_row] = 0;
+    if (row < rows) {
+      const uint4* x = reinterpret_cast<const uint4*>(p.X + (size_t)row * np.px);
+      const uint4* res = np.R ? reinterpret_cast<const uint4*>(np.R + (size_t)row * np.pr) : nullptr;
+      uint4* out = np.R ? reinterpret_cast<uint4*>(np.U + (size_t)row * np.pu) : nullptr;
+      for (int i = my_lane; i < nv; i += kLanes) {
+        uint4 a = x[i];
+        uint32_t w[4] = {a.x, a.y, a.z, a.w};
+        if (res) {
+          const uint4 b = res[i];
+          const uint32_t t[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = bf16_pair(bf16_lo(w[k]) + bf16_lo(t[k]), bf16_hi(w[k]) + bf16_hi(t[k]));
+          out[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          sum = fmaf(bf16_lo(w[k]), bf16_lo(w[k]), sum);
+          sum = fmaf(bf16_hi(w[k]), bf16_hi(w[k]), sum);
+        }
+        srow[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if constexpr (kWarpsPerRow > 1) {
+      if (lane == 0) s_sum[warp] = sum;
+      __syncthreads();
+      sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWarpsPerRow; ++i) sum += s_sum[my_row * kWarpsPerRow + i];
+    }
+    __syncwarp();
+    const float v = rsqrtf(sum / (float)K + np.eps);
+    if (row < rows) {
+      bool bad = !(sum <= 3.4028235e38f);
+      const uint4* wt = reinterpret_cast<const uint4*>(np.W);
+      for (int i = my_lane; i < nv; i += kLanes) {  // the vectors this thread wrote
+        const uint4 a = srow[i], b = __ldg(wt + i);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w}, t[4] = {b.x, b.y, b.z, b.w};
+        uint32_t h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          h[k] = bf16_pair(bf16_lo(w[k]) * bf16_lo(t[k]) * v, bf16_hi(w[k]) * bf16_hi(t[k]) * v);
+          bad = bad || (h[k] & 0x7F80u) == 0x7F80u || (h[k] & 0x7F800000u) == 0x7F800000u;
+        }
+        srow[i] = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+      if (bad) s_bad[my_row] = 1;
+    }
+    __syncthreads();
+    const unsigned qrow = row0 + r;
+    if (qrow < rows) {
+      RowCtx rc;
+      rc.smem_row = ptx::smem_u32(tile) + r * pitch;
+      rc.sf_row = (qrow & 31) * 16 + ((qrow >> 5) & 3) * 4;
+      rc.row_blk = qrow >> 7;
+      rc.row = qrow;
+      const bool nan_row = s_bad[r];
+      for (int g = g0; g < G; g += kNormThreads / R) quantise_group<false>(p, rc, idx2_addr, g, nan_row);
+    }
+    __syncthreads();
+  }
+}
+
+size_t norm_smem_bytes(int K, int R) { return (size_t)2 * K + (size_t)R * (2 * K + kRowSkew); }
+
+template <int R>
+int launch_norm(const NormParams& np, const mg::DeviceInfo& di, cudaStream_t st) {
+  auto kern = norm_reorder_kernel<R>;
+  const size_t smem = norm_smem_bytes(np.q.K, R);
+  if (smem > 48 * 1024) MG_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const int tiles = (np.q.rows + R - 1) / R;
+  int per_sm = (int)((size_t)di.smem_optin / (smem + 1024));
+  per_sm = per_sm < 1 ? 1 : per_sm > 4 ? 4 : per_sm;
+  const int most = di.sm_count * per_sm;
+  MG_CUDA_TRY(mg::launch_kernel(kern, dim3(tiles < most ? tiles : most), dim3(kNormThreads), smem, st, np));
+  return MG_OK;
+}
+
 size_t smem_bytes(int K, int R, int S) {
   return (size_t)((2 * K + 15) & ~15) + (size_t)S * R * (2 * K + kRowSkew) + 16 * 8 + 16;
 }
@@ -556,4 +694,40 @@ extern "C" size_t mg_code_pitch(int weights, int segment, int kseg) {
   const int kp = (kseg + 127) / 128 * 128;
   if (segment == 0 || weights) return (size_t)kp / 2;
   return segment == 1 ? (size_t)kp / 4 * 3 : (size_t)kp;
+}
+
+extern "C" int mg_rms_norm_reorder_quantize(const void* X, size_t ldx, const void* R, size_t ldr, const void* W, float eps,
+                                            void* U, size_t ldu, int M, int K, const int16_t* idx, int KN, int KS, int KO,
+                                            uint8_t* C4, uint8_t* C6, uint8_t* C8, const size_t* pitches, uint8_t* SF4,
+                                            uint8_t* SF6, uint8_t* SF8, void* stream) {
+  NormParams np{};
+  if (!(eps >= 0.f && eps <= 3.4028235e38f)) return MG_ERR_SHAPE;
+  if (M > 0) {
+    if (!W || (R != nullptr) != (U != nullptr)) return MG_ERR_NULL;
+    if (M == 1) ldx = ldr = ldu = (size_t)(K > 0 ? K : 0);  // one row has no pitch
+    if (ldx < (size_t)K || (R && (ldr < (size_t)K || ldu < (size_t)K))) return MG_ERR_SHAPE;
+    if (!mg::aligned(W, 16) || !mg::aligned(R, 16) || !mg::aligned(U, 16)) return MG_ERR_ALIGN;
+    if (ldx % 8 || (R && (ldr % 8 || ldu % 8))) return MG_ERR_ALIGN;
+  }
+  int rc = fill_params(false, X, M, K, idx, KN, KS, KO, C4, C6, C8, pitches, SF4, SF6, SF8, &np.q);
+  if (rc != MG_OK || np.q.rows == 0) return rc;
+  np.R = static_cast<const uint16_t*>(R);
+  np.U = static_cast<uint16_t*>(U);
+  np.W = static_cast<const uint16_t*>(W);
+  np.px = ldx;
+  np.pr = ldr;
+  np.pu = ldu;
+  np.eps = eps;
+  mg::DeviceInfo di;
+  if ((rc = mg::device_info(&di)) != MG_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // more rows to a tile leave fewer bank conflicts in the gather; fewer fill the SMs
+  int rows = 8;
+  while (rows > 1 && ((M + rows - 1) / rows < 2 * di.sm_count || norm_smem_bytes(K, rows) > (size_t)di.smem_optin / 2)) rows /= 2;
+  switch (rows) {
+    case 8: return launch_norm<8>(np, di, st);
+    case 4: return launch_norm<4>(np, di, st);
+    case 2: return launch_norm<2>(np, di, st);
+    default: return launch_norm<1>(np, di, st);
+  }
 }

@@ -7,7 +7,7 @@ kind; in deployment the weight side is done once.  `QuantizedWeights` holds what
 and can be saved / loaded; `MixedLinear` owns one or several of them that share an input
 (q/k/v, gate/up) and launches them as one grouped GEMM.
 """
-from typing import List
+from typing import List, Optional
 
 import torch
 
@@ -105,6 +105,23 @@ class QuantizedWeights:
         return cls.from_state(torch.load(path, map_location="cpu"), device)
 
 
+def _norm_weight(w, K, dtype):
+    """The weight of a module's norm: None, or a contiguous vector of K elements (in `dtype`, if given)."""
+    if w is None:
+        return None
+    if w.dim() != 1 or w.numel() != K:
+        raise ValueError("norm_weight must be a vector of in_features elements")
+    return (w if dtype is None else w.to(dtype)).detach().contiguous()
+
+
+def _residual_rows(residual, x):
+    if residual is None:
+        return None
+    if residual.shape != x.shape:
+        raise ValueError("the residual must have x's shape")
+    return residual.reshape(-1, x.shape[-1]).contiguous()
+
+
 # ----------------------------------------------------------------------------- custom op
 # quantise -> grouped GEMM as ONE torch operator, so that the module below is an ordinary op to
 # torch's dispatcher (autograd-free inference graphs, stream capture, fake-tensor tracing): every
@@ -125,6 +142,10 @@ def mixed_linear(x: torch.Tensor, reorder_index: torch.Tensor, split: List[int],
     KN, KS, KO = split
     M = x.size(0)
     A = api.reorder_quantize_x(x, reorder_index, KN, KS, KO, M, 0, out=tuple(act_scratch))
+    return _products(A, M, weight_parts, fused_parts)
+
+
+def _products(A, M, weight_parts, fused_parts):
     Bs = [tuple(weight_parts[6 * j:6 * j + 6]) for j in range(len(weight_parts) // 6)]
     if M <= 128 and len(fused_parts) == 6 and len(Bs) > 1:
         F = fused_parts
@@ -136,10 +157,31 @@ def mixed_linear(x: torch.Tensor, reorder_index: torch.Tensor, split: List[int],
 
 @mixed_linear.register_fake
 def _(x, reorder_index, split, weight_parts, fused_parts, act_scratch):
+    return _products_fake(x, weight_parts, fused_parts)
+
+
+def _products_fake(x, weight_parts, fused_parts):
     n = len(weight_parts) // 6
     if x.size(0) <= 128 and len(fused_parts) == 6 and n > 1:
         return [x.new_empty((x.size(0), fused_parts[0].size(0)))]
     return [x.new_empty((x.size(0), weight_parts[6 * j].size(0))) for j in range(n)]
+
+
+# the same behind a root-mean-square norm: its last output is the stream after the residual's addition
+# (one element when there is no residual)
+@torch.library.custom_op("mixedgemm_b200::mixed_norm_linear", mutates_args=("act_scratch",))
+def mixed_norm_linear(x: torch.Tensor, residual: Optional[torch.Tensor], norm_weight: torch.Tensor, eps: float,
+                      reorder_index: torch.Tensor, split: List[int], weight_parts: List[torch.Tensor],
+                      fused_parts: List[torch.Tensor], act_scratch: List[torch.Tensor]) -> List[torch.Tensor]:
+    KN, KS, KO = split
+    A = api.rms_norm_reorder_quantize_x(x, norm_weight, reorder_index, KN, KS, KO, eps=eps, residual=residual,
+                                        out=tuple(act_scratch))
+    return _products(A[:6], x.size(0), weight_parts, fused_parts) + [A[6] if residual is not None else x.new_empty(1)]
+
+
+@mixed_norm_linear.register_fake
+def _(x, residual, norm_weight, eps, reorder_index, split, weight_parts, fused_parts, act_scratch):
+    return _products_fake(x, weight_parts, fused_parts) + [x.new_empty(x.shape if residual is not None else (1,))]
 
 
 class MixedLinear(torch.nn.Module):
@@ -147,9 +189,13 @@ class MixedLinear(torch.nn.Module):
 
     forward(x) quantises x once (reorder index and split of the weights) and multiplies it with
     every weight in one grouped launch where the kernel takes the shapes; returns one tensor, or
-    a list when the module holds several weights."""
+    a list when the module holds several weights.
 
-    def __init__(self, weights, bias=None, max_tokens=None):
+    With norm_weight the module takes the root-mean-square norm in front of the projections with it:
+    forward(x, residual) normalises x + residual in the quantiser's launch and returns
+    (outputs, x + residual), forward(x) normalises x and returns the outputs."""
+
+    def __init__(self, weights, bias=None, max_tokens=None, norm_weight=None, eps=1e-6):
         """weights: one QuantizedWeights or several that share an input; bias: None, or one bf16
         [N_j] tensor (or None) per weight, added to the bf16 product; max_tokens: when given, the
         buffers for the quantised activation are allocated now for that many rows (forward then
@@ -181,6 +227,7 @@ class MixedLinear(torch.nn.Module):
         self._a = None
         if max_tokens is not None:
             self._a = api.alloc_quantized_x(int(max_tokens), *self.split, self.reorder_index.device)
+        self.norm_weight, self.eps = _norm_weight(norm_weight, w0.in_features, torch.bfloat16), float(eps)
 
     @classmethod
     def from_dense(cls, Ws, calibration_x):
@@ -201,12 +248,20 @@ class MixedLinear(torch.nn.Module):
         lib_sf = [api.sf_bytes(M, k) for k in self.split]
         return [self._a[i][:M] for i in range(3)] + [self._a[3 + i][:max(lib_sf[i], 1)] for i in range(3)]
 
-    def forward(self, x):
+    def forward(self, x, residual=None):
         lead = x.shape[:-1]
         x2 = x.reshape(-1, x.shape[-1]).contiguous()
         M = x2.size(0)
-        outs = torch.ops.mixedgemm_b200.mixed_linear(x2, self.reorder_index, list(self.split), self._parts,
-                                                     self._fused_parts, self._scratch(M, x2.device))
+        stream = None
+        if self.norm_weight is None:
+            if residual is not None:
+                raise ValueError("a residual needs a module with norm_weight")
+            outs = torch.ops.mixedgemm_b200.mixed_linear(x2, self.reorder_index, list(self.split), self._parts,
+                                                         self._fused_parts, self._scratch(M, x2.device))
+        else:
+            *outs, stream = torch.ops.mixedgemm_b200.mixed_norm_linear(
+                x2, _residual_rows(residual, x), self.norm_weight, self.eps, self.reorder_index, list(self.split),
+                self._parts, self._fused_parts, self._scratch(M, x2.device))
         if len(outs) != len(self.weights):  # the decode path: one product over the concatenated weight
             Y, outs, n0 = outs[0], [], 0
             for w in self.weights:
@@ -214,4 +269,140 @@ class MixedLinear(torch.nn.Module):
                 n0 += w.out_features
         outs = [o if b_ is None else o + b_.to(o.device) for o, b_ in zip(outs, self.bias)]
         outs = [o.reshape(*lead, o.size(-1)) for o in outs]
-        return outs[0] if len(outs) == 1 else outs
+        outs = outs[0] if len(outs) == 1 else outs
+        return outs if residual is None else (outs, stream.reshape(x.shape))
+
+
+# ----------------------------------------------------------------------------- 8-bit integers
+class Int8Weights:
+    """8-bit weights of one projection: codes int8 [N, K] and a scale for each output channel."""
+
+    def __init__(self, codes, scale):
+        self.codes, self.scale = codes, scale
+
+    @property
+    def out_features(self):
+        return self.codes.size(0)
+
+    @property
+    def in_features(self):
+        return self.codes.size(1)
+
+    @classmethod
+    def from_dense(cls, W):
+        """Quantise a [N, K] weight (bf16, fp16 or fp32) on its device."""
+        return cls(*api.quantize_int8(W))
+
+    @classmethod
+    def cat(cls, weights):
+        """One weight whose rows are the rows of `weights` in order.  The inputs are re-pointed at row
+        ranges of the new buffers, so nothing is held twice."""
+        K = weights[0].in_features
+        if any(w.in_features != K for w in weights):
+            raise ValueError("weights to concatenate must have the same in_features")
+        N, dev = sum(w.out_features for w in weights), weights[0].codes.device
+        whole = cls(torch.empty_strided((N, K), ((K + 15) // 16 * 16, 1), dtype=torch.int8, device=dev),
+                    torch.empty(N, dtype=torch.float32, device=dev))
+        n0 = 0
+        for w in weights:
+            n1 = n0 + w.out_features
+            whole.codes[n0:n1].copy_(w.codes)
+            whole.scale[n0:n1].copy_(w.scale)
+            w.codes, w.scale = whole.codes[n0:n1], whole.scale[n0:n1]
+            n0 = n1
+        return whole
+
+    def state(self):
+        return {"version": _FORMAT_VERSION, "codes": self.codes.cpu().contiguous(), "scale": self.scale.cpu()}
+
+    def save(self, path):
+        torch.save(self.state(), path)
+
+    @classmethod
+    def from_state(cls, st, device):
+        if st.get("version") != _FORMAT_VERSION:
+            raise RuntimeError("Int8Weights: unknown container version %r" % (st.get("version"),))
+        N, K = st["codes"].shape
+        codes = torch.empty_strided((N, K), ((K + 15) // 16 * 16, 1), dtype=torch.int8, device=device)
+        codes.copy_(st["codes"])
+        return cls(codes, st["scale"].to(device))
+
+    @classmethod
+    def load(cls, path, device="cuda"):
+        return cls.from_state(torch.load(path, map_location="cpu"), device)
+
+
+@torch.library.custom_op("mixedgemm_b200::int8_linear", mutates_args=())
+def int8_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:
+    """x [M, K] times 8-bit weights: quantise every token, one product."""
+    q, s = api.quantize_int8(x)
+    return api.matmul_int8(q, codes, s, scale, bias=bias, out_dtype=x.dtype)
+
+
+@int8_linear.register_fake
+def _(x, codes, scale, bias):
+    return x.new_empty((x.size(0), codes.size(0)))
+
+
+@torch.library.custom_op("mixedgemm_b200::int8_norm_linear", mutates_args=())
+def int8_norm_linear(x: torch.Tensor, residual: Optional[torch.Tensor], norm_weight: torch.Tensor, eps: float,
+                     codes: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor]) -> List[torch.Tensor]:
+    """The same behind a root-mean-square norm: [product, stream after the residual's addition]; without
+    a residual the second is one element."""
+    q, s, *u = api.rms_norm_int8(x, norm_weight, eps=eps, residual=residual)
+    return [api.matmul_int8(q, codes, s, scale, bias=bias, out_dtype=x.dtype), u[0] if u else x.new_empty(1)]
+
+
+@int8_norm_linear.register_fake
+def _(x, residual, norm_weight, eps, codes, scale, bias):
+    return [x.new_empty((x.size(0), codes.size(0))), x.new_empty(x.shape if residual is not None else (1,))]
+
+
+class Int8Linear(torch.nn.Module):
+    """MixedLinear's counterpart with 8-bit weights and activations (a scale per channel and per token),
+    for projections that 4-bit weights hurt.  Several weights that share x are one product over their
+    concatenated rows, handed out as column ranges.  norm_weight, residual and what forward returns are
+    as in MixedLinear; x may be bf16, fp16 or fp32, and norm_weight has its type."""
+
+    def __init__(self, weights, bias=None, norm_weight=None, eps=1e-6):
+        super().__init__()
+        self.weights = list(weights) if isinstance(weights, (list, tuple)) else [weights]
+        if bias is None:
+            bias = [None] * len(self.weights)
+        elif torch.is_tensor(bias):
+            bias = [bias]
+        if len(bias) != len(self.weights):
+            raise ValueError("one bias (or None) per weight")
+        for b_, w in zip(bias, self.weights):
+            if b_ is not None and (b_.dim() != 1 or b_.numel() != w.out_features):
+                raise ValueError("a bias must be a vector of out_features elements")
+        self.fused = Int8Weights.cat(self.weights) if len(self.weights) > 1 else self.weights[0]
+        self.bias = None
+        if any(b_ is not None for b_ in bias):
+            self.bias = torch.cat([torch.zeros(w.out_features, device=w.scale.device) if b_ is None else
+                                   b_.to(w.scale.device, torch.float32) for b_, w in zip(bias, self.weights)])
+        self.norm_weight, self.eps = _norm_weight(norm_weight, self.fused.in_features, None), float(eps)
+
+    @classmethod
+    def from_dense(cls, Ws, **kw):
+        """Ws: one or several [N_j, K] weights that share an input; other arguments as in the constructor."""
+        Ws = list(Ws) if isinstance(Ws, (list, tuple)) else [Ws]
+        return cls([Int8Weights.from_dense(W) for W in Ws], **kw)
+
+    def forward(self, x, residual=None):
+        lead = x.shape[:-1]
+        x2 = x.reshape(-1, x.shape[-1]).contiguous()
+        stream = None
+        if self.norm_weight is None:
+            if residual is not None:
+                raise ValueError("a residual needs a module with norm_weight")
+            y = torch.ops.mixedgemm_b200.int8_linear(x2, self.fused.codes, self.fused.scale, self.bias)
+        else:
+            y, stream = torch.ops.mixedgemm_b200.int8_norm_linear(x2, _residual_rows(residual, x), self.norm_weight,
+                                                                  self.eps, self.fused.codes, self.fused.scale, self.bias)
+        outs, n0 = [], 0
+        for w in self.weights:
+            outs.append(y[:, n0:n0 + w.out_features].reshape(*lead, w.out_features))
+            n0 += w.out_features
+        outs = outs[0] if len(outs) == 1 else outs
+        return outs if residual is None else (outs, stream.reshape(x.shape))

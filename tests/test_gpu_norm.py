@@ -1,0 +1,272 @@
+"""RMS norm in front of the MX quantiser, and the modules that take a norm or 8-bit weights.
+
+Tolerance of the norm, derived as for the 8-bit form (tests/test_gpu_int8.py): a row of K values is
+shared by 32 lanes or more, so a thread adds at most 8 ceil(K / 256) squares one after the other; 13
+roundings of the tree follow, half of all that counts after the square root, and rsqrtf and the
+products add 14: EPS_H(K) = (8 ceil(K / 256) + 41) / 2 units of 2^-24.  h is then rounded to bf16, so it
+equals the 64-bit value's rounding except where that value lies within EPS_H (relative) of the middle
+between two bf16 numbers.  Codes and scales of a 32-group without such
+an element have to be those of reorder_quantize_x of the 64-bit h, byte for byte.
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import mx_oracle as orc
+from tests import helpers as H
+
+pytestmark = pytest.mark.gpu
+
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def exact_h(x, w, r, eps):
+    """(u, h in 64 bits)"""
+    u = x if r is None else (x.float() + r.float()).to(torch.bfloat16)
+    f = u.double()
+    return u, f / torch.sqrt(f.pow(2).mean(1, keepdim=True) + eps) * w.double()
+
+
+def near_a_middle(h):
+    """Elements whose bf16 rounding EPS_H could turn."""
+    eps = (8 * -(-h.shape[1] // 256) + 41) / 2 * 2.0 ** -24
+    return (h * (1 - eps)).to(torch.bfloat16) != (h * (1 + eps)).to(torch.bfloat16)
+
+
+def compare_groups(got, want, near, idx, split):
+    """Codes and scales, a 32-group at a time, where no element of the group is near a middle."""
+    M, K = near.shape
+    open_ = near[:, idx.long()].view(M, K // 32, 32).any(2)
+    assert open_.numel() < 100 or float(open_.float().mean()) < 0.5  # something is left to compare
+    at = 0
+    for i, (k, nbytes) in enumerate(zip(split, (16, 24, 32))):
+        g = k // 32
+        if g == 0:
+            continue
+        ok = ~open_[:, at:at + g]
+        at += g
+        a, b = (t[i].cpu().contiguous().view(M, g, nbytes) for t in (got, want))
+        assert torch.equal(a[ok], b[ok]), "codes of segment %d" % i
+        rows, kb = torch.arange(M)[:, None], torch.arange(g)[None, :]
+        off = rows % 32 * 16 + rows // 32 % 4 * 4 + kb % 4 + kb // 4 * 512 + rows // 128 * 512 * ((k + 127) // 128)
+        assert torch.equal(got[3 + i].cpu()[off][ok], want[3 + i].cpu()[off][ok]), "scales of segment %d" % i
+
+
+@pytest.mark.parametrize("split", [(0, 0, 32), (32, 0, 0), (64, 32, 32), (0, 96, 0), (640, 352, 32), (2560, 1408, 128),
+                                   (8960, 4928, 448), (20448, 11264, 1024)])
+def test_norm_then_split_against_64_bits(split):
+    import mixedgemm_b200 as mg
+    K = sum(split)
+    for M, residual in ((1, True), (7, False), (150, True), (700 if K < 8192 else 310, True), (2500 if K <= 4096 else 5, False)):
+        x = H.make_x(M, K, seed=M + K) if K >= 64 else torch.randn(M, K, generator=gen(M)).to(torch.bfloat16)
+        r = torch.randn(M, K, generator=gen(M + 1)).to(torch.bfloat16) if residual else None
+        w = (1 + 0.2 * torch.randn(K, generator=gen(2))).to(torch.bfloat16)
+        idx = torch.randperm(K, generator=gen(3)).to(torch.int16)
+        got = mg.rms_norm_reorder_quantize_x(x.cuda(), w.cuda(), idx.cuda(), *split, eps=1e-5,
+                                             residual=r.cuda() if residual else None)
+        u, h = exact_h(x, w, r, 1e-5)
+        if residual:
+            assert torch.equal(got[6].cpu(), u)
+        want = mg.reorder_quantize_x(h.to(torch.bfloat16).cuda(), idx.cuda(), *split)
+        assert len(got) == 6 + residual and all(a.shape == b.shape and a.stride() == b.stride() for a, b in zip(got, want))
+        compare_groups(got, want, near_a_middle(h), idx, split)
+    assert mg.device_status() == 0
+
+
+@pytest.mark.parametrize("M", [1, 5, 300, 1300])
+def test_same_bytes_as_the_quantiser_where_the_norm_is_exact(M):
+    """Rows of +-2^j have the root-mean-square 2^j: h = +-w whatever the rounding of the statistics."""
+    import mixedgemm_b200 as mg
+    K, split = 4096, (2560, 1408, 128)
+    g = gen(M)
+    sign = torch.randint(0, 2, (M, K), generator=g) * 2 - 1
+    x = (sign * torch.exp2(torch.randint(-6, 7, (M, 1), generator=g).float())).to(torch.bfloat16)
+    w = (torch.randn(K, generator=g) * 3).to(torch.bfloat16)
+    idx = torch.randperm(K, generator=g).to(torch.int16).cuda()
+    got = mg.rms_norm_reorder_quantize_x(x.cuda(), w.cuda(), idx, *split, eps=0.0)
+    h = (sign * w.float()).to(torch.bfloat16)
+    want = H.oracle_outputs(H.bits(h), idx.cpu().numpy(), *split)
+    H.compare_quantised(got, want, M, split, "norm")
+
+
+def test_rows_in_place_pitched_and_given_buffers():
+    import mixedgemm_b200 as mg
+    M, K, split = 70, 1024, (640, 256, 128)
+    x, r = H.make_x(M, K, seed=1), H.make_x(M, K, seed=2)
+    w = (1 + 0.2 * torch.randn(K, generator=gen(3))).to(torch.bfloat16).cuda()
+    idx = torch.randperm(K, generator=gen(4)).to(torch.int16).cuda()
+    ref = mg.rms_norm_reorder_quantize_x(x.cuda(), w, idx, *split, residual=r.cuda())
+    buf = torch.full((2, M, K + 24), 5.0, dtype=torch.bfloat16, device="cuda")
+    xv, rv = buf[0, :, :K], buf[1, :, :K]
+    xv.copy_(x), rv.copy_(r)
+    out = mg.alloc_quantized_x(M, *split, "cuda", padded=False)
+    got = mg.rms_norm_reorder_quantize_x(xv, w, idx, *split, residual=rv, residual_out=rv, out=out)
+    assert got[6] is rv and torch.equal(rv, ref[6]) and torch.equal(xv.cpu(), x)
+    for i in range(3):
+        assert got[i] is out[i] and torch.equal(got[i], ref[i])
+    assert bool((buf[:, :, K:] == 5).all())
+
+
+def test_rows_that_are_not_finite_give_nan_products_and_spoil_no_other():
+    import mixedgemm_b200 as mg
+    M, N, K, split = 40, 256, 1024, (640, 256, 128)
+    x = H.make_x(M, K, seed=1)
+    x[3, 7], x[9, 1000], x[11] = float("nan"), float("inf"), 1e25
+    x[12] = 0
+    w = torch.ones(K, dtype=torch.bfloat16, device="cuda")
+    idx = torch.randperm(K, generator=gen(4)).to(torch.int16).cuda()
+    B = mg.reorder_quantize_w(H.make_w(N, K).cuda(), idx, *split)
+    y = []
+    for rows in (x, x.clone().nan_to_num(0, 0, 0)):
+        A = mg.rms_norm_reorder_quantize_x(rows.cuda(), w, idx, *split)
+        y.append(mg.matmul(A[0], B[0], A[1], B[1], A[2], B[2], A[3], B[3], A[4], B[4], A[5], B[5]))
+    bad = [3, 9, 11]
+    assert bool(torch.isnan(y[0][bad]).all()) and bool((y[0][12] == 0).all())
+    keep = [i for i in range(M) if i not in bad]
+    assert torch.equal(y[0][keep], y[1][keep]) and bool(torch.isfinite(y[0][keep]).all())
+    # a weight that overflows h has the same answer
+    w[5] = 3e38
+    x = torch.full((2, K), 1.0, dtype=torch.bfloat16)
+    x[0, 5] = 30
+    A = mg.rms_norm_reorder_quantize_x(x.cuda(), w, idx, *split)
+    y = mg.matmul(A[0], B[0], A[1], B[1], A[2], B[2], A[3], B[3], A[4], B[4], A[5], B[5])
+    assert bool(torch.isnan(y[0]).all()) and not bool(torch.isnan(y[1]).any())
+    assert mg.device_status() == 0
+
+
+def test_refusals():
+    import mixedgemm_b200 as mg
+    K, split = 256, (128, 64, 64)
+    x, w = torch.zeros(4, K, dtype=torch.bfloat16, device="cuda"), torch.ones(K, dtype=torch.bfloat16, device="cuda")
+    idx = torch.arange(K, dtype=torch.int16, device="cuda")
+    f = mg.rms_norm_reorder_quantize_x
+    odd = torch.zeros(4, K + 4, dtype=torch.bfloat16, device="cuda")
+    good = mg.alloc_quantized_x(4, *split, "cuda")
+    bad = [
+        lambda: f(x.half(), w.half(), idx, *split), lambda: f(x, w, idx, 128, 64, 32), lambda: f(x, w, idx.int(), *split),
+        lambda: f(x, w, idx[:200], *split), lambda: f(x, w, idx, 120, 72, 64), lambda: f(x, w, idx, *split, eps=-1.0),
+        lambda: f(odd[:, :K], w, idx, *split), lambda: f(odd[:, 1:K + 1], w, idx, *split), lambda: f(x, w, idx, *split, residual=x[:3]),
+        lambda: f(x, w, idx, *split, residual_out=x), lambda: f(x, w, idx, *split, residual=odd[:, :K]),
+        lambda: f(x, w[:128], idx, *split), lambda: f(x, w, idx, *split, out=mg.alloc_quantized_x(3, *split, "cuda")),
+        lambda: f(x, w, idx, *split, out=good[:3] + tuple(t[:100] for t in good[3:])), lambda: f(x.cpu(), w, idx, *split),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail("case %d was not refused" % i)
+    assert f(x[:0], w, idx, *split)[0].shape == (0, 64)
+
+
+# ------------------------------------------------------------------------------------------ modules
+
+def dense(N, K, seed):
+    return H.make_w(N, K, seed=seed).cuda()
+
+
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_mixed_linear_with_a_norm_is_its_operators_in_a_row(M):
+    import mixedgemm_b200 as mg
+    from mixedgemm_b200.linear import MixedLinear, QuantizedWeights
+    K = 2048
+    X = H.make_x(300, K, seed=3).cuda()
+    r = torch.randn(M, K, generator=gen(8)).to(torch.bfloat16).cuda()
+    w = (1 + 0.2 * torch.randn(K, generator=gen(9))).to(torch.bfloat16).cuda()
+    idx = mg.reorder_index(X)
+    Ws = [QuantizedWeights.from_dense(dense(N, K, 5 + N), idx) for N in (512, 256)]
+    lin = MixedLinear(Ws, norm_weight=w, eps=1e-5)
+    x = X[:M].contiguous()
+    ys, stream = lin(x, residual=r)
+    A = mg.rms_norm_reorder_quantize_x(x, w, idx, *lin.split, eps=1e-5, residual=r)
+    assert torch.equal(stream, A[6]) and torch.equal(stream, (x.float() + r.float()).to(torch.bfloat16))
+    for y, q in zip(ys, lin.weights):
+        B = q.parts
+        ref = mg.matmul(A[0], B[0], A[1], B[1], A[2], B[2], A[3], B[3], A[4], B[4], A[5], B[5])
+        assert (y.float() - ref.float()).norm() <= 0.01 * ref.float().norm()  # another tile order may round otherwise
+    again = lin(stream)  # without a residual: the outputs alone
+    assert isinstance(again, list) and all((a.float() - y.float()).norm() <= 0.01 * y.float().norm() for a, y in zip(again, ys))
+    with pytest.raises(ValueError):
+        MixedLinear(Ws)(x, residual=r)
+    with pytest.raises(ValueError):
+        lin(x, residual=r[:, :8])
+    assert mg.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("lead", [(1,), (3, 50)])
+def test_int8_linear(lead, dtype, tmp_path):
+    import mixedgemm_b200 as mg
+    from mixedgemm_b200.linear import Int8Linear, Int8Weights
+    K, Ns = 1000, (384, 130)
+    x = H.make_x(150, K, seed=3).to(dtype).cuda()[:int(np.prod(lead))].reshape(*lead, K)
+    r = torch.randn(*lead, K, generator=gen(8)).to(dtype).cuda()
+    Ws = [dense(N, K, N) for N in Ns]
+    bias = torch.randn(Ns[1], generator=gen(1)).cuda()
+    w = (1 + 0.2 * torch.randn(K, generator=gen(9))).to(dtype).cuda()
+    plain, norm = Int8Linear.from_dense(Ws, bias=[None, bias]), Int8Linear.from_dense(Ws, norm_weight=w, eps=1e-5)
+    ys = plain(x)
+    for y, W, b in zip(ys, Ws, (0, bias)):
+        assert y.shape == (*lead, W.shape[0]) and y.dtype == dtype
+        ref = x.double() @ W.double().t() + b
+        # x: half a step of amax / 127 per element; W likewise: a few per cent of a row's norm
+        assert float((y.double() - ref).norm() / ref.norm()) < 0.1
+    q, s = mg.quantize_int8(x.reshape(-1, K))
+    f = plain.fused
+    ref = mg.matmul_int8(q, f.codes, s, f.scale, bias=plain.bias, out_dtype=dtype)
+    assert torch.equal(torch.cat(ys, -1).reshape(-1, sum(Ns)), ref)
+    yn, stream = norm(x, residual=r)
+    q, s, u = mg.rms_norm_int8(x.reshape(-1, K), w, eps=1e-5, residual=r.reshape(-1, K))
+    assert torch.equal(stream, u.reshape(x.shape)) and torch.equal(
+        torch.cat(yn, -1).reshape(-1, sum(Ns)), mg.matmul_int8(q, f.codes, s, f.scale, out_dtype=dtype))
+    again = norm(stream)
+    assert all(torch.equal(a, y) for a, y in zip(again, yn))
+    # the container on disk
+    plain.weights[1].save(str(tmp_path / "w.pt"))
+    back = Int8Linear(Int8Weights.load(str(tmp_path / "w.pt")), bias=bias)
+    assert torch.equal(back(x), ys[1])
+    with pytest.raises(ValueError):
+        plain(x, residual=r)
+    with pytest.raises(ValueError):
+        Int8Linear.from_dense(Ws, norm_weight=w[:10])
+
+
+def test_a_block_of_both_kinds_in_a_graph():
+    """norm -> 4-bit q/k/v, 8-bit o, norm -> 4-bit gate, 8-bit down: the operators as a layer uses
+    them, eager and replayed with new inputs."""
+    import mixedgemm_b200 as mg
+    from mixedgemm_b200.linear import Int8Linear, MixedLinear, QuantizedWeights
+    M, K, F = 20, 2048, 1024  # a split with KS and KO multiples of 64, as the product needs
+    X = H.make_x(300, K, seed=3).cuda()
+    idx = mg.reorder_index(X)
+    w = [(1 + 0.2 * torch.randn(K, generator=gen(i))).to(torch.bfloat16).cuda() for i in range(2)]
+    qkv = MixedLinear([QuantizedWeights.from_dense(dense(N, K, N), idx) for N in (2048, 256, 256)], norm_weight=w[0], max_tokens=M)
+    o = Int8Linear.from_dense(dense(K, K, 11))
+    gate = MixedLinear(QuantizedWeights.from_dense(dense(F, K, 12), idx), norm_weight=w[1], max_tokens=M)
+    down = Int8Linear.from_dense(dense(K, F, 13))
+
+    def block(x, stream):
+        (q, _, _), stream = qkv(x, residual=stream)
+        h, stream = gate(o(q), residual=stream)
+        return down(torch.nn.functional.silu(h)), stream
+
+    x, s = X[:M].contiguous(), X[M:2 * M].contiguous()
+    want = block(x, s)
+    x2, s2 = X[40:60].contiguous(), X[60:80].contiguous()
+    want2 = block(x2, s2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    xin, sin = x.clone(), s.clone()
+    with torch.cuda.stream(side):
+        got = block(xin, sin)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out = block(xin, sin)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    xin.copy_(x2), sin.copy_(s2)
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want2))
+    assert mg.device_status() == 0

@@ -70,3 +70,21 @@ def test_python_layer_refuses_tensors_off_the_gpu(lib):
                  lambda: mg.matmul_int8(q, q, s, s)):
         with pytest.raises(RuntimeError, match="CUDA tensor"):
             call()
+
+
+def mx_norm(lib, X=P, ldx=128, R=None, ldr=0, W=P, eps=1e-6, U=None, ldu=0, M=4, K=128, idx=P, split=(64, 32, 32), codes=P, scales=P):
+    return lib.mg_rms_norm_reorder_quantize(X, ldx, R, ldr, W, eps, U, ldu, M, K, idx, *split, codes, codes, codes, None,
+                                            scales, scales, scales, None)
+
+
+@pytest.mark.parametrize("want, args", [
+    (OK, dict(M=0, X=None, W=None, idx=None, codes=None, scales=None)),
+    (SHAPE, dict(M=-1)), (SHAPE, dict(K=120)), (SHAPE, dict(split=(80, 16, 32))), (SHAPE, dict(eps=-1.0)), (SHAPE, dict(eps=float("nan"))),
+    (SHAPE, dict(ldx=120)), (SHAPE, dict(R=P, U=P, ldr=120, ldu=128)), (SHAPE, dict(R=P, U=P, ldr=128, ldu=120)),
+    (NULL, dict(X=None)), (NULL, dict(W=None)), (NULL, dict(idx=None)), (NULL, dict(codes=None)), (NULL, dict(scales=None)),
+    (NULL, dict(R=P, ldr=128, ldu=128)), (NULL, dict(U=P, ldr=128, ldu=128)),
+    (ALIGN, dict(X=P + 2)), (ALIGN, dict(W=P + 8)), (ALIGN, dict(ldx=132)), (ALIGN, dict(R=P + 2, U=P, ldr=128, ldu=128)),
+    (ALIGN, dict(R=P, U=P, ldr=130, ldu=128)), (ALIGN, dict(R=P, U=P, ldr=128, ldu=129)), (ALIGN, dict(codes=P + 4)),
+])
+def test_mx_norm_refusals(lib, want, args):
+    assert mx_norm(lib, **args) == want
