@@ -28,6 +28,7 @@
 namespace {
 
 using mg::wait_parity;
+using mg::wait_parity_cluster;
 
 constexpr int kRows = 128;      // channels of a CTA's tile
 constexpr int kThreads = 192;
@@ -49,6 +50,16 @@ struct Int8Params {
 template <int MMA_M, int MMA_N>
 constexpr uint32_t kIdescI8 =
     (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(MMA_N >> 3) << 17) | ((uint32_t)(MMA_M >> 4) << 24);
+
+// Tile order: token tiles in groups of eight, all channel tiles of a group before the next group, so
+// that the tiles that run at one time share operands in L2.
+__device__ __forceinline__ void raster(int t, int tiles_m, int tiles_n, int& m_tile, int& n_tile) {
+  constexpr int kGroup = 8;
+  const int g = t / (kGroup * tiles_n), r = t - g * kGroup * tiles_n;
+  const int rows = min(kGroup, tiles_m - g * kGroup);
+  m_tile = g * kGroup + r % rows;
+  n_tile = r / rows;
+}
 
 template <typename T>
 __device__ __forceinline__ T round_to(float f);
@@ -260,6 +271,207 @@ __global__ void __launch_bounds__(kThreads) int8_gemm_kernel(const Int8Params p,
   if (warp == 1) ptx::tmem_dealloc(tmem, BT);
 }
 
+// ---------------------------------------------------------------- CTA-pair form
+// Two CTAs of a cluster compute 256 channels x BT tokens with tcgen05.mma.cta_group::2: each stages
+// its own 128 channels and half of the tokens, and one instruction of the leader drives both tensor
+// cores.  The loads of both CTAs are counted on the leader's barrier.  Two accumulators alternate, so
+// the epilogue of a tile runs under the products of the next.  Persistent: cluster c takes tiles
+// c, c + clusters, ...
+template <int BT>
+struct PairCfg {
+  static constexpr int STAGES = BT == 256 ? 6 : 8;
+  static constexpr uint32_t W_BYTES = 128 * 128;
+  static constexpr uint32_t T_BYTES = BT / 2 * 128;
+  static constexpr uint32_t STAGE_BYTES = W_BYTES + T_BYTES;
+  static constexpr uint32_t SCALE_BYTES = 4 * BT * 4;  // the tile's token scales, once per epilogue warp
+  static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + SCALE_BYTES + 256;
+};
+
+template <int BT, typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT) {
+  using C = PairCfg<BT>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = ptx::smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  const uint32_t scales = base + C::STAGES * C::STAGE_BYTES;
+  const uint32_t bar0 = scales + C::SCALE_BYTES;
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (C::STAGES + s); };
+  auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * C::STAGES + a); };
+  auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * C::STAGES + 2 + a); };
+  volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(gbase + C::STAGES * C::STAGE_BYTES + C::SCALE_BYTES +
+                                                                        8 * (2 * C::STAGES + 4));
+  volatile int* stop = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_ctarank();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      ptx::mbar_init(full_bar(s), 1);  // (used in the leader only)
+      ptx::mbar_init(empty_bar(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      ptx::mbar_init(tfull_bar(a), 1);
+      ptx::mbar_init(tempty_bar(a), 8);  // four epilogue warps in each CTA (used in the leader only)
+    }
+    *stop = 0;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tmap(&tmW);
+    ptx::prefetch_tmap(&tmT);
+  }
+  ptx::cluster_sync();  // both CTAs' barriers exist before anything arrives on them
+  if (warp == 1) {
+    ptx::tmem_alloc_pair(ptx::smem_u32(const_cast<uint32_t*>(tmem_holder)), 2 * BT);
+    ptx::tmem_relinquish_pair();
+  }
+  ptx::grid_dep_launch_dependents();
+  ptx::tc_fence_before();
+  ptx::cluster_sync();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  ptx::grid_dep_wait();  // the prologue above touched no global memory
+
+  const int tiles_n = (p.N + 255) / 256, tiles_m = (p.M + BT - 1) / BT;
+  const int first = (int)ptx::cluster_id_x(), step = (int)ptx::nclusters_x();
+  const int count = (tiles_n * tiles_m - first + step - 1) / step;
+  auto locate = [&](int i, int& n0, int& m0) {
+    int m_tile, n_tile;
+    raster(first + i * step, tiles_m, tiles_n, m_tile, n_tile);
+    n0 = n_tile * 256 + (int)rank * 128;
+    m0 = m_tile * BT;
+  };
+
+  if (warp == 0) {
+    const bool leader = ptx::elect_one();
+    int slot = 0;
+    uint32_t phase = 0;
+    bool live = true;
+    for (int i = 0; i < count && live; ++i) {
+      int n0, m0;
+      locate(i, n0, m0);
+      m0 += (int)rank * (BT / 2);
+#pragma unroll 1
+      for (int s = 0; s < p.stages; ++s) {
+        if (!wait_parity(empty_bar(slot), phase ^ 1u, stop, p.status, p.wait_cycles, 1)) { live = false; break; }
+        if (leader) {
+          const uint32_t sbase = base + slot * C::STAGE_BYTES;
+          const uint32_t fb = ptx::map_to_cta(full_bar(slot), 0);
+          if (rank == 0) ptx::mbar_expect_tx(full_bar(slot), 2 * C::STAGE_BYTES);
+          ptx::tma_load_2d_pair(sbase, &tmW, s * 128, n0, fb);
+          ptx::tma_load_2d_pair(sbase + C::W_BYTES, &tmT, s * 128, m0, fb);
+        }
+        if (++slot == C::STAGES) { slot = 0; phase ^= 1u; }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const bool leader = ptx::elect_one();
+      constexpr uint32_t kIdesc = kIdescI8<256, BT>;
+      int slot = 0;
+      uint32_t phase = 0;
+      bool live = true;
+      for (int i = 0; i < count && live; ++i) {
+        const int acc = i & 1;
+        if (!wait_parity_cluster(tempty_bar(acc), (((uint32_t)i >> 1) & 1u) ^ 1u, stop, p.status, p.wait_cycles, 4)) break;
+        ptx::tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)acc * BT;
+        uint32_t accumulate = 0;
+#pragma unroll 1
+        for (int s = 0; s < p.stages; ++s) {
+          if (!wait_parity_cluster(full_bar(slot), phase, stop, p.status, p.wait_cycles, 2)) { live = false; break; }
+          ptx::tc_fence_after();
+          const uint32_t sbase = base + slot * C::STAGE_BYTES;
+          const uint32_t w_lo = ptx::desc_lo(sbase), t_lo = ptx::desc_lo(sbase + C::W_BYTES);
+          if (leader) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              ptx::mma_i8_pair(d, w_lo + j * 2, t_lo + j * 2, ptx::kDescHiSw128, kIdesc, accumulate);
+              accumulate = 1;
+            }
+            ptx::tc_commit_pair(empty_bar(slot), 3);  // frees the stage in both CTAs
+          }
+          if (++slot == C::STAGES) { slot = 0; phase ^= 1u; }
+        }
+        if (leader && live) ptx::tc_commit_pair(tfull_bar(acc), 3);
+      }
+    }
+  } else {
+    const int quad = warp & 3;  // tensor-memory lanes this warp may read
+    const uint32_t my_scales = scales + (uint32_t)(warp - 2) * (BT * 4);
+    float* g_scales = reinterpret_cast<float*>(gbase + (my_scales - base));
+    for (int i = 0; i < count; ++i) {
+      int n0, m0;
+      locate(i, n0, m0);
+      const int acc = i & 1, n = n0 + quad * 32 + lane;
+      const bool real = n < p.N;
+      const float sb = real ? p.sb[n] : 0.f;
+      const float bias = real && p.bias ? p.bias[n] : 0.f;
+#pragma unroll
+      for (int c = 0; c < BT; c += 32) g_scales[c + lane] = m0 + c + lane < p.M ? p.sa[m0 + c + lane] : 0.f;
+      __syncwarp();
+      const bool store = wait_parity(tfull_bar(acc), ((uint32_t)i >> 1) & 1u, stop, p.status, p.wait_cycles, 8) && real && !*stop;
+      __syncwarp();
+      ptx::tc_fence_after();
+      const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)acc * BT;
+      T* out = static_cast<T*>(p.D) + (size_t)m0 * p.ldd + n;
+#pragma unroll 1
+      for (int c = 0; c < BT; c += 64) {
+        uint32_t r[2][32];
+        ptx::tmem_ld_32x32(taddr + c, r[0]);
+        ptx::tmem_ld_32x32(taddr + c + 32, r[1]);
+        ptx::tmem_ld_wait();
+        if (c + 64 >= BT) {  // the accumulator is in registers: hand it back
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive_release_cluster(ptx::map_to_cta(tempty_bar(acc), 0));
+        }
+        if (store) {
+          const int left = p.M - m0 - c;
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const uint4 sv = ptx::lds_v4(my_scales + (uint32_t)(c + v * 4) * 4u);
+            const uint32_t sa[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float f = __fmul_rn((float)(int)r[v >> 3][(v & 7) * 4 + k], __uint_as_float(sa[k]));
+              if (v * 4 + k < left) out[(size_t)(c + v * 4 + k) * p.ldd] = round_to<T>(__fmaf_rn(f, sb, bias));
+            }
+          }
+        }
+      }
+      __syncwarp();  // the scales have been read
+    }
+  }
+
+  ptx::tc_fence_before();
+  // A CTA that gave up tells its peer (which is still here: it cannot pass the barrier below before
+  // this CTA arrives), so that both take the same path through the second barrier.
+  __syncthreads();
+  if (threadIdx.x == 0 && *stop) ptx::st_cluster_u32(ptx::map_to_cta(ptx::smem_u32(const_cast<int*>(stop)), rank ^ 1u), 1u);
+  ptx::cluster_sync();
+  ptx::tc_fence_after();
+  if (*stop) {
+    // give copies and MMAs that are still in flight time to land before either CTA goes away
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    ptx::cluster_sync();
+  }
+  if (warp == 1) ptx::tmem_dealloc_pair(tmem, 2 * BT);
+}
+
+template <int BT, typename T>
+int launch_pair(const Int8Params& p, const CUtensorMap& w, const CUtensorMap& t, int sms, cudaStream_t st) {
+  using C = PairCfg<BT>;
+  auto kern = int8_gemm_pair_kernel<BT, T>;
+  MG_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+  const int tiles = ((p.N + 255) / 256) * ((p.M + BT - 1) / BT);
+  const int clusters = tiles < sms / 2 ? tiles : sms / 2;
+  MG_CUDA_TRY(mg::launch_kernel(kern, dim3(clusters * 2), dim3(kThreads), C::SMEM, st, p, w, t));
+  return MG_OK;
+}
+
 template <int BT, typename T>
 int launch_small(const Int8Params& p, const CUtensorMap& w, const CUtensorMap& t, int splits, cudaStream_t st) {
   using C = SmallCfg<BT>;
@@ -288,6 +500,15 @@ template <typename T>
 int launch_int8(const Int8Params& p, const int8_t* A, size_t lda, const int8_t* B, size_t ldb, int K, int sms,
                 cudaStream_t st) {
   const mg::Options opt = mg::options();
+  CUtensorMap w, t;
+  int rc;
+  const int pair = opt.int8_pair >= 0 ? opt.int8_pair : p.M > 128 ? 256 : 0;
+  if (pair > 0) {
+    const int bt = pair == 128 ? 128 : 256;
+    if ((rc = mg::make_map(&w, CU_TENSOR_MAP_DATA_TYPE_UINT8, B, K, p.N, ldb, 128, 128))) return rc;
+    if ((rc = mg::make_map(&t, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, K, p.M, lda, 128, bt / 2))) return rc;
+    return bt == 128 ? launch_pair<128, T>(p, w, t, sms, st) : launch_pair<256, T>(p, w, t, sms, st);
+  }
   int bt = p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
   if (opt.int8_tokens == 32 || opt.int8_tokens == 64 || opt.int8_tokens == 128) bt = opt.int8_tokens;
   const int tiles = ((p.N + kRows - 1) / kRows) * ((p.M + bt - 1) / bt);
@@ -296,8 +517,6 @@ int launch_int8(const Int8Params& p, const int8_t* A, size_t lda, const int8_t* 
   if (opt.int8_split > 0) splits = opt.int8_split >= 8 ? 8 : opt.int8_split >= 4 ? 4 : opt.int8_split >= 2 ? 2 : 1;
   while (splits > p.stages) splits /= 2;
   if ((p.M + bt - 1) / bt > 65535) return MG_ERR_SHAPE;
-  CUtensorMap w, t;
-  int rc;
   if ((rc = mg::make_map(&w, CU_TENSOR_MAP_DATA_TYPE_UINT8, B, K, p.N, ldb, 128, kRows))) return rc;
   if ((rc = mg::make_map(&t, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, K, p.M, lda, 128, bt))) return rc;
   if (bt == 32) return launch_small<32, T>(p, w, t, splits, st);

@@ -47,6 +47,7 @@ struct Options {
                         // (host-side fault injection for the bounded-wait test; the kernel then gives up
                         // after the wait limit and returns normally)
   int int8_tokens;      // INT8_TOKENS: 32 / 64 / 128 / 256 forces the token tile of the 8-bit product
+  int int8_pair;        // INT8_PAIR: 0 turns the CTA-pair form off, 128 / 256 forces it with that token tile
   int int8_split;       // INT8_SPLIT: 1 / 2 / 4 / 8 forces the number of CTAs that share a tile's K
 };
 Options options();

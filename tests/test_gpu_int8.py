@@ -234,10 +234,20 @@ def test_product_against_64_bits(M, N, K, dtype):
 @pytest.mark.parametrize("tile", [32, 64, 128])
 @pytest.mark.parametrize("split", [1, 2, 4, 8])
 def test_product_of_every_tile_and_split(tile, split, mgopt):
+    mgopt.set("INT8_PAIR", 0)
     mgopt.set("INT8_TOKENS", tile)
     mgopt.set("INT8_SPLIT", split)
     for M, N, K in ((1, 130, 1024), (37, 300, 1931), (140, 257, 4096), (300, 640, 128)):
         run_product(M, N, K, torch.float32, with_bias=True, seed=tile + split)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tile", [128, 256])
+def test_product_of_the_pair_form(tile, dtype, mgopt):
+    """One tile, many tiles to a pair (both accumulators, several turns), ragged edges, one slice of K."""
+    mgopt.set("INT8_PAIR", tile)
+    for M, N, K in ((1, 1, 1), (200, 130, 1024), (140, 257, 1931), (513, 640, 128), (1000, 5000, 300), (2300, 3000, 128)):
+        run_product(M, N, K, dtype, with_bias=True, seed=tile)
 
 
 def test_product_does_not_depend_on_tile_or_split(mgopt):
@@ -252,6 +262,9 @@ def test_product_does_not_depend_on_tile_or_split(mgopt):
             mgopt.set("INT8_TOKENS", tile)
             mgopt.set("INT8_SPLIT", split)
             assert torch.equal(mg.matmul_int8(av, bv, sa, sb), ref)
+    for pair in (128, 256):
+        mgopt.set("INT8_PAIR", pair)
+        assert torch.equal(mg.matmul_int8(av, bv, sa, sb), ref)
 
 
 def test_product_of_the_longest_row_does_not_overflow():
