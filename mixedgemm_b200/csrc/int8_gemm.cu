@@ -19,6 +19,8 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
+#include <cmath>
 
 #include "mg_common.h"
 #include "mg_wait.cuh"
@@ -98,6 +100,7 @@ struct Channel {
 // column, 10 us for a tile of 256 tokens.
 template <int NC, typename T>
 __device__ __forceinline__ void finish(const int* sum, uint32_t scales, int c, int left, const Channel<T>& ch, size_t ldd) {
+  constexpr int kStep = NC < 8 ? NC : 8;
   T v[NC];
 #pragma unroll
   for (int i = 0; i < NC; i += 4) {
@@ -111,10 +114,18 @@ __device__ __forceinline__ void finish(const int* sum, uint32_t scales, int c, i
   if (left >= NC) {
 #pragma unroll
     for (int i = 0; i < NC; ++i) out[(size_t)i * ldd] = v[i];
-  } else {
+    return;
+  }
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
-      if (i < left) out[(size_t)i * ldd] = v[i];
+  for (int i = 0; i < NC; i += kStep) {
+    if (left >= i + kStep) {
+#pragma unroll
+      for (int k = 0; k < kStep; ++k) out[(size_t)(i + k) * ldd] = v[i + k];
+    } else if (left > i) {
+#pragma unroll
+      for (int k = 0; k < kStep; ++k)
+        if (i + k < left) out[(size_t)(i + k) * ldd] = v[i + k];
+    }
   }
 }
 
@@ -130,7 +141,7 @@ __device__ __forceinline__ void stage_scales(float* dst, const Int8Params& p, in
 // share its K slices and add their sums through distributed shared memory.
 template <int BT>
 struct SmallCfg {
-  static constexpr int STAGES = BT == 32 ? 5 : BT == 64 ? 4 : 4;
+  static constexpr int STAGES = BT == 32 ? 10 : BT == 64 ? 8 : 5;
   static constexpr uint32_t W_BYTES = kRows * 128;
   static constexpr uint32_t T_BYTES = BT * 128;
   static constexpr uint32_t STAGE_BYTES = W_BYTES + T_BYTES;
@@ -181,7 +192,7 @@ __global__ void __launch_bounds__(kThreads) int8_gemm_kernel(const Int8Params p,
   ptx::grid_dep_launch_dependents();
   ptx::tc_fence_before();
   __syncthreads();
-  if (splits > 1) ptx::cluster_sync();  // every CTA of the cluster runs before anyone stores into it
+  if (splits > 1) ptx::cluster_arrive();  // (waited for below, before anyone stores into another CTA)
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   ptx::grid_dep_wait();  // the prologue above touched no global memory
@@ -190,6 +201,7 @@ __global__ void __launch_bounds__(kThreads) int8_gemm_kernel(const Int8Params p,
   const int quad = warp & 3, row = quad * 32 + lane;  // an epilogue warp's tensor-memory lanes = channels of the tile
   const Channel<T> chan(p, warp >= 2 ? n0 + row : p.N, m0);
   const uint32_t my_scales = scales + (uint32_t)((warp - 2) & 3) * (BT * 4);
+  const int left = p.M - m0;     // tokens of this tile and beyond
   const int cols = BT / splits;  // columns this CTA finishes
   const uint32_t per_sender = (uint32_t)kRows * cols * 4;
   const int s0 = (int)((long long)p.stages * rank / splits), s1 = (int)((long long)p.stages * (rank + 1) / splits);
@@ -238,24 +250,25 @@ __global__ void __launch_bounds__(kThreads) int8_gemm_kernel(const Int8Params p,
     ptx::tc_fence_after();
     if (splits == 1) {
 #pragma unroll 1
-      for (int c = 0; c < BT; c += 32) {
+      for (int c = 0; c < BT && c < left; c += 32) {
         uint32_t r[32];
         ptx::tmem_ld_32x32(taddr + c, r);
         ptx::tmem_ld_wait();
-        if (store) finish<32>(reinterpret_cast<const int*>(r), my_scales, c, p.M - m0 - c, chan, p.ldd);
+        if (store) finish<32>(reinterpret_cast<const int*>(r), my_scales, c, left - c, chan, p.ldd);
       }
     } else {
       // Column group g of this tile (BT / splits columns) is finished by CTA g: the others send it
       // theirs, 16 bytes (four columns of a channel) at a time.
+      ptx::cluster_wait();  // every CTA of the cluster runs
 #pragma unroll 1
-      for (int c = 0; c < BT; c += 32) {
+      for (int c = 0; c < BT && c < left; c += 32) {
         uint32_t r[32];
         ptx::tmem_ld_32x32(taddr + c, r);
         ptx::tmem_ld_wait();
 #pragma unroll
         for (int v = 0; v < 8; ++v) {
           const int col = c + v * 4, g = col / cols;
-          if (g != rank) {
+          if (g != rank && col < left) {
             const uint32_t dst = recv + (uint32_t)(rank - (rank > g)) * per_sender +
                                  (uint32_t)((col - g * cols) >> 2) * (kRows * 16u) + (uint32_t)row * 16u;
             ptx::st_cluster_v4(ptx::map_to_cta(dst, (uint32_t)g), r[v * 4], r[v * 4 + 1], r[v * 4 + 2], r[v * 4 + 3]);
@@ -266,6 +279,8 @@ __global__ void __launch_bounds__(kThreads) int8_gemm_kernel(const Int8Params p,
   }
 
   if (splits > 1) {
+    __syncwarp();
+    if (warp < 2) ptx::cluster_wait();
     // every wait above is bounded, so every thread of the cluster arrives here; a CTA that gave up
     // tells the others first, so that nobody adds sums that were never sent
     __syncthreads();
@@ -275,7 +290,7 @@ __global__ void __launch_bounds__(kThreads) int8_gemm_kernel(const Int8Params p,
     if (warp >= 2 && !*stop) {
       const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16);
       const int first = rank * cols;
-      for (int c = 0; c < cols; c += 4) {
+      for (int c = 0; c < cols && first + c < left; c += 4) {
         uint32_t r[4];
         ptx::tmem_ld_32x4(taddr + first + c, r);
         ptx::tmem_ld_wait();
@@ -288,7 +303,7 @@ __global__ void __launch_bounds__(kThreads) int8_gemm_kernel(const Int8Params p,
           sum[2] += (int)a.z;
           sum[3] += (int)a.w;
         }
-        if (chan.real) finish<4>(sum, my_scales, first + c, p.M - m0 - first - c, chan, p.ldd);
+        if (chan.real) finish<4>(sum, my_scales, first + c, left - first - c, chan, p.ldd);
       }
     }
   }
@@ -446,20 +461,21 @@ int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tm
       __syncwarp();
       ptx::tc_fence_after();
       const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)acc * BT;
+      const int left = min(p.M - m0, BT);
 #pragma unroll 1
-      for (int c = 0; c < BT; c += 64) {
+      for (int c = 0; c < left; c += 64) {
         uint32_t r[2][32];
         ptx::tmem_ld_32x32(taddr + c, r[0]);
         ptx::tmem_ld_32x32(taddr + c + 32, r[1]);
         ptx::tmem_ld_wait();
-        if (c + 64 >= BT) {  // the accumulator is in registers: hand it back
+        if (c + 64 >= left) {  // the accumulator is in registers: hand it back
           ptx::tc_fence_before();
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive_release_cluster(ptx::map_to_cta(tempty_bar(acc), 0));
         }
         if (store) {
-          finish<32>(reinterpret_cast<const int*>(r[0]), my_scales, c, p.M - m0 - c, chan, p.ldd);
-          finish<32>(reinterpret_cast<const int*>(r[1]), my_scales, c + 32, p.M - m0 - c - 32, chan, p.ldd);
+          finish<32>(reinterpret_cast<const int*>(r[0]), my_scales, c, left - c, chan, p.ldd);
+          finish<32>(reinterpret_cast<const int*>(r[1]), my_scales, c + 32, left - c - 32, chan, p.ldd);
         }
       }
       __syncwarp();  // the scales have been read
@@ -516,32 +532,111 @@ int launch_small(const Int8Params& p, const CUtensorMap& w, const CUtensorMap& t
   return MG_OK;
 }
 
+// How many clusters of `splits` such CTAs the device holds at one time (asked once per device and shape;
+// 0 where it holds none).
+template <int BT, typename T>
+int small_capacity(int splits, int sms) {
+  if (splits == 1) return sms;
+  static std::atomic<int> known[64][4];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  std::atomic<int>& slot = known[dev][splits == 2 ? 0 : splits == 4 ? 1 : 2];
+  int k = slot.load();
+  if (k == 0) {
+    using C = SmallCfg<BT>;
+    auto kern = int8_gemm_kernel<BT, T>;
+    int n = 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1, 1, splits);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C::smem(splits);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = splits;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const bool ok = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::smem(kMaxSplit)) == cudaSuccess &&
+                    cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n >= 1;
+    if (!ok) (void)cudaGetLastError();  // the question is allowed to fail; the answer is then "none"
+    k = ok ? n : -1;
+    slot.store(k);
+  }
+  return k > 0 ? k : 0;
+}
+
+// Which form takes the problem: the one with the least of
+//   T = fixed + wave * waves + sqrt(compute^2 + bytes^2)   in us,
+// compute = waves * K stages of a CTA * stage, bytes = those of the operands and the result / 7.2 MB per us,
+// waves = tiles / (clusters that run at one time).  The constants are fitted to 117 problems (M = 1 ... 2048,
+// N and K = 1024, 4096, 14336, bf16 results, cold weights) run with every form: over them the choice is
+// 1 % slower than the best form on average and 14 % at most.  What they say: a stage of the pair form runs at
+// the tensor cores' rate (0.28 us for 256 x 256 x 128), one of the small form at the rate of its loads; a
+// pair costs a microsecond more to set up; adding sums across a cluster costs 1.6 us.  For example
+// 2048 x 4096 x 4096: pair 256 25.3 us, pair 128 26.9, small 128 41.0; 64 x 4096 x 4096: small 64 with
+// four splits 7.8, one split 9.3, pair 128 9.1; 1 x 4096 x 4096: small 32 with four splits 6.6, one 8.4.
+struct FormCost {
+  double fixed, wave, stage;
+};
+constexpr FormCost kPair256 = {3.1, 1.8, 0.281}, kPair128 = {2.75, 1.4, 0.155};
+constexpr FormCost kSmall32 = {-1.2, 3.5, 0.183}, kSmall64 = {-0.9, 3.7, 0.188}, kSmall128 = {-0.5, 4.1, 0.224};
+constexpr double kSplitCost = 1.6, kBytesPerUs = 7.2e6;
+
+struct Form {
+  bool pair;
+  int tokens, splits;
+};
+
+template <typename T>
+Form choose_form(int M, int N, int K, int sms, const mg::Options& opt) {
+  const double stages = (K + 127) / 128;
+  const double bytes = ((double)N * K + (double)M * K + (double)sizeof(T) * M * N) / kBytesPerUs;
+  Form best = {true, 256, 1};
+  double least = 1e300;
+  auto offer = [&](const Form& f, const FormCost& c, double tiles, int capacity, double extra) {
+    const double waves = std::ceil(tiles / capacity), compute = waves * std::ceil(stages / f.splits) * c.stage;
+    const double t = c.fixed + extra + waves * c.wave + std::sqrt(compute * compute + bytes * bytes);
+    if (t < least) {
+      least = t;
+      best = f;
+    }
+  };
+  auto tiles = [&](int channels, int tokens) { return std::ceil((double)N / channels) * std::ceil((double)M / tokens); };
+  if (opt.int8_pair != 0) {
+    if (opt.int8_pair != 128) offer({true, 256, 1}, kPair256, tiles(256, 256), sms / 2, 0);
+    if (opt.int8_pair <= 128) offer({true, 128, 1}, kPair128, tiles(256, 128), sms / 2, 0);
+  }
+  if (opt.int8_pair <= 0) {
+    for (int splits = 1; splits <= kMaxSplit && splits <= stages; splits *= 2) {
+      if (opt.int8_split > 0 && opt.int8_split != splits && !(opt.int8_split > splits && splits * 2 > stages)) continue;
+      for (int tokens = 32; tokens <= 128; tokens *= 2) {
+        if (opt.int8_tokens > 0 && opt.int8_tokens != tokens) continue;
+        if ((double)M / tokens > 65535) continue;  // (the grid's second dimension)
+        const int capacity = tokens == 32   ? small_capacity<32, T>(splits, sms)
+                             : tokens == 64 ? small_capacity<64, T>(splits, sms)
+                                            : small_capacity<128, T>(splits, sms);
+        if (capacity < 1) continue;
+        const FormCost& c = tokens == 32 ? kSmall32 : tokens == 64 ? kSmall64 : kSmall128;
+        offer({false, tokens, splits}, c, tiles(kRows, tokens), capacity, splits > 1 ? kSplitCost : 0);
+      }
+    }
+  }
+  return best;
+}
+
 template <typename T>
 int launch_int8(const Int8Params& p, const int8_t* A, size_t lda, const int8_t* B, size_t ldb, int K, int sms,
                 cudaStream_t st) {
-  const mg::Options opt = mg::options();
+  const Form f = choose_form<T>(p.M, p.N, K, sms, mg::options());
   CUtensorMap w, t;
   int rc;
-  const int pair = opt.int8_pair >= 0 ? opt.int8_pair : p.M > 128 ? 256 : 0;
-  if (pair > 0) {
-    const int bt = pair == 128 ? 128 : 256;
-    if ((rc = mg::make_map(&w, CU_TENSOR_MAP_DATA_TYPE_UINT8, B, K, p.N, ldb, 128, 128))) return rc;
-    if ((rc = mg::make_map(&t, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, K, p.M, lda, 128, bt / 2))) return rc;
-    return bt == 128 ? launch_pair<128, T>(p, w, t, sms, st) : launch_pair<256, T>(p, w, t, sms, st);
-  }
-  int bt = p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
-  if (opt.int8_tokens == 32 || opt.int8_tokens == 64 || opt.int8_tokens == 128) bt = opt.int8_tokens;
-  const int tiles = ((p.N + kRows - 1) / kRows) * ((p.M + bt - 1) / bt);
-  int splits = 1;
-  while (splits < kMaxSplit && tiles * splits * 2 <= sms && p.stages >= splits * 4) splits *= 2;
-  if (opt.int8_split > 0) splits = opt.int8_split >= 8 ? 8 : opt.int8_split >= 4 ? 4 : opt.int8_split >= 2 ? 2 : 1;
-  while (splits > p.stages) splits /= 2;
-  if ((p.M + bt - 1) / bt > 65535) return MG_ERR_SHAPE;
-  if ((rc = mg::make_map(&w, CU_TENSOR_MAP_DATA_TYPE_UINT8, B, K, p.N, ldb, 128, kRows))) return rc;
-  if ((rc = mg::make_map(&t, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, K, p.M, lda, 128, bt))) return rc;
-  if (bt == 32) return launch_small<32, T>(p, w, t, splits, st);
-  if (bt == 64) return launch_small<64, T>(p, w, t, splits, st);
-  return launch_small<128, T>(p, w, t, splits, st);
+  if ((rc = mg::make_map(&w, CU_TENSOR_MAP_DATA_TYPE_UINT8, B, K, p.N, ldb, 128, 128))) return rc;
+  if ((rc = mg::make_map(&t, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, K, p.M, lda, 128, f.pair ? f.tokens / 2 : f.tokens))) return rc;
+  if (f.pair) return f.tokens == 128 ? launch_pair<128, T>(p, w, t, sms, st) : launch_pair<256, T>(p, w, t, sms, st);
+  if (f.tokens == 32) return launch_small<32, T>(p, w, t, f.splits, st);
+  if (f.tokens == 64) return launch_small<64, T>(p, w, t, f.splits, st);
+  return launch_small<128, T>(p, w, t, f.splits, st);
 }
 
 }  // namespace

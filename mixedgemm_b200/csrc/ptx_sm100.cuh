@@ -209,6 +209,9 @@ __device__ __forceinline__ uint32_t nclusters_x() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The two halves of it, for work in between.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // Address of the same shared-memory location in CTA `cta` of the cluster.
 __device__ __forceinline__ uint32_t map_to_cta(uint32_t saddr, uint32_t cta) {
   uint32_t r;
