@@ -11,6 +11,9 @@ Differences from the reference binding, all deliberate:
     multiple of 128;
   * errors surface as RuntimeError (MixedGemmError), as the reference's std::runtime_error do.
 """
+import contextlib
+import ctypes
+
 import torch
 
 from . import _capi
@@ -20,12 +23,25 @@ def _stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+_HERE = contextlib.nullcontext()
+
+
+def _device(dev):
+    """`with` block in which `dev` is current; free of charge in the usual case, where it is current already."""
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
 def _ptr(t):
     return t.data_ptr() if t is not None and t.numel() > 0 else None
 
 
 def sf_bytes(rows, kseg):
     return _capi.load().mg_sf_bytes(rows, kseg)
+
+
+def _sf_bytes(rows, kseg):
+    """mg_sf_bytes without the call into the library (checks and allocations ask for it many times)."""
+    return -(-rows // 128) * -(-kseg // 128) * 512 if rows > 0 and kseg > 0 else 0
 
 
 def _check_in(X, reorder_index, KN, KS, KO, what):
@@ -39,7 +55,7 @@ def _check_in(X, reorder_index, KN, KS, KO, what):
 
 def _alloc_codes(rows, logical, pitch, device):
     """[rows, logical] uint8 view of a buffer whose rows are `pitch` bytes apart."""
-    buf = torch.empty((rows, pitch), dtype=torch.uint8, device=device)
+    buf = torch.empty_strided((rows, pitch), (pitch, 1), dtype=torch.uint8, device=device)
     return buf[:, :logical] if pitch != logical else buf
 
 
@@ -48,14 +64,14 @@ def alloc_quantized_x(M, KN, KS, KO, device, padded=True, one_buffer=False):
     With padded=True the code tensors are row-pitched views (same shape, same contents) whose pitch
     the GEMM can read in place even when a segment is only a multiple of 64.  With one_buffer=True
     all six are carved out of a single allocation, so that one transfer moves them together."""
-    lib = _capi.load()
     u8 = dict(dtype=torch.uint8, device=device)
     logical = (KN // 2, KS // 4 * 3, KO)
-    pitch = [lib.mg_code_pitch(0, i, k) if padded else l for i, (k, l) in enumerate(zip((KN, KS, KO), logical))]
-    sf_len = [max(lib.mg_sf_bytes(M, k), (M // 128 + 1) * 128 * k // 32) for k in (KN, KS, KO)]
+    # mg_code_pitch, worked out here: a call into the library costs half of what a buffer does
+    pitch = [-(-k // 128) * n if padded else l for k, n, l in zip((KN, KS, KO), (64, 96, 128), logical)]
+    sf_len = [max(_sf_bytes(M, k), (M // 128 + 1) * 128 * k // 32) for k in (KN, KS, KO)]
     if not one_buffer:
         return tuple(_alloc_codes(M, l, p, device) for l, p in zip(logical, pitch)) + tuple(
-            torch.empty(n, **u8) for n in sf_len)
+            torch.empty_strided((n,), (1,), **u8) for n in sf_len)
     sizes = [M * p for p in pitch] + sf_len
     offs, off = [], 0
     for n in sizes:
@@ -83,13 +99,12 @@ def alloc_quantized_w(N, KN, KS, KO, device, padded=True):
 
 
 def _pitches(tensors):
-    import ctypes
-    return (ctypes.c_size_t * len(tensors))(*[t.stride(0) if t.size(1) else 0 for t in tensors])
+    return (ctypes.c_size_t * len(tensors))(*[t.stride()[0] if t.shape[1] else 0 for t in tensors])
 
 
 def _check_codes(tensors, what):
     for t in tensors:
-        if not t.is_cuda or t.dtype != torch.uint8 or t.dim() != 2 or (t.size(1) and t.stride(1) != 1):
+        if not t.is_cuda or t.dtype != torch.uint8 or t.dim() != 2 or (t.stride()[1] != 1 and t.shape[1]):
             raise RuntimeError("%s: code tensors must be 2-D CUDA uint8 with unit column stride" % what)
 
 
@@ -97,21 +112,21 @@ def _check_operands(A, B, what):
     """A = (AN, AS, AO, SFAN, SFAS, SFAO), B likewise for the weights.  The reference infers M, N and
     the K split from AN, BN, AS and AO alone (bindings.cpp:30-34); the kernels build tensor maps and
     whole-atom scale copies from those sizes, so every other tensor is held to them here."""
-    lib = _capi.load()
     _check_codes(tuple(A[:3]) + tuple(B[:3]), what)
-    M, N = A[0].size(0), B[0].size(0)
-    KN, KS, KO = A[0].size(1) * 2, A[1].size(1) * 4 // 3, A[2].size(1)
-    if A[1].size(0) != M or A[2].size(0) != M or B[1].size(0) != N or B[2].size(0) != N:
+    (M, an), (Ms, as_), (Mo, ao) = A[0].shape, A[1].shape, A[2].shape
+    (N, bn), (Ns, bs), (No, bo) = B[0].shape, B[1].shape, B[2].shape
+    KN, KS, KO = an * 2, as_ * 4 // 3, ao
+    if Ms != M or Mo != M or Ns != N or No != N:
         raise RuntimeError("%s: the three code tensors of an operand must have the same row count" % what)
-    if A[1].size(1) * 4 != KS * 3 or B[0].size(1) * 2 != KN or B[1].size(1) * 2 != KS or B[2].size(1) * 2 != KO:
+    if as_ * 4 != KS * 3 or bn * 2 != KN or bs * 2 != KS or bo * 2 != KO:
         raise RuntimeError("%s: code widths of the two operands do not describe the same K split" % what)
     dev = A[0].device
     for t, rows, k in ((A[3], M, KN), (A[4], M, KS), (A[5], M, KO), (B[3], N, KN), (B[4], N, KS), (B[5], N, KO)):
         if not t.is_cuda or t.dtype != torch.uint8 or not t.is_contiguous():
             raise RuntimeError("%s: scale tensors must be contiguous CUDA uint8 tensors" % what)
-        if t.numel() < lib.mg_sf_bytes(rows, k):
+        if t.numel() < _sf_bytes(rows, k):
             raise RuntimeError("%s: a scale tensor holds %d bytes, %d are read (whole 512-byte atoms)" % (
-                what, t.numel(), lib.mg_sf_bytes(rows, k)))
+                what, t.numel(), _sf_bytes(rows, k)))
     for t in tuple(A) + tuple(B):
         if t.device != dev:
             raise RuntimeError("%s: all operands must be on one device" % what)
@@ -141,7 +156,6 @@ def reorder_quantize_x_multi(problems):
     with `out` the six buffers to write (alloc_quantized_x) or None.  Every entry gives the bytes of
     its own reorder_quantize_x call; the CTAs are shared out in proportion to the sizes
     (mg_reorder_quantize_multi).  Returns the list of six-tuples."""
-    import ctypes
     lib = _capi.load()
     n = len(problems)
     if not 1 <= n <= 8:
@@ -202,7 +216,7 @@ def _workspace(dev, nbytes):
     512-byte aligned blocks; the kernels want 1024, so over-allocate and slice.)"""
     if nbytes == 0:
         return None, 0
-    key = (dev.type, dev.index, torch.cuda.current_stream(dev).cuda_stream)
+    key = (dev.type, dev.index, torch._C._cuda_getCurrentRawStream(dev.index))
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < nbytes + 1024:
         if torch.cuda.is_current_stream_capturing():
@@ -227,18 +241,18 @@ def matmul(AN, BN, AS, BS, AO, BO, SFAN, SFBN, SFAS, SFBS, SFAO, SFBO, out=None,
     if dt not in (torch.bfloat16, torch.float32):
         raise RuntimeError("matmul: output dtype must be bfloat16 or float32")
     D = out if out is not None else torch.empty((M, N), dtype=dt, device=dev)
-    if D.dim() != 2 or D.size(0) != M or D.size(1) != N or D.stride(1) != 1 or D.device != dev:
+    if tuple(D.shape) != (M, N) or D.stride()[1] != 1 or D.device != dev:
         raise RuntimeError("matmul: out must be [M,N] on the operands' device with unit column stride")
     if C is not None and (C.dtype != torch.bfloat16 or tuple(C.shape) != (M, N) or C.device != dev or
                           C.stride(1) != 1 or C.stride(0) != D.stride(0)):
         raise RuntimeError("matmul: C must be bf16 [M,N] on the operands' device with out's row pitch")
     pitches = _pitches((AN, BN, AS, BS, AO, BO))
-    with torch.cuda.device(dev):
+    with _device(dev):
         ws, wsb = _workspace(dev, lib.mg_matmul_pitched_workspace_bytes(M, N, KN, KS, KO, pitches))
         st = lib.mg_matmul_pitched(_ptr(AN), _ptr(BN), _ptr(AS), _ptr(BS), _ptr(AO), _ptr(BO), pitches,
                                    int(dt == torch.float32), M, N, KN, KS, KO, _ptr(C), _ptr(D), D.stride(0),
                                    _ptr(SFAN), _ptr(SFBN), _ptr(SFAS), _ptr(SFBS), _ptr(SFAO), _ptr(SFBO), ws, wsb,
-                                   _stream())
+                                   torch._C._cuda_getCurrentRawStream(dev.index))
     _capi.check(st, "matmul")
     return D
 
@@ -262,7 +276,6 @@ def matmul_group(A, Bs, outs=None):
     """Products of one quantised activation A = (AN, AS, AO, SFAN, SFAS, SFAO) with several quantised
     weights Bs = [(BN, BS, BO, SFBN, SFBS, SFBO), ...] (q/k/v, gate/up) in one launch where the
     grouped kernel applies, otherwise one matmul per weight.  Returns the list of [M, N_j] bf16 tensors."""
-    import ctypes
     lib = _capi.load()
     M = A[0].size(0)
     KN, KS, KO = A[0].size(1) * 2, A[1].size(1) * 4 // 3, A[2].size(1)
@@ -329,7 +342,6 @@ def matmul_multi(problems, flags=None):
     (mg_problem_t.ready_flags).  Problems the
     CTA-pair kernel does not take (M <= 128, N not a multiple of 256, buffers that need the padded
     copy) fall back to one matmul per problem; flags are then refused.  Returns the outputs."""
-    import ctypes
     lib = _capi.load()
     n = len(problems)
     outs = []
@@ -393,42 +405,50 @@ _ELEMENT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # MG_BF16, M
 
 
 def _on(dev, fn, *args):
-    """fn(*args, stream) with `dev` current; the usual case, `dev` being current already, costs nothing."""
-    if torch.cuda.current_device() == dev.index:
-        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
-    with torch.cuda.device(dev):
+    """fn(*args, current stream of `dev`) with `dev` current."""
+    with _device(dev):
         return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
 
 
-def _rows(t, what, name, dev=None, like=None, dtype=None):
-    """Row pitch (elements) of a 2-D CUDA tensor whose rows are dense and do not overlap."""
-    if not t.is_cuda or t.dim() != 2 or (dev is not None and t.device != dev):
-        raise RuntimeError("%s: %s must be a 2-D CUDA tensor%s" % (what, name, "" if dev is None else " on the others' device"))
-    if like is not None and t.shape != like:
-        raise RuntimeError("%s: %s has shape %s where %s is expected" % (what, name, tuple(t.shape), tuple(like)))
-    if dtype is not None and t.dtype != dtype:
-        raise RuntimeError("%s: %s must be %s, not %s" % (what, name, dtype, t.dtype))
-    M, K = t.shape
-    s0, s1 = t.stride()
-    if (s1 != 1 and K > 1) or (s0 < K and M > 1):
-        raise RuntimeError("%s: the rows of %s must have unit stride and must not overlap (strides %s)" % (what, name, (s0, s1)))
-    return s0 if M > 1 else K
+def _rows(t, what, name, shape, dev, dtype):
+    """Row pitch (elements) of a 2-D tensor whose rows are dense and do not overlap; `shape` None: any."""
+    own, step = t.shape, t.stride()
+    if len(own) == 2 and t.device == dev and t.dtype == dtype and (shape is None or own == shape):
+        M, K = own
+        if (step[1] == 1 or K <= 1) and (step[0] >= K or M <= 1):
+            return step[0] if M > 1 else K
+        raise RuntimeError("%s: the rows of %s must have unit stride and must not overlap (strides %s)" % (what, name, step))
+    raise RuntimeError("%s: %s must be a 2-D %s tensor%s on %s, not %s %s on %s" % (
+        what, name, dtype, "" if shape is None else " of shape %s" % (tuple(shape),), dev, t.dtype, tuple(own), t.device))
 
 
 def _vector(t, what, name, n, dev, dtype):
-    if not t.is_cuda or t.device != dev or t.dtype != dtype or t.numel() != n or not t.is_contiguous():
-        raise RuntimeError("%s: %s must be a contiguous %s tensor of %d elements on the others' device" % (what, name, dtype, n))
+    if t.device != dev or t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        raise RuntimeError("%s: %s must be a contiguous %s tensor of %d elements on %s" % (what, name, dtype, n, dev))
     return t
+
+
+def _activation(X, what):
+    """Device and row pitch of the activation that a call starts with."""
+    if not X.is_cuda:
+        raise RuntimeError("%s: X must be a CUDA tensor" % what)
+    if X.dtype not in _ELEMENT:
+        raise RuntimeError("%s: X must be bfloat16, float16 or float32, not %s" % (what, X.dtype))
+    dev = X.device
+    return dev, _rows(X, what, "X", None, dev, X.dtype)
+
+
+def _new(shape, dtype, dev):
+    return torch.empty_strided(shape, (shape[1], 1) if len(shape) == 2 else (1,), dtype=dtype, device=dev)
 
 
 def _int8_outputs(M, K, dev, out, what):
     """(codes, row pitch, scale): the caller's, or new ones whose rows matmul_int8 can read in place."""
     if out is None:
         pitch = (K + 15) // 16 * 16
-        return (torch.empty_strided((M, K), (pitch, 1), dtype=torch.int8, device=dev), pitch,
-                torch.empty(M, dtype=torch.float32, device=dev))
+        return (torch.empty_strided((M, K), (pitch, 1), dtype=torch.int8, device=dev), pitch, _new((M,), torch.float32, dev))
     q, scale = out
-    return q, _rows(q, what, "the codes", dev, (M, K), torch.int8), _vector(scale, what, "the scale", M, dev, torch.float32)
+    return q, _rows(q, what, "the codes", (M, K), dev, torch.int8), _vector(scale, what, "the scale", M, dev, torch.float32)
 
 
 def quantize_int8(X, out=None):
@@ -437,12 +457,10 @@ def quantize_int8(X, out=None):
     magnitude of the row / 127, codes rounded to nearest even.  The rows of X may be any distance
     apart; those of the codes start on 16-byte boundaries, as matmul_int8 needs them.  A row with a
     value that is not finite gets the scale NaN and codes 0.  `out` = (codes, scale) to write into."""
-    ldx = _rows(X, "quantize_int8", "X")
-    if X.dtype not in _ELEMENT:
-        raise RuntimeError("quantize_int8: X must be bfloat16, float16 or float32, not %s" % X.dtype)
+    dev, ldx = _activation(X, "quantize_int8")
     M, K = X.shape
-    q, ldq, scale = _int8_outputs(M, K, X.device, out, "quantize_int8")
-    st = _on(X.device, _capi.load().mg_quantize_int8, X.data_ptr(), _ELEMENT[X.dtype], M, K, ldx, q.data_ptr(), ldq,
+    q, ldq, scale = _int8_outputs(M, K, dev, out, "quantize_int8")
+    st = _on(dev, _capi.load().mg_quantize_int8, X.data_ptr(), _ELEMENT[X.dtype], M, K, ldx, q.data_ptr(), ldq,
              scale.data_ptr())
     if st:
         _capi.check(st, "quantize_int8")
@@ -450,18 +468,17 @@ def quantize_int8(X, out=None):
 
 
 def _norm_inputs(X, weight, residual, residual_out, what):
-    """Checks of the fused norms; returns (ldx, ldr, residual_out, ldu)."""
-    ldx = _rows(X, what, "X")
-    _vector(weight, what, "the norm's weight", X.size(1), X.device, X.dtype)
+    """Checks of the fused norms; returns (device, ldx, ldr, residual_out, ldu)."""
+    dev, ldx = _activation(X, what)
+    _vector(weight, what, "the norm's weight", X.shape[1], dev, X.dtype)
     if residual is None:
         if residual_out is not None:
             raise RuntimeError("%s: residual_out without a residual" % what)
-        return ldx, 0, None, 0
-    ldr = _rows(residual, what, "the residual", X.device, X.shape, X.dtype)
+        return dev, ldx, 0, None, 0
+    ldr = _rows(residual, what, "the residual", X.shape, dev, X.dtype)
     if residual_out is None:
-        residual_out = torch.empty(X.shape, dtype=X.dtype, device=X.device)
-        return ldx, ldr, residual_out, X.size(1)
-    return ldx, ldr, residual_out, _rows(residual_out, what, "residual_out", X.device, X.shape, X.dtype)
+        return dev, ldx, ldr, _new(X.shape, X.dtype, dev), X.shape[1]
+    return dev, ldx, ldr, residual_out, _rows(residual_out, what, "residual_out", X.shape, dev, X.dtype)
 
 
 def rms_norm_int8(X, weight, eps=1e-6, residual=None, residual_out=None, out=None):
@@ -471,12 +488,10 @@ def rms_norm_int8(X, weight, eps=1e-6, residual=None, residual_out=None, out=Non
     weight [K] and residual [M,K] have X's type; residual_out may be `residual` (or X) itself, to
     update the stream in place.  A row whose sum of squares is not a finite fp32 number gets the
     scale NaN and codes 0."""
-    ldx, ldr, u, ldu = _norm_inputs(X, weight, residual, residual_out, "rms_norm_int8")
-    if X.dtype not in _ELEMENT:
-        raise RuntimeError("rms_norm_int8: X must be bfloat16, float16 or float32, not %s" % X.dtype)
+    dev, ldx, ldr, u, ldu = _norm_inputs(X, weight, residual, residual_out, "rms_norm_int8")
     M, K = X.shape
-    q, ldq, scale = _int8_outputs(M, K, X.device, out, "rms_norm_int8")
-    st = _on(X.device, _capi.load().mg_rms_norm_int8, X.data_ptr(), None if u is None else residual.data_ptr(),
+    q, ldq, scale = _int8_outputs(M, K, dev, out, "rms_norm_int8")
+    st = _on(dev, _capi.load().mg_rms_norm_int8, X.data_ptr(), None if u is None else residual.data_ptr(),
              weight.data_ptr(), eps, _ELEMENT[X.dtype], M, K, ldx, ldr, None if u is None else u.data_ptr(), ldu,
              q.data_ptr(), ldq, scale.data_ptr())
     if st:
@@ -492,24 +507,22 @@ def rms_norm_reorder_quantize_x(X, weight, reorder_index, KN, KS, KO, eps=1e-6, 
     may be `residual` (or X) itself; `out` the six buffers of alloc_quantized_x().  Rows start on
     16-byte boundaries.  A row with a sum of squares or an h that is not finite gets NaN scales."""
     what = "rms_norm_reorder_quantize_x"
-    ldx, ldr, u, ldu = _norm_inputs(X, weight, residual, residual_out, what)
+    dev, ldx, ldr, u, ldu = _norm_inputs(X, weight, residual, residual_out, what)
     M, K = X.shape
     if X.dtype != torch.bfloat16:
         raise RuntimeError("%s: X must be bfloat16, not %s" % (what, X.dtype))
     if K != KN + KS + KO:
         raise RuntimeError("%s: K = %d does not match KN+KS+KO" % (what, K))
-    dev = X.device
     _vector(reorder_index, what, "reorder_index", K, dev, torch.int16)
     if out is None:
         out = alloc_quantized_x(M, KN, KS, KO, dev)
     else:
-        lib = _capi.load()
         _check_codes(out[:3], what)
         for t, n in zip(out[:3], (KN // 2, KS // 4 * 3, KO)):
             if tuple(t.shape) != (M, n) or t.device != dev:
                 raise RuntimeError("%s: a code buffer has shape %s where %s is expected" % (what, tuple(t.shape), (M, n)))
         for t, k in zip(out[3:], (KN, KS, KO)):
-            if t.numel() < lib.mg_sf_bytes(M, k) or t.device != dev or t.dtype != torch.uint8 or not t.is_contiguous():
+            if t.numel() < _sf_bytes(M, k) or t.device != dev or t.dtype != torch.uint8 or not t.is_contiguous():
                 raise RuntimeError("%s: a scale buffer is too small or on another device" % what)
     XN, XS, XO, s4, s6, s8 = out
     st = _on(dev, _capi.load().mg_rms_norm_reorder_quantize, X.data_ptr(), ldx, None if u is None else residual.data_ptr(),
@@ -526,24 +539,26 @@ def matmul_int8(A, B, scale_a, scale_b, bias=None, out=None, out_dtype=None):
     `out_dtype` (bfloat16 unless given; float16 or float32).  scale_a [M], scale_b [N] and bias [N]
     are fp32.  Rows of A and B start on 16-byte boundaries (those of quantize_int8 do); K is at most
     131071.  `out` [M,N] receives the result instead of a new tensor; its rows may be any distance apart."""
-    lda = _rows(A, "matmul_int8", "A", dtype=torch.int8)
+    what = "matmul_int8"
+    if not A.is_cuda:
+        raise RuntimeError("%s: A must be a CUDA tensor" % what)
     dev = A.device
-    ldb = _rows(B, "matmul_int8", "B", dev, dtype=torch.int8)
+    lda = _rows(A, what, "A", None, dev, torch.int8)
+    ldb = _rows(B, what, "B", None, dev, torch.int8)
     M, K = A.shape
-    N = B.size(0)
-    if B.size(1) != K:
-        raise RuntimeError("matmul_int8: A has rows of %d elements, B of %d" % (K, B.size(1)))
-    _vector(scale_a, "matmul_int8", "scale_a", M, dev, torch.float32)
-    _vector(scale_b, "matmul_int8", "scale_b", N, dev, torch.float32)
+    N, Kb = B.shape
+    if Kb != K:
+        raise RuntimeError("%s: A has rows of %d elements, B of %d" % (what, K, Kb))
+    _vector(scale_a, what, "scale_a", M, dev, torch.float32)
+    _vector(scale_b, what, "scale_b", N, dev, torch.float32)
     if bias is not None:
-        _vector(bias, "matmul_int8", "the bias", N, dev, torch.float32)
+        _vector(bias, what, "the bias", N, dev, torch.float32)
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype or torch.bfloat16, device=dev)
-        ldd = N
+        out, ldd = _new((M, N), out_dtype or torch.bfloat16, dev), N
     else:
-        ldd = _rows(out, "matmul_int8", "out", dev, (M, N), out_dtype)
+        ldd = _rows(out, what, "out", (M, N), dev, out_dtype or out.dtype)
     if out.dtype not in _ELEMENT:
-        raise RuntimeError("matmul_int8: the result must be bfloat16, float16 or float32, not %s" % out.dtype)
+        raise RuntimeError("%s: the result must be bfloat16, float16 or float32, not %s" % (what, out.dtype))
     st = _on(dev, _capi.load().mg_matmul_int8, A.data_ptr(), lda, B.data_ptr(), ldb, scale_a.data_ptr(),
              scale_b.data_ptr(), None if bias is None else bias.data_ptr(), M, N, K, out.data_ptr(),
              _ELEMENT[out.dtype], ldd)
@@ -567,7 +582,6 @@ def set_wait_limit_us(us):
 
 def device_status():
     """Reads and clears the device error word (non-zero after a kernel gave up on a bounded wait)."""
-    import ctypes
     lib = _capi.load()
     v = ctypes.c_int(0)
     st = lib.mg_device_status(ctypes.byref(v), _stream())

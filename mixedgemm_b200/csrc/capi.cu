@@ -80,6 +80,7 @@ int device_info(DeviceInfo* out) {
     MG_CUDA_TRY(cudaDeviceGetAttribute(&di.sm_count, cudaDevAttrMultiProcessorCount, dev));
     MG_CUDA_TRY(cudaDeviceGetAttribute(&di.smem_optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev));
     MG_CUDA_TRY(cudaDeviceGetAttribute(&di.cc_major, cudaDevAttrComputeCapabilityMajor, dev));
+    di.device = dev;
     g_info[dev] = di;
     g_info_ok[dev] = true;
   }

@@ -498,10 +498,12 @@ int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tm
 }
 
 template <int BT, typename T>
-int launch_pair(const Int8Params& p, const CUtensorMap& w, const CUtensorMap& t, int sms, cudaStream_t st) {
+int launch_pair(const Int8Params& p, const CUtensorMap& w, const CUtensorMap& t, const mg::DeviceInfo& di, cudaStream_t st) {
   using C = PairCfg<BT>;
   auto kern = int8_gemm_pair_kernel<BT, T>;
-  MG_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+  static std::atomic<unsigned long long> allowed;
+  MG_CUDA_TRY(mg::allow_smem(kern, C::SMEM, di.device, allowed));
+  const int sms = di.sm_count;
   const int tiles = ((p.N + 255) / 256) * ((p.M + BT - 1) / BT);
   const int clusters = tiles < sms / 2 ? tiles : sms / 2;
   MG_CUDA_TRY(mg::launch_kernel(kern, dim3(clusters * 2), dim3(kThreads), C::SMEM, st, p, w, t));
@@ -509,11 +511,13 @@ int launch_pair(const Int8Params& p, const CUtensorMap& w, const CUtensorMap& t,
 }
 
 template <int BT, typename T>
-int launch_small(const Int8Params& p, const CUtensorMap& w, const CUtensorMap& t, int splits, cudaStream_t st) {
+int launch_small(const Int8Params& p, const CUtensorMap& w, const CUtensorMap& t, int splits, const mg::DeviceInfo& di,
+                 cudaStream_t st) {
   using C = SmallCfg<BT>;
   auto kern = int8_gemm_kernel<BT, T>;
   const size_t smem = C::smem(splits);
-  MG_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::smem(kMaxSplit)));
+  static std::atomic<unsigned long long> allowed;
+  MG_CUDA_TRY(mg::allow_smem(kern, C::smem(kMaxSplit), di.device, allowed));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((p.N + kRows - 1) / kRows, (p.M + BT - 1) / BT, splits);
   cfg.blockDim = dim3(kThreads);
@@ -535,12 +539,10 @@ int launch_small(const Int8Params& p, const CUtensorMap& w, const CUtensorMap& t
 // How many clusters of `splits` such CTAs the device holds at one time (asked once per device and shape;
 // 0 where it holds none).
 template <int BT, typename T>
-int small_capacity(int splits, int sms) {
-  if (splits == 1) return sms;
-  static std::atomic<int> known[64][4];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-  std::atomic<int>& slot = known[dev][splits == 2 ? 0 : splits == 4 ? 1 : 2];
+int small_capacity(int splits, const mg::DeviceInfo& di) {
+  if (splits == 1) return di.sm_count;
+  static std::atomic<int> known[64][3];
+  std::atomic<int>& slot = known[di.device][splits == 2 ? 0 : splits == 4 ? 1 : 2];
   int k = slot.load();
   if (k == 0) {
     using C = SmallCfg<BT>;
@@ -589,7 +591,8 @@ struct Form {
 };
 
 template <typename T>
-Form choose_form(int M, int N, int K, int sms, const mg::Options& opt) {
+Form choose_form(int M, int N, int K, const mg::DeviceInfo& di, const mg::Options& opt) {
+  const int sms = di.sm_count;
   const double stages = (K + 127) / 128;
   const double bytes = ((double)N * K + (double)M * K + (double)sizeof(T) * M * N) / kBytesPerUs;
   Form best = {true, 256, 1};
@@ -613,9 +616,9 @@ Form choose_form(int M, int N, int K, int sms, const mg::Options& opt) {
       for (int tokens = 32; tokens <= 128; tokens *= 2) {
         if (opt.int8_tokens > 0 && opt.int8_tokens != tokens) continue;
         if ((double)M / tokens > 65535) continue;  // (the grid's second dimension)
-        const int capacity = tokens == 32   ? small_capacity<32, T>(splits, sms)
-                             : tokens == 64 ? small_capacity<64, T>(splits, sms)
-                                            : small_capacity<128, T>(splits, sms);
+        const int capacity = tokens == 32   ? small_capacity<32, T>(splits, di)
+                             : tokens == 64 ? small_capacity<64, T>(splits, di)
+                                            : small_capacity<128, T>(splits, di);
         if (capacity < 1) continue;
         const FormCost& c = tokens == 32 ? kSmall32 : tokens == 64 ? kSmall64 : kSmall128;
         offer({false, tokens, splits}, c, tiles(kRows, tokens), capacity, splits > 1 ? kSplitCost : 0);
@@ -626,17 +629,17 @@ Form choose_form(int M, int N, int K, int sms, const mg::Options& opt) {
 }
 
 template <typename T>
-int launch_int8(const Int8Params& p, const int8_t* A, size_t lda, const int8_t* B, size_t ldb, int K, int sms,
-                cudaStream_t st) {
-  const Form f = choose_form<T>(p.M, p.N, K, sms, mg::options());
+int launch_int8(const Int8Params& p, const int8_t* A, size_t lda, const int8_t* B, size_t ldb, int K,
+                const mg::DeviceInfo& di, cudaStream_t st) {
+  const Form f = choose_form<T>(p.M, p.N, K, di, mg::options());
   CUtensorMap w, t;
   int rc;
   if ((rc = mg::make_map(&w, CU_TENSOR_MAP_DATA_TYPE_UINT8, B, K, p.N, ldb, 128, 128))) return rc;
   if ((rc = mg::make_map(&t, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, K, p.M, lda, 128, f.pair ? f.tokens / 2 : f.tokens))) return rc;
-  if (f.pair) return f.tokens == 128 ? launch_pair<128, T>(p, w, t, sms, st) : launch_pair<256, T>(p, w, t, sms, st);
-  if (f.tokens == 32) return launch_small<32, T>(p, w, t, f.splits, st);
-  if (f.tokens == 64) return launch_small<64, T>(p, w, t, f.splits, st);
-  return launch_small<128, T>(p, w, t, f.splits, st);
+  if (f.pair) return f.tokens == 128 ? launch_pair<128, T>(p, w, t, di, st) : launch_pair<256, T>(p, w, t, di, st);
+  if (f.tokens == 32) return launch_small<32, T>(p, w, t, f.splits, di, st);
+  if (f.tokens == 64) return launch_small<64, T>(p, w, t, f.splits, di, st);
+  return launch_small<128, T>(p, w, t, f.splits, di, st);
 }
 
 }  // namespace
@@ -673,7 +676,7 @@ extern "C" int mg_matmul_int8(const int8_t* A, size_t lda, const int8_t* B, size
   p.wait_cycles = mg::wait_limit_cycles();
   if ((rc = mg::device_status_word(&p.status)) != MG_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == MG_BF16) return launch_int8<__nv_bfloat16>(p, A, lda, B, ldb, K, di.sm_count, st);
-  if (dtype == MG_FP16) return launch_int8<__half>(p, A, lda, B, ldb, K, di.sm_count, st);
-  return launch_int8<float>(p, A, lda, B, ldb, K, di.sm_count, st);
+  if (dtype == MG_BF16) return launch_int8<__nv_bfloat16>(p, A, lda, B, ldb, K, di, st);
+  if (dtype == MG_FP16) return launch_int8<__half>(p, A, lda, B, ldb, K, di, st);
+  return launch_int8<float>(p, A, lda, B, ldb, K, di, st);
 }

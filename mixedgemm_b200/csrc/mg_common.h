@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <utility>
 
 #include "mixedgemm_c.h"
@@ -23,6 +24,7 @@ struct DeviceInfo {
   int sm_count;
   int smem_optin;
   int cc_major;
+  int device;  // index of the device these are of, below 64
 };
 int device_info(DeviceInfo* out);
 
@@ -76,6 +78,16 @@ cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+// Raises a kernel's limit of dynamic shared memory, once per device (`done`: one bit for each, kept by the caller).
+template <typename... KArgs>
+cudaError_t allow_smem(void (*kernel)(KArgs...), size_t bytes, int device, std::atomic<unsigned long long>& done) {
+  const unsigned long long bit = 1ull << device;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 static inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }

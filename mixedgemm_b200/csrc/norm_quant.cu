@@ -20,6 +20,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "mg_common.h"
 #include "ptx_sm100.cuh"
 
@@ -27,8 +29,6 @@ namespace {
 
 constexpr float kTiny = 0x1p-100f;
 
-// Most threads of a CTA whose threads hold `held` values in registers.
-constexpr int max_threads(int held) { return held >= 64 ? 512 : 1024; }
 
 struct RowQuantParams {
   const void* X;
@@ -64,61 +64,84 @@ struct Elem<float> {
   using Raw = uint32_t;
 };
 
-// CH elements of one chunk <-> fp32.  Aligned chunks are whole 16-byte vectors; the others hold four
-// elements that are moved one by one, those beyond `n` reading as zero.
-template <typename T, bool ALIGNED, int CH>
-__device__ __forceinline__ void load_chunk(const void* row, int e0, int n, float (&f)[CH]) {
-  using Raw = typename Elem<T>::Raw;
-  if constexpr (ALIGNED) {
-    static_assert(CH * sizeof(Raw) == 16, "a chunk is one vector");
-    union {
-      uint4 v;
-      Raw e[CH];
-    } u;
-    u.v = *reinterpret_cast<const uint4*>(static_cast<const Raw*>(row) + e0);
-#pragma unroll
-    for (int j = 0; j < CH; ++j) f[j] = Elem<T>::up(u.e[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < CH; ++j) f[j] = j < n ? Elem<T>::up(static_cast<const Raw*>(row)[e0 + j]) : 0.f;
-  }
-}
+template <typename T, bool ALIGNED>
+constexpr int kChunk = ALIGNED ? 16 / (int)sizeof(typename Elem<T>::Raw) : 4;
 
-template <typename T, bool ALIGNED, int CH>
-__device__ __forceinline__ void store_chunk(void* row, int e0, int n, const float (&f)[CH]) {
+// A chunk of a row as it lies in memory: a whole 16-byte vector, or four elements that are moved one by
+// one (those beyond the row's end read as zero).
+template <typename T, bool ALIGNED>
+struct Chunk {
   using Raw = typename Elem<T>::Raw;
-  if constexpr (ALIGNED) {
-    union {
-      uint4 v;
-      Raw e[CH];
-    } u;
-#pragma unroll
-    for (int j = 0; j < CH; ++j) u.e[j] = Elem<T>::down(f[j]);
-    *reinterpret_cast<uint4*>(static_cast<Raw*>(row) + e0) = u.v;
-  } else {
-#pragma unroll
-    for (int j = 0; j < CH; ++j)
-      if (j < n) static_cast<Raw*>(row)[e0 + j] = Elem<T>::down(f[j]);
-  }
-}
+  static constexpr int CH = kChunk<T, ALIGNED>;
+  union {
+    uint4 v;
+    Raw e[16 / sizeof(Raw)];
+  };
 
-// rint(fl(p * f)) of four values as the four bytes of a word: adding 1.5 * 2^23 leaves the integer,
-// rounded to nearest even, in the low mantissa bits.
-__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float f) {
+  __device__ __forceinline__ void load(const Raw* row, int e0, int n) {
+    if constexpr (ALIGNED) {
+      v = *reinterpret_cast<const uint4*>(row + e0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < CH; ++j) e[j] = j < n ? row[e0 + j] : (Raw)0;
+    }
+  }
+  __device__ __forceinline__ void load_const(const Raw* row, int e0, int n) {  // never written while the kernel runs
+    if constexpr (ALIGNED) {
+      v = __ldg(reinterpret_cast<const uint4*>(row + e0));
+    } else {
+#pragma unroll
+      for (int j = 0; j < CH; ++j) e[j] = j < n ? __ldg(row + e0 + j) : (Raw)0;
+    }
+  }
+  __device__ __forceinline__ void store(Raw* row, int e0, int n) const {
+    if constexpr (ALIGNED) {
+      *reinterpret_cast<uint4*>(row + e0) = v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < CH; ++j)
+        if (j < n) row[e0 + j] = e[j];
+    }
+  }
+  __device__ __forceinline__ float at(int j) const { return Elem<T>::up(e[j]); }
+  __device__ __forceinline__ void add(const Chunk& r) {  // the one rounding of the stream
+#pragma unroll
+    for (int j = 0; j < CH; ++j) e[j] = Elem<T>::down(at(j) + r.at(j));
+  }
+};
+
+// The code of p f in the low byte: adding 1.5 * 2^23 leaves the integer, rounded to nearest even, in the low
+// mantissa bits.  The plain form rounds the product first, which is its definition; behind a norm p f
+// is not more exact than that rounding, and one instruction does both.
+template <bool NORM>
+__device__ __forceinline__ uint32_t code(float p, float f) {
   const float kMagic = 12582912.0f;
-  const uint32_t ia = __float_as_uint(__fadd_rn(__fmul_rn(a, f), kMagic));
-  const uint32_t ib = __float_as_uint(__fadd_rn(__fmul_rn(b, f), kMagic));
-  const uint32_t ic = __float_as_uint(__fadd_rn(__fmul_rn(c, f), kMagic));
-  const uint32_t id = __float_as_uint(__fadd_rn(__fmul_rn(d, f), kMagic));
-  return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
+  return __float_as_uint(NORM ? __fmaf_rn(p, f, kMagic) : __fadd_rn(__fmul_rn(p, f), kMagic));
+}
+template <bool NORM>
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float f) {
+  return __byte_perm(__byte_perm(code<NORM>(a, f), code<NORM>(b, f), 0x0040),
+                     __byte_perm(code<NORM>(c, f), code<NORM>(d, f), 0x0040), 0x5410);
 }
 
-template <bool ALIGNED, int CH>
+// max(top, |a|, |b|), NaN when one of them is.
+__device__ __forceinline__ float max_abs(float top, float a, float b) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(top), "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+template <bool NORM, bool ALIGNED, int CH>
 __device__ __forceinline__ void store_codes(int8_t* q, int n, const float (&p)[CH], float f, bool bad) {
   uint32_t w[CH / 4];
 #pragma unroll
   for (int j = 0; j < CH / 4; ++j)
-    w[j] = bad ? 0u : codes4(p[j * 4], p[j * 4 + 1], p[j * 4 + 2], p[j * 4 + 3], f);
+    w[j] = bad ? 0u : codes4<NORM>(p[j * 4], p[j * 4 + 1], p[j * 4 + 2], p[j * 4 + 3], f);
   if constexpr (CH == 8) {
     *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
   } else {
@@ -132,142 +155,227 @@ __device__ __forceinline__ void store_codes(int8_t* q, int n, const float (&p)[C
   }
 }
 
-// Sum and integer maximum over the threads of a row: blockDim.x lanes, one or more whole warps.
-__device__ __forceinline__ void reduce_row(float& sum, uint32_t& top, int warps, float* s_sum, uint32_t* s_top) {
+// Sum and maximum over the threads of a row: blockDim.x lanes, one or more whole warps.  The
+// caller alternates between two sets of shared words, so that one barrier per row is enough.
+struct RowShared {
+  float sum[32];
+  float top[32];
+};
+
+__device__ __forceinline__ void reduce_row(float& sum, float& top, int warps, RowShared& sh) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   }
   if (warps == 1) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (lane == 0) {
-    s_sum[warp] = sum;
-    s_top[warp] = top;
+    sh.sum[warp] = sum;
+    sh.top[warp] = top;
   }
   __syncthreads();
-  sum = lane < warps ? s_sum[lane] : 0.f;
-  top = lane < warps ? s_top[lane] : 0u;
+  sum = lane < warps ? sh.sum[lane] : 0.f;
+  top = lane < warps ? sh.top[lane] : 0.f;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   }
 }
 
-// One row for blockDim.x threads (blockDim.y rows per CTA when a row is one warp's).  CPT chunks per
-// thread stay in registers; CPT = 0 is the form for rows that do not fit, which reads them twice.
-template <typename T, bool ALIGNED>
-constexpr int kChunk = ALIGNED ? 16 / (int)sizeof(typename Elem<T>::Raw) : 4;
+// What a row's statistics make of it: codes = rint(u w f), scale.
+struct RowScale {
+  float f, scale;
+  bool bad;
+};
 
-template <typename T, bool NORM, bool ALIGNED, int CPT>
-__global__ void __launch_bounds__(max_threads(CPT * kChunk<T, ALIGNED>)) row_quant_kernel(const RowQuantParams p) {
-  constexpr int CH = kChunk<T, ALIGNED>;
-  using Raw = typename Elem<T>::Raw;
-  __shared__ float s_sum[32];
-  __shared__ uint32_t s_top[32];
-  ptx::grid_dep_launch_dependents();
-  ptx::grid_dep_wait();
-  const int row = (int)(blockIdx.x * blockDim.y + threadIdx.y);
-  if (row >= p.M) return;  // whole warps; with several warps to a row blockDim.y is 1
-  const int K = p.K, nt = blockDim.x, warps = nt >> 5;
-  const Raw* x = static_cast<const Raw*>(p.X) + (size_t)row * p.px;
-  const Raw* r = p.R ? static_cast<const Raw*>(p.R) + (size_t)row * p.pr : nullptr;
-  Raw* u = p.R ? static_cast<Raw*>(p.U) + (size_t)row * p.pu : nullptr;
-  int8_t* q = p.Q + (size_t)row * p.pq;
-  const int chunks = (K + CH - 1) / CH;
-
-  float sum = 0.f;
-  uint32_t top = 0;
-  // one chunk: read, add, keep u w (or x) in f, and count it in
-  auto take = [&](int c, float (&f)[CH], bool count) {
-    const int e0 = c * CH, n = K - e0;
-    load_chunk<T, ALIGNED, CH>(x, e0, n, f);
-    if constexpr (NORM) {
-      if (r) {
-        float g[CH];
-        load_chunk<T, ALIGNED, CH>(r, e0, n, g);
-#pragma unroll
-        for (int j = 0; j < CH; ++j) f[j] = Elem<T>::up(Elem<T>::down(f[j] + g[j]));
-        if (!count || CPT > 0) store_chunk<T, ALIGNED, CH>(u, e0, n, f);
-      }
-      float w[CH];
-      load_chunk<T, ALIGNED, CH>(p.W, e0, n, w);
-#pragma unroll
-      for (int j = 0; j < CH; ++j) {
-        if (count) sum = fmaf(f[j], f[j], sum);
-        f[j] *= w[j];
-      }
-    }
-    if (count) {
-#pragma unroll
-      for (int j = 0; j < CH; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
-    }
-  };
-
-  float keep[CPT > 0 ? CPT : 1][CH];
-  if constexpr (CPT > 0) {
-#pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      const int c = i * nt + (int)threadIdx.x;
-      if (c < chunks) take(c, keep[i], true);
-    }
-  } else {
-    for (int c = threadIdx.x; c < chunks; c += nt) take(c, keep[0], true);
-  }
-  reduce_row(sum, top, warps, s_sum, s_top);
-
-  float v = 1.f, a = __uint_as_float(top);
-  bool bad = top >= 0x7f800000u;
+template <bool NORM>
+__device__ __forceinline__ RowScale row_scale(float sum, float top, const RowQuantParams& p) {
+  float v = 1.f, a = top;
+  bool bad = !(top <= 3.4028235e38f);
   if constexpr (NORM) {
     bad = bad || !(sum <= 3.4028235e38f);
-    v = rsqrtf(sum / (float)K + p.eps);
+    v = rsqrtf(sum / (float)p.K + p.eps);
     a *= v;
     bad = bad || !(a <= 3.4028235e38f);
   }
   a = fmaxf(a, kTiny);
-  const float f = v * (127.0f / a);
-  if (threadIdx.x == 0) p.S[row] = bad ? __uint_as_float(0x7fc00000u) : a / 127.0f;
-  if constexpr (CPT > 0) {
+  return {v * (127.0f / a), bad ? __uint_as_float(0x7fc00000u) : a / 127.0f, bad};
+}
+
+// Persistent: blockDim.x threads take a row at a time (blockDim.y rows side by side in a CTA when a row is
+// one warp's).  u w (or x) of a thread's CPT chunks stays in registers, in fp32, from the statistics to the
+// codes, and the next row's chunks are on their way while the row is reduced.
+// CPT = 0 is the form for rows that do not fit: it reads them twice.
+constexpr int max_threads(int cpt) { return cpt >= 4 ? 512 : 1024; }  // (registers)
+
+// MODE: plain, norm, or norm behind the residual's addition
+enum { kPlain = 0, kNorm = 1, kNormAdd = 2 };
+
+template <typename T, int MODE, bool ALIGNED, int CPT>
+__global__ void __launch_bounds__(max_threads(CPT)) row_quant_kernel(const RowQuantParams p) {
+  constexpr bool NORM = MODE != kPlain, ADD = MODE == kNormAdd;
+  using Ck = Chunk<T, ALIGNED>;
+  using Raw = typename Ck::Raw;
+  constexpr int CH = Ck::CH;
+  __shared__ RowShared sh[2];
+  ptx::grid_dep_launch_dependents();
+  ptx::grid_dep_wait();
+  const int K = p.K, nt = blockDim.x, warps = nt >> 5, chunks = (K + CH - 1) / CH;
+  const unsigned rows = (unsigned)p.M, step = gridDim.x * blockDim.y;
+  const Raw* W = static_cast<const Raw*>(p.W);
+  auto x_row = [&](unsigned row) { return static_cast<const Raw*>(p.X) + (size_t)row * p.px; };
+  auto r_row = [&](unsigned row) { return static_cast<const Raw*>(p.R) + (size_t)row * p.pr; };
+  auto u_row = [&](unsigned row) { return static_cast<Raw*>(p.U) + (size_t)row * p.pu; };
+
+  // u w (or x) of a chunk in fp32, counted into the statistics when asked for
+  float sum, top;
+  auto values = [&](const Ck& c, int i, bool count, float (&f)[CH]) {
+    if constexpr (NORM) {
+      Ck w;
+      w.load_const(W, i * CH, K - i * CH);
 #pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      const int c = i * nt + (int)threadIdx.x;
-      if (c < chunks) store_codes<ALIGNED, CH>(q + c * CH, K - c * CH, keep[i], f, bad);
+      for (int j = 0; j < CH; ++j) {
+        const float u = c.at(j);
+        if (count) sum = fmaf(u, u, sum);
+        f[j] = u * w.at(j);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < CH; ++j) f[j] = c.at(j);
+    }
+    if (count) {
+#pragma unroll
+      for (int j = 0; j < CH; j += 2) top = max_abs(top, f[j], f[j + 1]);
+    }
+  };
+
+  unsigned row = blockIdx.x * blockDim.y + threadIdx.y;
+  if constexpr (CPT > 0) {
+    Ck next[CPT], next_r[ADD ? CPT : 1];
+    auto fetch = [&](unsigned at) {
+      const Raw* x = x_row(at);
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) {
+        const int c = i * nt + (int)threadIdx.x;
+        if (c < chunks) next[i].load(x, c * CH, K - c * CH);
+      }
+      if constexpr (ADD) {
+        const Raw* r = r_row(at);
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) {
+          const int c = i * nt + (int)threadIdx.x;
+          if (c < chunks) next_r[i].load(r, c * CH, K - c * CH);
+        }
+      }
+    };
+    if (row < rows) fetch(row);
+    for (int turn = 0; row < rows; row += step, turn ^= 1) {
+      Ck cur[NORM ? 1 : CPT];
+      float f[NORM ? CPT : 1][CH];
+      sum = top = 0.f;
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) {
+        const int c = i * nt + (int)threadIdx.x;
+        if (c < chunks) {
+          if constexpr (ADD) {
+            next[i].add(next_r[i]);
+            next[i].store(u_row(row), c * CH, K - c * CH);
+          }
+          if constexpr (!NORM) cur[i] = next[i];
+          values(next[i], c, true, f[NORM ? i : 0]);
+        }
+      }
+      if (row + step < rows) fetch(row + step);
+      reduce_row(sum, top, warps, sh[turn]);
+      const RowScale rs = row_scale<NORM>(sum, top, p);
+      if (threadIdx.x == 0) p.S[row] = rs.scale;
+      int8_t* q = p.Q + (size_t)row * p.pq;
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) {
+        const int c = i * nt + (int)threadIdx.x;
+        if (c < chunks) {
+          if constexpr (!NORM) values(cur[i], c, false, f[0]);
+          store_codes<NORM, ALIGNED, CH>(q + c * CH, K - c * CH, f[NORM ? i : 0], rs.f, rs.bad);
+        }
+      }
     }
   } else {
-    for (int c = threadIdx.x; c < chunks; c += nt) {
-      take(c, keep[0], false);
-      store_codes<ALIGNED, CH>(q + c * CH, K - c * CH, keep[0], f, bad);
+    for (int turn = 0; row < rows; row += step, turn ^= 1) {
+      const Raw* x = x_row(row);
+      auto take = [&](int c) {
+        Ck v;
+        v.load(x, c * CH, K - c * CH);
+        if constexpr (ADD) {
+          Ck r;
+          r.load(r_row(row), c * CH, K - c * CH);
+          v.add(r);
+        }
+        return v;
+      };
+      sum = top = 0.f;
+      float f[CH];
+      for (int c = threadIdx.x; c < chunks; c += nt) values(take(c), c, true, f);
+      reduce_row(sum, top, warps, sh[turn]);
+      const RowScale rs = row_scale<NORM>(sum, top, p);
+      if (threadIdx.x == 0) p.S[row] = rs.scale;
+      int8_t* q = p.Q + (size_t)row * p.pq;
+      for (int c = threadIdx.x; c < chunks; c += nt) {
+        const Ck v = take(c);  // (U may be X or R: every thread writes what it alone reads, after its last read)
+        if constexpr (ADD) v.store(u_row(row), c * CH, K - c * CH);
+        values(v, c, false, f);
+        store_codes<NORM, ALIGNED, CH>(q + c * CH, K - c * CH, f, rs.f, rs.bad);
+      }
     }
   }
 }
 
-template <typename T, bool NORM, bool ALIGNED>
-int launch_rows(const RowQuantParams& p, int sms, cudaStream_t st) {
-  constexpr int CH = kChunk<T, ALIGNED>;
-  const int chunks = (p.K + CH - 1) / CH;
-  int cpt, nt, rows = 1;
-  if (chunks <= 128 && p.M > 1) {  // a warp to a row, four rows to a CTA
-    cpt = chunks <= 64 ? 2 : 4;
-    nt = 32;
-    rows = 4;
-  } else {
-    // few rows want many threads (latency), many rows want many chunks in flight per thread
-    const int most = p.M <= sms ? 1024 : 256;
-    cpt = 2;
-    while (cpt < 8 && (chunks + cpt - 1) / cpt > most) cpt *= 2;
-    nt = ((chunks + cpt - 1) / cpt + 31) / 32 * 32;
-    if (nt > max_threads(cpt * CH)) {
-      nt = 1024;
-      cpt = 0;
+// CTAs of `nt` threads of this kernel that an SM holds (asked once per device and size).
+template <typename T, int MODE, bool ALIGNED, int CPT>
+int resident(int nt, int device) {
+  static std::atomic<int> known[64][33];
+  std::atomic<int>& slot = known[device][nt / 32];
+  int k = slot.load(std::memory_order_relaxed);
+  if (k == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&k, row_quant_kernel<T, MODE, ALIGNED, CPT>, nt, 0) != cudaSuccess || k < 1) {
+      (void)cudaGetLastError();
+      k = 1;
     }
+    slot.store(k, std::memory_order_relaxed);
   }
-  auto kern = cpt == 0   ? row_quant_kernel<T, NORM, ALIGNED, 0>
-              : cpt == 2 ? row_quant_kernel<T, NORM, ALIGNED, 2>
-              : cpt == 4 ? row_quant_kernel<T, NORM, ALIGNED, 4>
-                         : row_quant_kernel<T, NORM, ALIGNED, 8>;
-  MG_CUDA_TRY(mg::launch_kernel(kern, dim3((p.M + rows - 1) / rows), dim3(nt, rows), 0, st, p));
+  return k;
+}
+
+template <typename T, int MODE, bool ALIGNED, int CPT>
+int launch_form(const RowQuantParams& p, int nt, int side, const mg::DeviceInfo& di, cudaStream_t st) {
+  const unsigned ctas = ((unsigned)p.M + side - 1) / side;
+  const unsigned most = (unsigned)di.sm_count * resident<T, MODE, ALIGNED, CPT>(nt * side, di.device);
+  MG_CUDA_TRY(mg::launch_kernel(row_quant_kernel<T, MODE, ALIGNED, CPT>, dim3(ctas < most ? ctas : most), dim3(nt, side), 0, st, p));
   return MG_OK;
+}
+
+template <typename T, int MODE, bool ALIGNED>
+int launch_rows(const RowQuantParams& p, const mg::DeviceInfo& di, cudaStream_t st) {
+  const int chunks = (p.K + kChunk<T, ALIGNED> - 1) / kChunk<T, ALIGNED>;
+  auto threads = [&](int cpt) { return ((chunks + cpt - 1) / cpt + 31) / 32 * 32; };
+  // a warp to a row, four rows to a CTA, when a warp can hold one; few rows want many threads (latency),
+  // many rows many bytes in flight per thread
+  if (chunks <= 64 && p.M > di.sm_count) return launch_form<T, MODE, ALIGNED, 2>(p, 32, 4, di, st);
+  if (p.M <= 2 * di.sm_count && threads(1) <= 1024) return launch_form<T, MODE, ALIGNED, 1>(p, threads(1), 1, di, st);
+  if (MODE != kNormAdd && threads(4) <= 512) return launch_form<T, MODE, ALIGNED, 4>(p, threads(4), 1, di, st);
+  if (threads(2) <= 1024) return launch_form<T, MODE, ALIGNED, 2>(p, threads(2), 1, di, st);
+  return launch_form<T, MODE, ALIGNED, 0>(p, 1024, 1, di, st);
+}
+
+template <typename T, bool NORM>
+int launch_type(const RowQuantParams& p, bool vec, const mg::DeviceInfo& di, cudaStream_t st) {
+  if constexpr (NORM) {
+    if (p.R) return vec ? launch_rows<T, kNormAdd, true>(p, di, st) : launch_rows<T, kNormAdd, false>(p, di, st);
+    return vec ? launch_rows<T, kNorm, true>(p, di, st) : launch_rows<T, kNorm, false>(p, di, st);
+  } else {
+    return vec ? launch_rows<T, kPlain, true>(p, di, st) : launch_rows<T, kPlain, false>(p, di, st);
+  }
 }
 
 // dtype: 0 bf16, 1 fp16, 2 fp32 (MG_BF16, MG_FP16, MG_FP32)
@@ -296,12 +404,9 @@ int row_quant(const RowQuantParams& p, int dtype, void* stream) {
     if (p.R) vec = vec && mg::aligned(p.R, 16) && mg::aligned(p.U, 16) && (one || (p.pr % ch == 0 && p.pu % ch == 0));
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == MG_BF16)
-    return vec ? launch_rows<__nv_bfloat16, NORM, true>(p, di.sm_count, st)
-               : launch_rows<__nv_bfloat16, NORM, false>(p, di.sm_count, st);
-  if (dtype == MG_FP16)
-    return vec ? launch_rows<__half, NORM, true>(p, di.sm_count, st) : launch_rows<__half, NORM, false>(p, di.sm_count, st);
-  return vec ? launch_rows<float, NORM, true>(p, di.sm_count, st) : launch_rows<float, NORM, false>(p, di.sm_count, st);
+  if (dtype == MG_BF16) return launch_type<__nv_bfloat16, NORM>(p, vec, di, st);
+  if (dtype == MG_FP16) return launch_type<__half, NORM>(p, vec, di, st);
+  return launch_type<float, NORM>(p, vec, di, st);
 }
 
 }  // namespace
