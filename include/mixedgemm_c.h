@@ -430,10 +430,10 @@ int mg_rms_norm_int8(const void* X, const void* R, const void* W, float eps, int
 /*
  * The same norm in front of the MX split: u = bf16(X + R) as above, h = bf16(u * W / sqrt(mean_k u^2 + eps)),
  * then what mg_reorder_quantize_pitched writes for h, byte for byte.
- *   X, R, U [M,K] bf16, rows ldx / ldr / ldu elements apart (multiples of 8), W [K] bf16, all 16-byte aligned;
+ *   X, R, U [M,K] bf16, 16-byte aligned, rows ldx / ldr / ldu elements apart (multiples of 8); W [K] bf16;
  *   R and U both NULL without a residual, U may be R or X itself; idx ... SF8 as in mg_reorder_quantize_pitched.
- * A row whose sum of squares is not a finite fp32 number, or that holds an h that is not finite, gets
- * scale bytes 255 (NaN), so that its row of a product is NaN.
+ * Scale bytes are 255 (NaN) throughout a row whose sum of squares is not a finite fp32 number and in a
+ * group that holds an h that is not finite: either way the row of a product is NaN, and no other.
  */
 int mg_rms_norm_reorder_quantize(const void* X, size_t ldx, const void* R, size_t ldr, const void* W, float eps,
                                  void* U, size_t ldu, int M, int K, const int16_t* idx, int KN, int KS, int KO,

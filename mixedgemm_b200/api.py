@@ -505,7 +505,8 @@ def rms_norm_reorder_quantize_x(X, weight, reorder_index, KN, KS, KO, eps=1e-6, 
     u = bf16(X + residual), h = bf16(u * weight / sqrt(mean(u^2) + eps)).  Returns the six tensors that
     reorder_quantize_x(h, ...) returns, byte for byte, and with a residual u as a seventh.  residual_out
     may be `residual` (or X) itself; `out` the six buffers of alloc_quantized_x().  Rows start on
-    16-byte boundaries.  A row with a sum of squares or an h that is not finite gets NaN scales."""
+    16-byte boundaries.  A row with a sum of squares that is not finite gets NaN scales, and so does a
+    group with such an h: that row of a product is NaN, and no other."""
     what = "rms_norm_reorder_quantize_x"
     dev, ldx, ldr, u, ldu = _norm_inputs(X, weight, residual, residual_out, what)
     M, K = X.shape

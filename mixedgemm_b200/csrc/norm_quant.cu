@@ -40,7 +40,7 @@ struct RowQuantParams {
   int M, K;
   size_t px, pr, pu;  // row pitches in elements of T
   size_t pq;          // row pitch of the codes in bytes
-  float eps;
+  float eps, inv_k;
 };
 
 template <typename T>
@@ -68,7 +68,8 @@ template <typename T, bool ALIGNED>
 constexpr int kChunk = ALIGNED ? 16 / (int)sizeof(typename Elem<T>::Raw) : 4;
 
 // A chunk of a row as it lies in memory: a whole 16-byte vector, or four elements that are moved one by
-// one (those beyond the row's end read as zero).
+// one.  `n` elements are left in the row: what lies beyond reads as zero and is not written, so that the
+// arithmetic in between needs no branches.
 template <typename T, bool ALIGNED>
 struct Chunk {
   using Raw = typename Elem<T>::Raw;
@@ -80,7 +81,8 @@ struct Chunk {
 
   __device__ __forceinline__ void load(const Raw* row, int e0, int n) {
     if constexpr (ALIGNED) {
-      v = *reinterpret_cast<const uint4*>(row + e0);
+      v = make_uint4(0, 0, 0, 0);
+      if (n > 0) v = *reinterpret_cast<const uint4*>(row + e0);
     } else {
 #pragma unroll
       for (int j = 0; j < CH; ++j) e[j] = j < n ? row[e0 + j] : (Raw)0;
@@ -88,7 +90,8 @@ struct Chunk {
   }
   __device__ __forceinline__ void load_const(const Raw* row, int e0, int n) {  // never written while the kernel runs
     if constexpr (ALIGNED) {
-      v = __ldg(reinterpret_cast<const uint4*>(row + e0));
+      v = make_uint4(0, 0, 0, 0);
+      if (n > 0) v = __ldg(reinterpret_cast<const uint4*>(row + e0));
     } else {
 #pragma unroll
       for (int j = 0; j < CH; ++j) e[j] = j < n ? __ldg(row + e0 + j) : (Raw)0;
@@ -96,7 +99,7 @@ struct Chunk {
   }
   __device__ __forceinline__ void store(Raw* row, int e0, int n) const {
     if constexpr (ALIGNED) {
-      *reinterpret_cast<uint4*>(row + e0) = v;
+      if (n > 0) *reinterpret_cast<uint4*>(row + e0) = v;
     } else {
 #pragma unroll
       for (int j = 0; j < CH; ++j)
@@ -143,9 +146,11 @@ __device__ __forceinline__ void store_codes(int8_t* q, int n, const float (&p)[C
   for (int j = 0; j < CH / 4; ++j)
     w[j] = bad ? 0u : codes4<NORM>(p[j * 4], p[j * 4 + 1], p[j * 4 + 2], p[j * 4 + 3], f);
   if constexpr (CH == 8) {
-    *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+    if (n > 0) *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+  } else if constexpr (ALIGNED) {
+    if (n > 0) *reinterpret_cast<uint32_t*>(q) = w[0];
   } else {
-    if (ALIGNED || (n >= 4 && (reinterpret_cast<uintptr_t>(q) & 3) == 0)) {
+    if (n >= 4 && (reinterpret_cast<uintptr_t>(q) & 3) == 0) {
       *reinterpret_cast<uint32_t*>(q) = w[0];
     } else {
 #pragma unroll
@@ -158,8 +163,7 @@ __device__ __forceinline__ void store_codes(int8_t* q, int n, const float (&p)[C
 // Sum and maximum over the threads of a row: blockDim.x lanes, one or more whole warps.  The
 // caller alternates between two sets of shared words, so that one barrier per row is enough.
 struct RowShared {
-  float sum[32];
-  float top[32];
+  float2 part[32];
 };
 
 __device__ __forceinline__ void reduce_row(float& sum, float& top, int warps, RowShared& sh) {
@@ -170,23 +174,25 @@ __device__ __forceinline__ void reduce_row(float& sum, float& top, int warps, Ro
   }
   if (warps == 1) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) {
-    sh.sum[warp] = sum;
-    sh.top[warp] = top;
-  }
+  if (lane == 0) sh.part[warp] = make_float2(sum, top);
   __syncthreads();
-  sum = lane < warps ? sh.sum[lane] : 0.f;
-  top = lane < warps ? sh.top[lane] : 0.f;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  const float2 part = lane < warps ? sh.part[lane] : make_float2(0.f, 0.f);
+  sum = part.x;
+  top = part.y;
+  int o = 1;
+  for (; o < warps; o *= 2) {
     sum += __shfl_xor_sync(0xffffffffu, sum, o);
     top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   }
+  if (o < 32) {  // the other lanes hold the sums of nothing
+    sum = __shfl_sync(0xffffffffu, sum, 0);
+    top = __shfl_sync(0xffffffffu, top, 0);
+  }
 }
 
-// What a row's statistics make of it: codes = rint(u w f), scale.
+// What a row's statistics make of it: codes = rint(u w f), scale = a / 127.
 struct RowScale {
-  float f, scale;
+  float f, a;
   bool bad;
 };
 
@@ -196,12 +202,12 @@ __device__ __forceinline__ RowScale row_scale(float sum, float top, const RowQua
   bool bad = !(top <= 3.4028235e38f);
   if constexpr (NORM) {
     bad = bad || !(sum <= 3.4028235e38f);
-    v = rsqrtf(sum / (float)p.K + p.eps);
+    v = rsqrtf(fmaf(sum, p.inv_k, p.eps));
     a *= v;
     bad = bad || !(a <= 3.4028235e38f);
   }
   a = fmaxf(a, kTiny);
-  return {v * (127.0f / a), bad ? __uint_as_float(0x7fc00000u) : a / 127.0f, bad};
+  return {v * (127.0f / a), a, bad};
 }
 
 // Persistent: blockDim.x threads take a row at a time (blockDim.y rows side by side in a CTA when a row is
@@ -214,7 +220,7 @@ constexpr int max_threads(int cpt) { return cpt >= 4 ? 512 : 1024; }  // (regist
 enum { kPlain = 0, kNorm = 1, kNormAdd = 2 };
 
 template <typename T, int MODE, bool ALIGNED, int CPT>
-__global__ void __launch_bounds__(max_threads(CPT)) row_quant_kernel(const RowQuantParams p) {
+__global__ void __launch_bounds__(max_threads(CPT), MODE == kPlain && CPT == 4 ? 2 : 1) row_quant_kernel(const RowQuantParams p) {
   constexpr bool NORM = MODE != kPlain, ADD = MODE == kNormAdd;
   using Ck = Chunk<T, ALIGNED>;
   using Raw = typename Ck::Raw;
@@ -258,15 +264,15 @@ __global__ void __launch_bounds__(max_threads(CPT)) row_quant_kernel(const RowQu
       const Raw* x = x_row(at);
 #pragma unroll
       for (int i = 0; i < CPT; ++i) {
-        const int c = i * nt + (int)threadIdx.x;
-        if (c < chunks) next[i].load(x, c * CH, K - c * CH);
+        const int e0 = (i * nt + (int)threadIdx.x) * CH;
+        next[i].load(x, e0, K - e0);
       }
       if constexpr (ADD) {
         const Raw* r = r_row(at);
 #pragma unroll
         for (int i = 0; i < CPT; ++i) {
-          const int c = i * nt + (int)threadIdx.x;
-          if (c < chunks) next_r[i].load(r, c * CH, K - c * CH);
+          const int e0 = (i * nt + (int)threadIdx.x) * CH;
+          next_r[i].load(r, e0, K - e0);
         }
       }
     };
@@ -278,27 +284,23 @@ __global__ void __launch_bounds__(max_threads(CPT)) row_quant_kernel(const RowQu
 #pragma unroll
       for (int i = 0; i < CPT; ++i) {
         const int c = i * nt + (int)threadIdx.x;
-        if (c < chunks) {
-          if constexpr (ADD) {
-            next[i].add(next_r[i]);
-            next[i].store(u_row(row), c * CH, K - c * CH);
-          }
-          if constexpr (!NORM) cur[i] = next[i];
-          values(next[i], c, true, f[NORM ? i : 0]);
+        if constexpr (ADD) {
+          next[i].add(next_r[i]);
+          next[i].store(u_row(row), c * CH, K - c * CH);
         }
+        if constexpr (!NORM) cur[i] = next[i];
+        values(next[i], c, true, f[NORM ? i : 0]);
       }
       if (row + step < rows) fetch(row + step);
       reduce_row(sum, top, warps, sh[turn]);
       const RowScale rs = row_scale<NORM>(sum, top, p);
-      if (threadIdx.x == 0) p.S[row] = rs.scale;
+      if (threadIdx.x == 0) p.S[row] = rs.bad ? __uint_as_float(0x7fc00000u) : rs.a / 127.0f;
       int8_t* q = p.Q + (size_t)row * p.pq;
 #pragma unroll
       for (int i = 0; i < CPT; ++i) {
         const int c = i * nt + (int)threadIdx.x;
-        if (c < chunks) {
-          if constexpr (!NORM) values(cur[i], c, false, f[0]);
-          store_codes<NORM, ALIGNED, CH>(q + c * CH, K - c * CH, f[NORM ? i : 0], rs.f, rs.bad);
-        }
+        if constexpr (!NORM) values(cur[i], c, false, f[0]);
+        store_codes<NORM, ALIGNED, CH>(q + c * CH, K - c * CH, f[NORM ? i : 0], rs.f, rs.bad);
       }
     }
   } else {
@@ -319,7 +321,7 @@ __global__ void __launch_bounds__(max_threads(CPT)) row_quant_kernel(const RowQu
       for (int c = threadIdx.x; c < chunks; c += nt) values(take(c), c, true, f);
       reduce_row(sum, top, warps, sh[turn]);
       const RowScale rs = row_scale<NORM>(sum, top, p);
-      if (threadIdx.x == 0) p.S[row] = rs.scale;
+      if (threadIdx.x == 0) p.S[row] = rs.bad ? __uint_as_float(0x7fc00000u) : rs.a / 127.0f;
       int8_t* q = p.Q + (size_t)row * p.pq;
       for (int c = threadIdx.x; c < chunks; c += nt) {
         const Ck v = take(c);  // (U may be X or R: every thread writes what it alone reads, after its last read)
@@ -359,12 +361,12 @@ template <typename T, int MODE, bool ALIGNED>
 int launch_rows(const RowQuantParams& p, const mg::DeviceInfo& di, cudaStream_t st) {
   const int chunks = (p.K + kChunk<T, ALIGNED> - 1) / kChunk<T, ALIGNED>;
   auto threads = [&](int cpt) { return ((chunks + cpt - 1) / cpt + 31) / 32 * 32; };
-  // a warp to a row, four rows to a CTA, when a warp can hold one; few rows want many threads (latency),
-  // many rows many bytes in flight per thread
+  // A warp to a row, four rows to a CTA, when two chunks per thread hold one; few rows want many threads
+  // (latency: 64 x 4096 1.7 us with one chunk per thread, 1.8 with two), many rows many bytes in flight per
+  // thread (14336 x 4096: 28.4 us with four, 36.5 with two, 44 with one, 61 read twice).
   if (chunks <= 64 && p.M > di.sm_count) return launch_form<T, MODE, ALIGNED, 2>(p, 32, 4, di, st);
   if (p.M <= 2 * di.sm_count && threads(1) <= 1024) return launch_form<T, MODE, ALIGNED, 1>(p, threads(1), 1, di, st);
-  if (MODE != kNormAdd && threads(4) <= 512) return launch_form<T, MODE, ALIGNED, 4>(p, threads(4), 1, di, st);
-  if (threads(2) <= 1024) return launch_form<T, MODE, ALIGNED, 2>(p, threads(2), 1, di, st);
+  if (threads(4) <= 512) return launch_form<T, MODE, ALIGNED, 4>(p, threads(4), 1, di, st);
   return launch_form<T, MODE, ALIGNED, 0>(p, 1024, 1, di, st);
 }
 
@@ -441,5 +443,6 @@ extern "C" int mg_rms_norm_int8(const void* X, const void* R, const void* W, flo
   p.pu = ldu;
   p.pq = ldq;
   p.eps = eps;
+  p.inv_k = 1.0f / (float)K;
   return row_quant<true>(p, dtype, stream);
 }

@@ -23,6 +23,8 @@
 #include <cuda_fp6.h>
 #include <cuda_fp8.h>
 
+#include <atomic>
+
 #include "mg_common.h"
 #include "ptx_sm100.cuh"
 
@@ -31,6 +33,7 @@ namespace {
 constexpr int kConsumerWarps = 16;
 constexpr int kConsumers = kConsumerWarps * 32;
 constexpr int kThreads = kConsumers + 32;  // + one producer warp
+constexpr size_t kStaticSmem = 256;        // of the kernel with a norm: the rows' partial sums
 constexpr int kRowSkew = 16;               // bytes added to the shared-memory row pitch
 
 struct SegOut {
@@ -117,33 +120,18 @@ __device__ __forceinline__ float scale_round(float x, float rs) {
   return __uint_as_float(__float_as_uint(r) | (__float_as_uint(x) & 0x80000000u));
 }
 
-// One (row, group): gather, scale, quantise, pack, store.  nan_row: the scale is NaN, whatever the values.
+// The 32 values of group g (already gathered) and their largest magnitude: scale, quantise, pack, store.
+// nan: the scale is NaN, whatever the values.
 template <bool WEIGHTS>
-__device__ __forceinline__ void quantise_group(const ReorderParams& p, const RowCtx& rc, uint32_t idx2_addr, int g,
-                                               bool nan_row = false) {
-  float x[32];
-  float maxv = 0.f;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const uint4 iv = lds_v4(idx2_addr + g * 64 + q * 16);
-    const unsigned o[4] = {iv.x, iv.y, iv.z, iv.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const unsigned lo = lds_u16(rc.smem_row + (o[j] & 0xFFFFu));
-      const unsigned hi = lds_u16(rc.smem_row + (o[j] >> 16));
-      x[q * 8 + j * 2] = __uint_as_float(lo << 16);
-      x[q * 8 + j * 2 + 1] = __uint_as_float(hi << 16);
-      maxv = fmaxf(maxv, fmaxf(fabsf(x[q * 8 + j * 2]), fabsf(x[q * 8 + j * 2 + 1])));
-    }
-  }
-
+__device__ __forceinline__ void emit_group(const ReorderParams& p, const RowCtx& rc, int g, float (&x)[32], float maxv,
+                                           bool nan) {
   const int seg = g < p.g4 ? 0 : (g < p.g46 ? 1 : 2);
   const int gs = g - (seg == 0 ? 0 : (seg == 1 ? p.g4 : p.g46));
   const int fmt = WEIGHTS ? 0 : seg;
   const SegOut so = seg == 0 ? p.seg[0] : (seg == 1 ? p.seg[1] : p.seg[2]);
 
   const int sf = scale_byte(maxv, fmt);
-  so.sf[rc.sf_row + (gs & 3) + (size_t)(gs >> 2) * 512 + (size_t)rc.row_blk * 512 * so.katoms] = (uint8_t)(nan_row ? 255 : sf);
+  so.sf[rc.sf_row + (gs & 3) + (size_t)(gs >> 2) * 512 + (size_t)rc.row_blk * 512 * so.katoms] = (uint8_t)(nan ? 255 : sf);
   const float rs = __uint_as_float(((unsigned)(254 - sf) << 23) | 0x800u);  // 2^(127-sf) * (1 + 2^-12)
 
 #pragma unroll
@@ -207,9 +195,106 @@ __device__ __forceinline__ void quantise_group(const ReorderParams& p, const Row
   }
 }
 
+// One (row, group): gather, scale, quantise, pack, store.
+template <bool WEIGHTS>
+__device__ __forceinline__ void quantise_group(const ReorderParams& p, const RowCtx& rc, uint32_t idx2_addr, int g) {
+  float x[32];
+  float maxv = 0.f;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint4 iv = lds_v4(idx2_addr + g * 64 + q * 16);
+    const unsigned o[4] = {iv.x, iv.y, iv.z, iv.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const unsigned lo = lds_u16(rc.smem_row + (o[j] & 0xFFFFu));
+      const unsigned hi = lds_u16(rc.smem_row + (o[j] >> 16));
+      x[q * 8 + j * 2] = __uint_as_float(lo << 16);
+      x[q * 8 + j * 2 + 1] = __uint_as_float(hi << 16);
+      maxv = fmaxf(maxv, fmaxf(fabsf(x[q * 8 + j * 2]), fabsf(x[q * 8 + j * 2 + 1])));
+    }
+  }
+  emit_group<WEIGHTS>(p, rc, g, x, maxv, false);
+}
+
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The same behind a root-mean-square norm: the staged row holds u, and h = bf16((u w) v) is formed on the
+// way from shared memory to the codes.  wp_addr: the norm's weight in reordered order, so that a group's
+// 32 weights are one run of 64 bytes, the same for all rows that the lanes of a warp walk.
+__device__ __forceinline__ void quantise_norm_group(const ReorderParams& p, const RowCtx& rc, uint32_t idx2_addr,
+                                                    uint32_t wp_addr, int g, float v, bool nan_row) {
+  float x[32];
+  float maxv = 0.f;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint4 iv = lds_v4(idx2_addr + g * 64 + q * 16), wv = lds_v4(wp_addr + g * 64 + q * 16);
+    const unsigned o[4] = {iv.x, iv.y, iv.z, iv.w}, w[4] = {wv.x, wv.y, wv.z, wv.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const unsigned lo = lds_u16(rc.smem_row + (o[j] & 0xFFFFu));
+      const unsigned hi = lds_u16(rc.smem_row + (o[j] >> 16));
+      const uint32_t h = bf16_pair(__uint_as_float(lo << 16) * bf16_lo(w[j]) * v, __uint_as_float(hi << 16) * bf16_hi(w[j]) * v);
+      x[q * 8 + j * 2] = bf16_lo(h);
+      x[q * 8 + j * 2 + 1] = bf16_hi(h);
+      asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(maxv) : "f"(maxv), "f"(x[q * 8 + j * 2]), "f"(x[q * 8 + j * 2 + 1]));
+    }
+  }
+  emit_group<false>(p, rc, g, x, maxv, nan_row || !(maxv <= 3.4028235e38f));
+}
+
+// What a norm in front of the quantiser adds to a problem.
+struct NormPart {
+  const uint16_t* R;  // residual, or null
+  uint16_t* U;        // the stream after the addition (with R only)
+  const uint16_t* W;
+  size_t px, pr, pu;  // row pitches in elements
+  float eps, inv_k;
+  int staged;         // the residual's rows are staged beside x (otherwise the consumers read them from memory)
+};
+
+// The norm's weight into shared memory, in reordered order: read in order (2-byte loads from all over it
+// cost 10 us at K = 14336), then permuted in place through registers.
+__device__ __forceinline__ void load_reordered_weight(const uint16_t* W, int K, const uint16_t* idx2, uint16_t* wp, int tid) {
+  constexpr int kMost = (32736 / 8 + kConsumers - 1) / kConsumers;  // 16-byte vectors of the longest row, per thread
+  const int nv = K >> 3;
+  if ((reinterpret_cast<uintptr_t>(W) & 15) == 0) {
+    for (int j = tid; j < nv; j += kConsumers) reinterpret_cast<uint4*>(wp)[j] = __ldg(reinterpret_cast<const uint4*>(W) + j);
+  } else {
+    for (int j = tid; j < K; j += kConsumers) wp[j] = __ldg(W + j);
+  }
+  ptx::named_barrier_sync(1, kConsumers);  // (the index is there as well)
+  const uint32_t base = ptx::smem_u32(wp);
+  uint32_t t[kMost][4];
+#pragma unroll
+  for (int u = 0; u < kMost; ++u) {
+    const int j = u * kConsumers + tid;
+    if (j < nv) {
+      const uint4 o = lds_v4(ptx::smem_u32(idx2) + j * 16);
+      t[u][0] = lds_u16(base + (o.x & 0xFFFFu)) | (lds_u16(base + (o.x >> 16)) << 16);
+      t[u][1] = lds_u16(base + (o.y & 0xFFFFu)) | (lds_u16(base + (o.y >> 16)) << 16);
+      t[u][2] = lds_u16(base + (o.z & 0xFFFFu)) | (lds_u16(base + (o.z >> 16)) << 16);
+      t[u][3] = lds_u16(base + (o.w & 0xFFFFu)) | (lds_u16(base + (o.w >> 16)) << 16);
+    }
+  }
+  ptx::named_barrier_sync(1, kConsumers);
+#pragma unroll
+  for (int u = 0; u < kMost; ++u) {
+    const int j = u * kConsumers + tid;
+    if (j < nv) ptx::sts_v4(base + j * 16, t[u][0], t[u][1], t[u][2], t[u][3]);
+  }
+}
+
 // One CTA's work: block `blk` of the `nblk` blocks that share the rows of problem p.
-template <int R, bool WEIGHTS>
-__device__ __forceinline__ void reorder_quantize_cta(const ReorderParams& p, int blk, int nblk) {
+// With NORM every stage is first normalised: kConsumerWarps / R warps share a row, read it once in 16-byte
+// vectors, add the residual (u goes to the stream and back to the staged row) and add up u^2; after one
+// barrier of the consumers the groups are quantised as always, from h = bf16((u w) v).
+template <int R, bool WEIGHTS, bool NORM = false>
+__device__ __forceinline__ void reorder_quantize_cta(const ReorderParams& p, int blk, int nblk, const NormPart* np = nullptr) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int K = p.K;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -217,8 +302,9 @@ __device__ __forceinline__ void reorder_quantize_cta(const ReorderParams& p, int
   const int pitch = 2 * K + kRowSkew;
   const int idx_bytes = (2 * K + 15) & ~15;
   uint16_t* idx2 = reinterpret_cast<uint16_t*>(smem);
-  uint8_t* tiles = smem + idx_bytes;
-  const int stage_bytes = R * pitch;
+  uint16_t* wp = reinterpret_cast<uint16_t*>(smem + idx_bytes);  // (with NORM)
+  uint8_t* tiles = smem + (NORM ? 2 : 1) * idx_bytes;
+  const int stage_bytes = (NORM && np->staged ? 2 : 1) * R * pitch;  // rows of x, then of the residual
   uint8_t* tail = tiles + (size_t)S * stage_bytes;  // barriers: full[8], empty[8], then the stop flag
   const uint32_t bar0 = ptx::smem_u32(tail);
   volatile int* stop = reinterpret_cast<volatile int*>(tail + 16 * 8);
@@ -251,10 +337,18 @@ __device__ __forceinline__ void reorder_quantize_cta(const ReorderParams& p, int
         const int row0 = row_begin + it * R;
         const int nrows = min(R, row_end - row0);
         const uint32_t fb = bar0 + 8 * s;
-        ptx::mbar_expect_tx(fb, (uint32_t)nrows * 2u * K);
         const uint32_t dst = ptx::smem_u32(tiles + (size_t)s * stage_bytes);
-        for (int r = 0; r < nrows; ++r)
-          ptx::bulk_load_1d(dst + r * pitch, p.X + (size_t)(row0 + r) * K, 2u * K, fb);
+        if constexpr (NORM) {
+          ptx::mbar_expect_tx(fb, (uint32_t)nrows * (np->staged ? 4u : 2u) * K);
+          for (int r = 0; r < nrows; ++r) {
+            ptx::bulk_load_1d(dst + r * pitch, p.X + (size_t)(row0 + r) * np->px, 2u * K, fb);
+            if (np->staged) ptx::bulk_load_1d(dst + (R + r) * pitch, np->R + (size_t)(row0 + r) * np->pr, 2u * K, fb);
+          }
+        } else {
+          ptx::mbar_expect_tx(fb, (uint32_t)nrows * 2u * K);
+          for (int r = 0; r < nrows; ++r)
+            ptx::bulk_load_1d(dst + r * pitch, p.X + (size_t)(row0 + r) * K, 2u * K, fb);
+        }
       }
     }
   } else {
@@ -294,6 +388,7 @@ __device__ __forceinline__ void reorder_quantize_cta(const ReorderParams& p, int
         idx2[i] = (uint16_t)(v * 2);
       }
     }
+    if constexpr (NORM) load_reordered_weight(np->W, K, idx2, wp, tid);
     ptx::named_barrier_sync(1, kConsumers);
     // a thread keeps its row
     constexpr int kGStep = kConsumers / R;
@@ -306,14 +401,66 @@ __device__ __forceinline__ void reorder_quantize_cta(const ReorderParams& p, int
     for (int it = 0; it < nstage; ++it, s = s + 1 == S ? 0 : s + 1, ph ^= (s == 0)) {
       wait_parity(bar0 + 8 * s, ph, stop, p.status, p.wait_cycles, 32);
       const int row = row_begin + it * R + r;
+      float v = 0.f;         // 1 / root-mean-square of this thread's row
+      bool nan_row = false;
+      if constexpr (NORM) {
+        // every barrier below is reached by all consumers, also after a wait that gave up
+        __shared__ float s_sum[2][kConsumerWarps];
+        constexpr int kWarpsPerRow = kConsumerWarps / R;
+        const int nr = warp / kWarpsPerRow, nlane = (warp % kWarpsPerRow) * 32 + lane;
+        const int nrow = row_begin + it * R + nr;
+        float sum = 0.f;
+        if (nrow < row_end && !*stop) {
+          const uint32_t xs = ptx::smem_u32(tiles + (size_t)s * stage_bytes) + nr * pitch, rs = xs + R * pitch;
+          const bool add = np->R != nullptr;
+          const uint4* rg = reinterpret_cast<const uint4*>(np->R + (size_t)nrow * np->pr);
+          uint4* ug = reinterpret_cast<uint4*>(np->U + (size_t)nrow * np->pu);
+#pragma unroll 4
+          for (int i = nlane; i < (K >> 3); i += kWarpsPerRow * 32) {
+            uint4 a = lds_v4(xs + i * 16);
+            if (add) {
+              const uint4 b = np->staged ? lds_v4(rs + i * 16) : rg[i];
+              a.x = bf16_pair(bf16_lo(a.x) + bf16_lo(b.x), bf16_hi(a.x) + bf16_hi(b.x));
+              a.y = bf16_pair(bf16_lo(a.y) + bf16_lo(b.y), bf16_hi(a.y) + bf16_hi(b.y));
+              a.z = bf16_pair(bf16_lo(a.z) + bf16_lo(b.z), bf16_hi(a.z) + bf16_hi(b.z));
+              a.w = bf16_pair(bf16_lo(a.w) + bf16_lo(b.w), bf16_hi(a.w) + bf16_hi(b.w));
+              ug[i] = a;
+              ptx::sts_v4(xs + i * 16, a.x, a.y, a.z, a.w);
+            }
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              sum = fmaf(bf16_lo(w[k]), bf16_lo(w[k]), sum);
+              sum = fmaf(bf16_hi(w[k]), bf16_hi(w[k]), sum);
+            }
+          }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) s_sum[it & 1][warp] = sum;  // (the other half may still be read)
+        __syncwarp();
+        ptx::named_barrier_sync(1, kConsumers);
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kWarpsPerRow; ++i) sum += s_sum[it & 1][r * kWarpsPerRow + i];
+        nan_row = !(sum <= 3.4028235e38f);
+        v = rsqrtf(fmaf(sum, np->inv_k, np->eps));
+      }
       if (worker && row < row_end && !*stop) {
         RowCtx rc;
         rc.smem_row = ptx::smem_u32(tiles + (size_t)s * stage_bytes) + r * pitch;
         rc.sf_row = (uint32_t)(row & 31) * 16 + (uint32_t)((row >> 5) & 3) * 4;
         rc.row_blk = (uint32_t)row >> 7;
         rc.row = (uint32_t)row;
-        for (int g = g0; g < G; g += kGStep) quantise_group<WEIGHTS>(p, rc, idx2_addr, g);
+        if constexpr (NORM) {
+          const uint32_t wp_addr = ptx::smem_u32(wp);
+          for (int g = g0; g < G; g += kGStep) quantise_norm_group(p, rc, idx2_addr, wp_addr, g, v, nan_row);
+        } else {
+          for (int g = g0; g < G; g += kGStep) quantise_group<WEIGHTS>(p, rc, idx2_addr, g);
+        }
       }
+      // (the consumers wrote into the stage that the next copy overwrites)
+      if constexpr (NORM) ptx::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar0 + 8 * (8 + s));
     }
@@ -354,145 +501,15 @@ __global__ void __launch_bounds__(kThreads, 1) reorder_quantize_multi_kernel(con
   }
 }
 
-// ---------------------------------------------------------------- behind a root-mean-square norm
-// u = bf16(x + r), h = bf16((u w) rsqrt(mean u^2 + eps)), then the codes and scales of h as above.
-//
-// A CTA takes R rows at a time.  kNormWarps / R warps share a row: they read it (and the residual)
-// once in 16-byte vectors, write u to the stream and to shared memory, add up u^2, and turn u into h
-// in place; then all threads quantise the R rows of the tile with the lanes of a warp walking the
-// rows of a group, as in the kernel above.  A row with a sum or a value that is not finite gets NaN
-// scales.  The phases of one CTA alternate; what overlaps loads with
-// arithmetic is that several CTAs share an SM.  The index stays in shared memory for the life of the CTA.
-// Bound: bytes (2 read + 0.63 written per element, 6 + 0.63 with a residual).
-constexpr int kNormWarps = 8;
-constexpr int kNormThreads = kNormWarps * 32;
-
-struct NormParams {
-  ReorderParams q;
-  const uint16_t* R;  // residual, or null
-  uint16_t* U;        // the stream after the addition (with R only)
-  const uint16_t* W;
-  size_t px, pr, pu;  // row pitches in elements
-  float eps;
-};
-
-__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
-__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 template <int R>
-__global__ void __launch_bounds__(kNormThreads) norm_reorder_kernel(const __grid_constant__ NormParams np) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float s_sum[kNormWarps];
-  __shared__ int s_bad[R];
-  constexpr int kWarpsPerRow = kNormWarps / R;
-  const ReorderParams& p = np.q;
-  const int K = p.K, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int pitch = 2 * K + kRowSkew;
-  uint16_t* idx2 = reinterpret_cast<uint16_t*>(smem);
-  uint8_t* tile = smem + 2 * K;  // K is a multiple of 32
-  ptx::grid_dep_launch_dependents();
-  ptx::grid_dep_wait();
-  for (int i = tid; i < K; i += kNormThreads) {
-    const unsigned v = (uint16_t)p.idx[i];
-    idx2[i] = (uint16_t)(min(v, (unsigned)(K - 1)) * 2);
-  }
-  const uint32_t idx2_addr = ptx::smem_u32(idx2);
-  const int nv = K >> 3, G = K >> 5;
-  const int my_row = warp / kWarpsPerRow, my_lane = (warp % kWarpsPerRow) * 32 + lane;
-  constexpr int kLanes = kWarpsPerRow * 32;
-  const int r = tid % R, g0 = tid / R;
-
-  const unsigned rows = (unsigned)p.rows;
-  for (unsigned row0 = blockIdx.x * R; row0 < rows; row0 += gridDim.x * R) {
-    const unsigned row = row0 + my_row;
-    uint4* srow = reinterpret_cast<uint4*>(tile + (size_t)my_row * pitch);
-    float sum = 0.f;
-    if (my_lane == 0) s_bad[my_row] = 0;
-    if (row < rows) {
-      const uint4* x = reinterpret_cast<const uint4*>(p.X + (size_t)row * np.px);
-      const uint4* res = np.R ? reinterpret_cast<const uint4*>(np.R + (size_t)row * np.pr) : nullptr;
-      uint4* out = np.R ? reinterpret_cast<uint4*>(np.U + (size_t)row * np.pu) : nullptr;
-      for (int i = my_lane; i < nv; i += kLanes) {
-        uint4 a = x[i];
-        uint32_t w[4] = {a.x, a.y, a.z, a.w};
-        if (res) {
-          const uint4 b = res[i];
-          const uint32_t t[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = bf16_pair(bf16_lo(w[k]) + bf16_lo(t[k]), bf16_hi(w[k]) + bf16_hi(t[k]));
-          out[i] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          sum = fmaf(bf16_lo(w[k]), bf16_lo(w[k]), sum);
-          sum = fmaf(bf16_hi(w[k]), bf16_hi(w[k]), sum);
-        }
-        srow[i] = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if constexpr (kWarpsPerRow > 1) {
-      if (lane == 0) s_sum[warp] = sum;
-      __syncthreads();
-      sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < kWarpsPerRow; ++i) sum += s_sum[my_row * kWarpsPerRow + i];
-    }
-    __syncwarp();
-    const float v = rsqrtf(sum / (float)K + np.eps);
-    if (row < rows) {
-      bool bad = !(sum <= 3.4028235e38f);
-      const uint4* wt = reinterpret_cast<const uint4*>(np.W);
-      for (int i = my_lane; i < nv; i += kLanes) {  // the vectors this thread wrote
-        const uint4 a = srow[i], b = __ldg(wt + i);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w}, t[4] = {b.x, b.y, b.z, b.w};
-        uint32_t h[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          h[k] = bf16_pair(bf16_lo(w[k]) * bf16_lo(t[k]) * v, bf16_hi(w[k]) * bf16_hi(t[k]) * v);
-          bad = bad || (h[k] & 0x7F80u) == 0x7F80u || (h[k] & 0x7F800000u) == 0x7F800000u;
-        }
-        srow[i] = make_uint4(h[0], h[1], h[2], h[3]);
-      }
-      if (bad) s_bad[my_row] = 1;
-    }
-    __syncthreads();
-    const unsigned qrow = row0 + r;
-    if (qrow < rows) {
-      RowCtx rc;
-      rc.smem_row = ptx::smem_u32(tile) + r * pitch;
-      rc.sf_row = (qrow & 31) * 16 + ((qrow >> 5) & 3) * 4;
-      rc.row_blk = qrow >> 7;
-      rc.row = qrow;
-      const bool nan_row = s_bad[r];
-      for (int g = g0; g < G; g += kNormThreads / R) quantise_group<false>(p, rc, idx2_addr, g, nan_row);
-    }
-    __syncthreads();
-  }
+__global__ void __launch_bounds__(kThreads, 1) norm_reorder_quantize_kernel(const __grid_constant__ ReorderParams p,
+                                                                            const __grid_constant__ NormPart np) {
+  reorder_quantize_cta<R, false, true>(p, (int)blockIdx.x, (int)gridDim.x, &np);
 }
 
-size_t norm_smem_bytes(int K, int R) { return (size_t)2 * K + (size_t)R * (2 * K + kRowSkew); }
-
-template <int R>
-int launch_norm(const NormParams& np, const mg::DeviceInfo& di, cudaStream_t st) {
-  auto kern = norm_reorder_kernel<R>;
-  const size_t smem = norm_smem_bytes(np.q.K, R);
-  if (smem > 48 * 1024) MG_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  const int tiles = (np.q.rows + R - 1) / R;
-  int per_sm = (int)((size_t)di.smem_optin / (smem + 1024));
-  per_sm = per_sm < 1 ? 1 : per_sm > 4 ? 4 : per_sm;
-  const int most = di.sm_count * per_sm;
-  MG_CUDA_TRY(mg::launch_kernel(kern, dim3(tiles < most ? tiles : most), dim3(kNormThreads), smem, st, np));
-  return MG_OK;
-}
-
-size_t smem_bytes(int K, int R, int S) {
-  return (size_t)((2 * K + 15) & ~15) + (size_t)S * R * (2 * K + kRowSkew) + 16 * 8 + 16;
+// norm: 0 without, 1 with (the weight beside the index), 2 with the residual's rows staged too
+size_t smem_bytes(int K, int R, int S, int norm = 0) {
+  return (size_t)(norm ? 2 : 1) * ((2 * K + 15) & ~15) + (size_t)S * (norm == 2 ? 2 : 1) * R * (2 * K + kRowSkew) + 16 * 8 + 16;
 }
 
 template <int R, bool WEIGHTS>
@@ -542,18 +559,18 @@ int fill_params(bool weights, const void* X, int rows, int K, const int16_t* idx
 
 // Rows per stage and stage count of a problem whose rows are shared by `grid` CTAs; returns the
 // shared memory a CTA needs, or 0 when the problem does not fit.
-size_t stage_shape(ReorderParams* p, int grid, size_t smem_optin, int* rows_per_stage) {
+size_t stage_shape(ReorderParams* p, int grid, size_t smem_optin, int* rows_per_stage, int norm = 0) {
   const int K = p->K, rows = p->rows;
   const size_t budget = smem_optin - 1024;
   const int rows_per_cta = rows / grid;
   static const int kRs[] = {8, 4, 2, 1};
   int R = 1;
   for (int cand : kRs)
-    if (smem_bytes(K, cand, 2) <= budget && (2 * cand <= rows_per_cta || cand == 1)) { R = cand; break; }
+    if (smem_bytes(K, cand, 2, norm) <= budget && (2 * cand <= rows_per_cta || cand == 1)) { R = cand; break; }
   int S = 2;
-  while (S < 4 && smem_bytes(K, R, S + 1) <= budget) ++S;
-  if (smem_bytes(K, R, 2) > budget) S = 1;
-  const size_t smem = smem_bytes(K, R, S);
+  while (S < 4 && smem_bytes(K, R, S + 1, norm) <= budget) ++S;
+  if (smem_bytes(K, R, 2, norm) > budget) S = 1;
+  const size_t smem = smem_bytes(K, R, S, norm);
   if (smem > smem_optin) return 0;
   p->num_tiles = (rows + R - 1) / R;
   p->stages = S;
@@ -696,21 +713,35 @@ extern "C" size_t mg_code_pitch(int weights, int segment, int kseg) {
   return segment == 1 ? (size_t)kp / 4 * 3 : (size_t)kp;
 }
 
+namespace {
+
+template <int R>
+int launch_norm(const ReorderParams& p, const NormPart& np, int grid, size_t smem, const mg::DeviceInfo& di, cudaStream_t st) {
+  auto kern = norm_reorder_quantize_kernel<R>;
+  static std::atomic<unsigned long long> allowed;
+  MG_CUDA_TRY(mg::allow_smem(kern, (size_t)di.smem_optin - kStaticSmem, di.device, allowed));
+  MG_CUDA_TRY(mg::launch_kernel(kern, dim3(grid), dim3(kThreads), smem, st, p, np));
+  return MG_OK;
+}
+
+}  // namespace
+
 extern "C" int mg_rms_norm_reorder_quantize(const void* X, size_t ldx, const void* R, size_t ldr, const void* W, float eps,
                                             void* U, size_t ldu, int M, int K, const int16_t* idx, int KN, int KS, int KO,
                                             uint8_t* C4, uint8_t* C6, uint8_t* C8, const size_t* pitches, uint8_t* SF4,
                                             uint8_t* SF6, uint8_t* SF8, void* stream) {
-  NormParams np{};
+  ReorderParams p;
+  NormPart np{};
   if (!(eps >= 0.f && eps <= 3.4028235e38f)) return MG_ERR_SHAPE;
   if (M > 0) {
     if (!W || (R != nullptr) != (U != nullptr)) return MG_ERR_NULL;
     if (M == 1) ldx = ldr = ldu = (size_t)(K > 0 ? K : 0);  // one row has no pitch
     if (ldx < (size_t)K || (R && (ldr < (size_t)K || ldu < (size_t)K))) return MG_ERR_SHAPE;
-    if (!mg::aligned(W, 16) || !mg::aligned(R, 16) || !mg::aligned(U, 16)) return MG_ERR_ALIGN;
+    if (!mg::aligned(W, 2) || !mg::aligned(R, 16) || !mg::aligned(U, 16)) return MG_ERR_ALIGN;
     if (ldx % 8 || (R && (ldr % 8 || ldu % 8))) return MG_ERR_ALIGN;
   }
-  int rc = fill_params(false, X, M, K, idx, KN, KS, KO, C4, C6, C8, pitches, SF4, SF6, SF8, &np.q);
-  if (rc != MG_OK || np.q.rows == 0) return rc;
+  int rc = fill_params(false, X, M, K, idx, KN, KS, KO, C4, C6, C8, pitches, SF4, SF6, SF8, &p);
+  if (rc != MG_OK || p.rows == 0) return rc;
   np.R = static_cast<const uint16_t*>(R);
   np.U = static_cast<uint16_t*>(U);
   np.W = static_cast<const uint16_t*>(W);
@@ -718,16 +749,24 @@ extern "C" int mg_rms_norm_reorder_quantize(const void* X, size_t ldx, const voi
   np.pr = ldr;
   np.pu = ldu;
   np.eps = eps;
+  np.inv_k = 1.0f / (float)K;
   mg::DeviceInfo di;
   if ((rc = mg::device_info(&di)) != MG_OK) return rc;
+  int grid = M < di.sm_count ? M : di.sm_count;
+  const int cap = mg::options().reorder_ctas;
+  if (cap > 0 && grid > cap) grid = cap;
+  // the residual is staged where two stages of one row fit with it (K up to about 19000)
+  const size_t room = (size_t)di.smem_optin - kStaticSmem;
+  np.staged = R && smem_bytes(K, 1, 2, 2) <= room - 1024;
+  int rows = 1;
+  const size_t smem = stage_shape(&p, grid, room, &rows, np.staged ? 2 : 1);
+  if (smem == 0) return MG_ERR_SHAPE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // more rows to a tile leave fewer bank conflicts in the gather; fewer fill the SMs
-  int rows = 8;
-  while (rows > 1 && ((M + rows - 1) / rows < 2 * di.sm_count || norm_smem_bytes(K, rows) > (size_t)di.smem_optin / 2)) rows /= 2;
   switch (rows) {
-    case 8: return launch_norm<8>(np, di, st);
-    case 4: return launch_norm<4>(np, di, st);
-    case 2: return launch_norm<2>(np, di, st);
-    default: return launch_norm<1>(np, di, st);
+    case 8: return launch_norm<8>(p, np, grid, smem, di, st);
+    case 4: return launch_norm<4>(p, np, grid, smem, di, st);
+    case 2: return launch_norm<2>(p, np, grid, smem, di, st);
+    default: return launch_norm<1>(p, np, grid, smem, di, st);
   }
 }
+

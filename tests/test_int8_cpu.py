@@ -83,7 +83,7 @@ def mx_norm(lib, X=P, ldx=128, R=None, ldr=0, W=P, eps=1e-6, U=None, ldu=0, M=4,
     (SHAPE, dict(ldx=120)), (SHAPE, dict(R=P, U=P, ldr=120, ldu=128)), (SHAPE, dict(R=P, U=P, ldr=128, ldu=120)),
     (NULL, dict(X=None)), (NULL, dict(W=None)), (NULL, dict(idx=None)), (NULL, dict(codes=None)), (NULL, dict(scales=None)),
     (NULL, dict(R=P, ldr=128, ldu=128)), (NULL, dict(U=P, ldr=128, ldu=128)),
-    (ALIGN, dict(X=P + 2)), (ALIGN, dict(W=P + 8)), (ALIGN, dict(ldx=132)), (ALIGN, dict(R=P + 2, U=P, ldr=128, ldu=128)),
+    (ALIGN, dict(X=P + 2)), (ALIGN, dict(W=P + 1)), (ALIGN, dict(ldx=132)), (ALIGN, dict(R=P + 2, U=P, ldr=128, ldu=128)),
     (ALIGN, dict(R=P, U=P, ldr=130, ldu=128)), (ALIGN, dict(R=P, U=P, ldr=128, ldu=129)), (ALIGN, dict(codes=P + 4)),
 ])
 def test_mx_norm_refusals(lib, want, args):
