@@ -13,6 +13,7 @@ Differences from the reference binding, all deliberate:
 """
 import contextlib
 import ctypes
+import os
 
 import torch
 
@@ -399,56 +400,27 @@ def matmul_multi(problems, flags=None):
     return outs
 
 
-# ----------------------------------------------------------------- 8-bit integers, a scale per row
+# ----------------------------------------------------------------- 8-bit integers and fused norms
 
-_ELEMENT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # MG_BF16, MG_FP16, MG_FP32
-
-
-def _on(dev, fn, *args):
-    """fn(*args, current stream of `dev`) with `dev` current."""
-    with _device(dev):
-        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+_ops_module = None
 
 
-def _rows(t, what, name, shape, dev, dtype):
-    """Row pitch (elements) of a 2-D tensor whose rows are dense and do not overlap; `shape` None: any."""
-    own, step = t.shape, t.stride()
-    if len(own) == 2 and t.device == dev and t.dtype == dtype and (shape is None or own == shape):
-        M, K = own
-        if (step[1] == 1 or K <= 1) and (step[0] >= K or M <= 1):
-            return step[0] if M > 1 else K
-        raise RuntimeError("%s: the rows of %s must have unit stride and must not overlap (strides %s)" % (what, name, step))
-    raise RuntimeError("%s: %s must be a 2-D %s tensor%s on %s, not %s %s on %s" % (
-        what, name, dtype, "" if shape is None else " of shape %s" % (tuple(shape),), dev, t.dtype, tuple(own), t.device))
-
-
-def _vector(t, what, name, n, dev, dtype):
-    if t.device != dev or t.dtype != dtype or t.numel() != n or not t.is_contiguous():
-        raise RuntimeError("%s: %s must be a contiguous %s tensor of %d elements on %s" % (what, name, dtype, n, dev))
-    return t
-
-
-def _activation(X, what):
-    """Device and row pitch of the activation that a call starts with."""
-    if not X.is_cuda:
-        raise RuntimeError("%s: X must be a CUDA tensor" % what)
-    if X.dtype not in _ELEMENT:
-        raise RuntimeError("%s: X must be bfloat16, float16 or float32, not %s" % (what, X.dtype))
-    dev = X.device
-    return dev, _rows(X, what, "X", None, dev, X.dtype)
-
-
-def _new(shape, dtype, dev):
-    return torch.empty_strided(shape, (shape[1], 1) if len(shape) == 2 else (1,), dtype=dtype, device=dev)
-
-
-def _int8_outputs(M, K, dev, out, what):
-    """(codes, row pitch, scale): the caller's, or new ones whose rows matmul_int8 can read in place."""
-    if out is None:
-        pitch = (K + 15) // 16 * 16
-        return (torch.empty_strided((M, K), (pitch, 1), dtype=torch.int8, device=dev), pitch, _new((M,), torch.float32, dev))
-    q, scale = out
-    return q, _rows(q, what, "the codes", (M, K), dev, torch.int8), _vector(scale, what, "the scale", M, dev, torch.float32)
+def _ops():
+    """The compiled torch module of the operators below (csrc/int8_bindings.cpp): checks, allocation and
+    launch in one call, because at one token the same steps in Python take longer than the kernels."""
+    global _ops_module
+    if _ops_module is None:
+        import importlib.util
+        from . import build
+        path = build.ext_path("mixedgemm_ops")
+        if not os.path.exists(path):
+            raise ImportError("mixedgemm_ops is not built; run `python -m mixedgemm_b200.build --ext`.  "
+                              "There is no fallback path.")
+        spec = importlib.util.spec_from_file_location("mixedgemm_ops", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _ops_module = module
+    return _ops_module
 
 
 def quantize_int8(X, out=None):
@@ -457,28 +429,7 @@ def quantize_int8(X, out=None):
     magnitude of the row / 127, codes rounded to nearest even.  The rows of X may be any distance
     apart; those of the codes start on 16-byte boundaries, as matmul_int8 needs them.  A row with a
     value that is not finite gets the scale NaN and codes 0.  `out` = (codes, scale) to write into."""
-    dev, ldx = _activation(X, "quantize_int8")
-    M, K = X.shape
-    q, ldq, scale = _int8_outputs(M, K, dev, out, "quantize_int8")
-    st = _on(dev, _capi.load().mg_quantize_int8, X.data_ptr(), _ELEMENT[X.dtype], M, K, ldx, q.data_ptr(), ldq,
-             scale.data_ptr())
-    if st:
-        _capi.check(st, "quantize_int8")
-    return q, scale
-
-
-def _norm_inputs(X, weight, residual, residual_out, what):
-    """Checks of the fused norms; returns (device, ldx, ldr, residual_out, ldu)."""
-    dev, ldx = _activation(X, what)
-    _vector(weight, what, "the norm's weight", X.shape[1], dev, X.dtype)
-    if residual is None:
-        if residual_out is not None:
-            raise RuntimeError("%s: residual_out without a residual" % what)
-        return dev, ldx, 0, None, 0
-    ldr = _rows(residual, what, "the residual", X.shape, dev, X.dtype)
-    if residual_out is None:
-        return dev, ldx, ldr, _new(X.shape, X.dtype, dev), X.shape[1]
-    return dev, ldx, ldr, residual_out, _rows(residual_out, what, "residual_out", X.shape, dev, X.dtype)
+    return _ops().quantize_int8(X, out)
 
 
 def rms_norm_int8(X, weight, eps=1e-6, residual=None, residual_out=None, out=None):
@@ -486,17 +437,9 @@ def rms_norm_int8(X, weight, eps=1e-6, residual=None, residual_out=None, out=Non
     u = X + residual (rounded to X's type), h = u * weight / sqrt(mean(u^2) + eps) in fp32.
     Returns (codes, scale), with a residual (codes, scale, u): u is the stream that goes on.
     weight [K] and residual [M,K] have X's type; residual_out may be `residual` (or X) itself, to
-    update the stream in place.  A row whose sum of squares is not a finite fp32 number gets the
-    scale NaN and codes 0."""
-    dev, ldx, ldr, u, ldu = _norm_inputs(X, weight, residual, residual_out, "rms_norm_int8")
-    M, K = X.shape
-    q, ldq, scale = _int8_outputs(M, K, dev, out, "rms_norm_int8")
-    st = _on(dev, _capi.load().mg_rms_norm_int8, X.data_ptr(), None if u is None else residual.data_ptr(),
-             weight.data_ptr(), eps, _ELEMENT[X.dtype], M, K, ldx, ldr, None if u is None else u.data_ptr(), ldu,
-             q.data_ptr(), ldq, scale.data_ptr())
-    if st:
-        _capi.check(st, "rms_norm_int8")
-    return (q, scale) if u is None else (q, scale, u)
+    update the stream in place (it must not overlap them in any other way).  A row whose sum of squares
+    is not a finite fp32 number gets the scale NaN and codes 0."""
+    return _ops().rms_norm_int8(X, weight, eps, residual, residual_out, out)
 
 
 def rms_norm_reorder_quantize_x(X, weight, reorder_index, KN, KS, KO, eps=1e-6, residual=None, residual_out=None,
@@ -504,34 +447,10 @@ def rms_norm_reorder_quantize_x(X, weight, reorder_index, KN, KS, KO, eps=1e-6, 
     """reorder_quantize_x of the root-mean-square norm of X [M,K] bf16 (+ residual), in one launch:
     u = bf16(X + residual), h = bf16(u * weight / sqrt(mean(u^2) + eps)).  Returns the six tensors that
     reorder_quantize_x(h, ...) returns, byte for byte, and with a residual u as a seventh.  residual_out
-    may be `residual` (or X) itself; `out` the six buffers of alloc_quantized_x().  Rows start on
-    16-byte boundaries.  A row with a sum of squares that is not finite gets NaN scales, and so does a
-    group with such an h: that row of a product is NaN, and no other."""
-    what = "rms_norm_reorder_quantize_x"
-    dev, ldx, ldr, u, ldu = _norm_inputs(X, weight, residual, residual_out, what)
-    M, K = X.shape
-    if X.dtype != torch.bfloat16:
-        raise RuntimeError("%s: X must be bfloat16, not %s" % (what, X.dtype))
-    if K != KN + KS + KO:
-        raise RuntimeError("%s: K = %d does not match KN+KS+KO" % (what, K))
-    _vector(reorder_index, what, "reorder_index", K, dev, torch.int16)
-    if out is None:
-        out = alloc_quantized_x(M, KN, KS, KO, dev)
-    else:
-        _check_codes(out[:3], what)
-        for t, n in zip(out[:3], (KN // 2, KS // 4 * 3, KO)):
-            if tuple(t.shape) != (M, n) or t.device != dev:
-                raise RuntimeError("%s: a code buffer has shape %s where %s is expected" % (what, tuple(t.shape), (M, n)))
-        for t, k in zip(out[3:], (KN, KS, KO)):
-            if t.numel() < _sf_bytes(M, k) or t.device != dev or t.dtype != torch.uint8 or not t.is_contiguous():
-                raise RuntimeError("%s: a scale buffer is too small or on another device" % what)
-    XN, XS, XO, s4, s6, s8 = out
-    st = _on(dev, _capi.load().mg_rms_norm_reorder_quantize, X.data_ptr(), ldx, None if u is None else residual.data_ptr(),
-             ldr, weight.data_ptr(), eps, None if u is None else u.data_ptr(), ldu, M, K, reorder_index.data_ptr(), KN, KS,
-             KO, _ptr(XN), _ptr(XS), _ptr(XO), _pitches((XN, XS, XO)), _ptr(s4), _ptr(s6), _ptr(s8))
-    if st:
-        _capi.check(st, what)
-    return tuple(out) if u is None else tuple(out) + (u,)
+    may be `residual` (or X) itself, as in rms_norm_int8; `out` the six buffers of alloc_quantized_x().
+    Rows start on 16-byte boundaries.  A row with a sum of squares that is not finite gets NaN scales, and
+    so does a group with such an h: that row of a product is NaN, and no other."""
+    return _ops().rms_norm_reorder_quantize_x(X, weight, reorder_index, KN, KS, KO, eps, residual, residual_out, out)
 
 
 def matmul_int8(A, B, scale_a, scale_b, bias=None, out=None, out_dtype=None):
@@ -540,32 +459,7 @@ def matmul_int8(A, B, scale_a, scale_b, bias=None, out=None, out_dtype=None):
     `out_dtype` (bfloat16 unless given; float16 or float32).  scale_a [M], scale_b [N] and bias [N]
     are fp32.  Rows of A and B start on 16-byte boundaries (those of quantize_int8 do); K is at most
     131071.  `out` [M,N] receives the result instead of a new tensor; its rows may be any distance apart."""
-    what = "matmul_int8"
-    if not A.is_cuda:
-        raise RuntimeError("%s: A must be a CUDA tensor" % what)
-    dev = A.device
-    lda = _rows(A, what, "A", None, dev, torch.int8)
-    ldb = _rows(B, what, "B", None, dev, torch.int8)
-    M, K = A.shape
-    N, Kb = B.shape
-    if Kb != K:
-        raise RuntimeError("%s: A has rows of %d elements, B of %d" % (what, K, Kb))
-    _vector(scale_a, what, "scale_a", M, dev, torch.float32)
-    _vector(scale_b, what, "scale_b", N, dev, torch.float32)
-    if bias is not None:
-        _vector(bias, what, "the bias", N, dev, torch.float32)
-    if out is None:
-        out, ldd = _new((M, N), out_dtype or torch.bfloat16, dev), N
-    else:
-        ldd = _rows(out, what, "out", (M, N), dev, out_dtype or out.dtype)
-    if out.dtype not in _ELEMENT:
-        raise RuntimeError("%s: the result must be bfloat16, float16 or float32, not %s" % (what, out.dtype))
-    st = _on(dev, _capi.load().mg_matmul_int8, A.data_ptr(), lda, B.data_ptr(), ldb, scale_a.data_ptr(),
-             scale_b.data_ptr(), None if bias is None else bias.data_ptr(), M, N, K, out.data_ptr(),
-             _ELEMENT[out.dtype], ldd)
-    if st:
-        _capi.check(st, "matmul_int8")
-    return out
+    return _ops().matmul_int8(A, B, scale_a, scale_b, bias, out, out_dtype)
 
 
 def set_option(name, value):

@@ -1,11 +1,12 @@
 """In-tree build of the native pieces (no JIT cache: the built files sit beside the sources).
 
   python -m mixedgemm_b200.build            # libmixedgemm_b200.so (nvcc, sm_100a)
-  python -m mixedgemm_b200.build --ext      # + the pybind11/torch module `mixedgemm`
+  python -m mixedgemm_b200.build --ext      # + the pybind11/torch modules `mixedgemm` and `mixedgemm_ops`
 
 `libmixedgemm_b200.so` is the C-ABI library declared in include/mixedgemm_c.h.
 `mixedgemm*.so` (under mixedgemm_b200/ext/) is the drop-in Python module with the
-reference's entry points; it links against the C-ABI library.
+reference's entry points; it links against the C-ABI library, and so does `mixedgemm_ops*.so`
+beside it, through which the package runs its 8-bit operators and fused norms.
 """
 import argparse
 import glob
@@ -57,33 +58,42 @@ def build_lib(force=False, verbose=False):
     return LIB
 
 
-def ext_path():
+# torch modules under ext/ and the file each is made of
+EXT_SOURCES = {"mixedgemm": "bindings.cpp", "mixedgemm_ops": "int8_bindings.cpp"}
+
+
+def ext_path(name="mixedgemm"):
     suffix = sysconfig.get_config_var("EXT_SUFFIX")
-    return os.path.join(EXT_DIR, "mixedgemm" + suffix)
+    return os.path.join(EXT_DIR, name + suffix)
 
 
 def build_ext(force=False, verbose=False):
-    """pybind11 + libtorch module `mixedgemm` (the reference's module name)."""
+    """pybind11 + libtorch modules: `mixedgemm` (the reference's module name) and `mixedgemm_ops` (the
+    operators of this package that take torch tensors through compiled code)."""
     import torch
     from torch.utils import cpp_extension
     build_lib(force=False, verbose=verbose)
-    src = os.path.join(CSRC, "bindings.cpp")
-    out = ext_path()
-    if not force and not _stale(out, [src, LIB] + glob.glob(os.path.join(INC, "*.h"))):
-        return out
     os.makedirs(EXT_DIR, exist_ok=True)
     tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-w", "-DTORCH_EXTENSION_NAME=mixedgemm",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
-           "-I" + INC, "-I" + sysconfig.get_paths()["include"], "-I/usr/local/cuda/include"]
-    cmd += ["-I" + p for p in cpp_extension.include_paths()]
-    cmd += [src, "-o", out, "-L" + PKG, "-lmixedgemm_b200", "-L" + tlib, "-ltorch", "-ltorch_cpu", "-lc10",
-            "-ltorch_python", "-lc10_cuda", "-ltorch_cuda", "-L/usr/local/cuda/lib64", "-lcudart",
-            "-Wl,-rpath,$ORIGIN/..", "-Wl,-rpath," + tlib]
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.check_call(cmd)
-    return out
+    procs = []
+    for name, source in EXT_SOURCES.items():
+        src, out = os.path.join(CSRC, source), ext_path(name)
+        if not force and not _stale(out, [src, LIB] + glob.glob(os.path.join(INC, "*.h"))):
+            continue
+        cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-w", "-DTORCH_EXTENSION_NAME=" + name,
+               "-DTORCH_API_INCLUDE_EXTENSION_H", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+               "-I" + INC, "-I" + sysconfig.get_paths()["include"], "-I/usr/local/cuda/include"]
+        cmd += ["-I" + p for p in cpp_extension.include_paths()]
+        cmd += [src, "-o", out, "-L" + PKG, "-lmixedgemm_b200", "-L" + tlib, "-ltorch", "-ltorch_cpu", "-lc10",
+                "-ltorch_python", "-lc10_cuda", "-ltorch_cuda", "-L/usr/local/cuda/lib64", "-lcudart",
+                "-Wl,-rpath,$ORIGIN/..", "-Wl,-rpath," + tlib]
+        if verbose:
+            print(" ".join(cmd))
+        procs.append((subprocess.Popen(cmd), cmd))
+    for p, cmd in procs:
+        if p.wait() != 0:
+            raise RuntimeError("g++ failed: " + " ".join(cmd))
+    return ext_path()
 
 
 if __name__ == "__main__":

@@ -63,8 +63,10 @@ def test_product_refusals(lib, want, args):
     assert product(lib, **args) == want
 
 
-def test_python_layer_refuses_tensors_off_the_gpu(lib):
+def test_python_layer_refuses_tensors_off_the_gpu():
     import mixedgemm_b200 as mg
+    from mixedgemm_b200 import build
+    build.build_ext()
     x, q, s = torch.zeros(2, 32), torch.zeros(2, 32, dtype=torch.int8), torch.ones(2)
     for call in (lambda: mg.quantize_int8(x), lambda: mg.rms_norm_int8(x, torch.ones(32)),
                  lambda: mg.matmul_int8(q, q, s, s)):
