@@ -36,7 +36,7 @@ const OptionSlot kOptionSlots[] = {
     {"REORDER_CTAS", &mg::Options::reorder_ctas, 0}, {"FAULT_SKIP_LOAD", &mg::Options::fault_skip_load, 0},
     {"GEMM_SCHED", &mg::Options::gemm_sched, 1},    {"GEMM_MAX_CLUSTERS", &mg::Options::gemm_max_clusters, 0},
     {"INT8_TOKENS", &mg::Options::int8_tokens, -1}, {"INT8_SPLIT", &mg::Options::int8_split, -1},
-    {"INT8_PAIR", &mg::Options::int8_pair, -1},
+    {"INT8_PAIR", &mg::Options::int8_pair, -1},     {"INT8_FEW", &mg::Options::int8_few, -1},
 };
 mg::Options g_options;
 bool g_options_ready = false;

@@ -319,6 +319,114 @@ __global__ void __launch_bounds__(kThreads) int8_gemm_kernel(const Int8Params p,
   if (warp == 1) ptx::tmem_dealloc(tmem, BT);
 }
 
+// ---------------------------------------------------------------- single tokens
+// One or two tokens: the weights are read once, straight into registers, and multiplied with dp4a.  The
+// product is bound by their bytes, and what the tensor-core form adds to reading them (staging, the MMA's
+// and the cluster's hand-overs) shows: 1 x 4096 x 4096 5.0 us here against 6.5 there, 1 x 6144 x 4096 6.7 / 8.4,
+// 1 x 4096 x 14336 11.4 / 12.8, 2 x 14336 x 4096 11.5 / 13.3.  With four tokens dp4a and the tokens' bytes are
+// the bound (4096 x 14336: 13.4 / 12.7).  A warp takes four channels, so that the tokens' bytes, which all warps
+// share through L1, serve four rows (two rows: 13.9 us at 1 x 14336 x 4096, four: 11.4); `parts` warps of a
+// CTA share them when there are too few channels to keep the memory busy.
+constexpr int kFewWarps = 4, kFewRows = 4, kFewUnroll = 4, kFewTokens = 2;
+
+__device__ __forceinline__ uint4 load_once(const void* p) {  // read once: not worth a place in L1
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+template <int MT, typename T>
+__global__ void __launch_bounds__(kFewWarps * 32) int8_few_tokens_kernel(const Int8Params p, const int8_t* __restrict__ A,
+                                                                         size_t lda, const int8_t* __restrict__ B, size_t ldb,
+                                                                         int K, int parts) {
+  __shared__ int s_sum[kFewWarps][kFewRows * MT];
+  ptx::grid_dep_launch_dependents();
+  ptx::grid_dep_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = warp / parts, part = warp - group * parts;
+  const int n0 = (int)(blockIdx.x * (kFewWarps / parts) + group) * kFewRows;
+  // rows beyond the last channel or token stand for the last one; nothing of them is stored
+  const int8_t* w[kFewRows];
+  const int8_t* x[MT];
+#pragma unroll
+  for (int r = 0; r < kFewRows; ++r) w[r] = B + (size_t)min(n0 + r, p.N - 1) * ldb;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) x[m] = A + (size_t)min(m, p.M - 1) * lda;
+
+  int sum[kFewRows][MT] = {};
+  const int chunks = K >> 4;  // whole 16-byte vectors
+  const int c1 = (int)((long long)chunks * (part + 1) / parts);
+  for (int c = (int)((long long)chunks * part / parts) + lane; c < c1; c += 32 * kFewUnroll) {
+    uint4 wv[kFewRows][kFewUnroll];
+#pragma unroll
+    for (int u = 0; u < kFewUnroll; ++u)
+#pragma unroll
+      for (int r = 0; r < kFewRows; ++r)
+        wv[r][u] = c + 32 * u < c1 ? load_once(w[r] + (size_t)(c + 32 * u) * 16) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < kFewUnroll; ++u) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        uint4 xv = make_uint4(0, 0, 0, 0);
+        if (c + 32 * u < c1) xv = __ldg(reinterpret_cast<const uint4*>(x[m] + (size_t)(c + 32 * u) * 16));
+#pragma unroll
+        for (int r = 0; r < kFewRows; ++r) {
+          sum[r][m] = __dp4a((int)wv[r][u].x, (int)xv.x, sum[r][m]);
+          sum[r][m] = __dp4a((int)wv[r][u].y, (int)xv.y, sum[r][m]);
+          sum[r][m] = __dp4a((int)wv[r][u].z, (int)xv.z, sum[r][m]);
+          sum[r][m] = __dp4a((int)wv[r][u].w, (int)xv.w, sum[r][m]);
+        }
+      }
+    }
+  }
+  // the last K % 16 bytes of a row, one a lane
+  if (part == parts - 1 && lane < (K & 15)) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < kFewRows; ++r) sum[r][m] += (int)w[r][chunks * 16 + lane] * (int)x[m][chunks * 16 + lane];
+  }
+#pragma unroll
+  for (int r = 0; r < kFewRows; ++r)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) sum[r][m] = __reduce_add_sync(0xffffffffu, sum[r][m]);
+  if (parts > 1) {
+    if (lane == 0) {
+#pragma unroll
+      for (int r = 0; r < kFewRows; ++r)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) s_sum[warp][r * MT + m] = sum[r][m];
+    }
+    __syncthreads();
+    if (part != 0) return;
+  }
+  // lane r * MT + m finishes channel n0 + r of token m
+  int total = 0;
+#pragma unroll
+  for (int r = 0; r < kFewRows; ++r)
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+      if (lane == r * MT + m) total = sum[r][m];
+  const int n = n0 + lane / MT, m = lane % MT;
+  if (lane < kFewRows * MT && n < p.N && m < p.M) {
+    for (int i = 1; i < parts; ++i) total += s_sum[warp + i][lane];
+    const float bias = p.bias ? p.bias[n] : 0.f;
+    static_cast<T*>(p.D)[(size_t)m * p.ldd + n] = round_to<T>(__fmaf_rn(__fmul_rn((float)total, p.sa[m]), p.sb[n], bias));
+  }
+}
+
+template <int MT, typename T>
+int launch_few(const Int8Params& p, const int8_t* A, size_t lda, const int8_t* B, size_t ldb, int K, int sms, cudaStream_t st) {
+  const int groups = (p.N + kFewRows - 1) / kFewRows;
+  // 16 warps an SM at least, but no part of a row shorter than one turn of its warp
+  int parts = 1;
+  while (parts < kFewWarps && (long long)groups * parts < 16ll * sms && K >= parts * 2 * 32 * 16) parts *= 2;
+  const int per_cta = kFewWarps / parts;
+  MG_CUDA_TRY(mg::launch_kernel(int8_few_tokens_kernel<MT, T>, dim3((groups + per_cta - 1) / per_cta), dim3(kFewWarps * 32), 0, st, p,
+                                A, lda, B, ldb, K, parts));
+  return MG_OK;
+}
+
 // ---------------------------------------------------------------- CTA-pair form
 // Two CTAs of a cluster compute 256 channels x BT tokens with tcgen05.mma.cta_group::2: each stages
 // its own 128 channels and half of the tokens, and one instruction of the leader drives both tensor
@@ -631,7 +739,10 @@ Form choose_form(int M, int N, int K, const mg::DeviceInfo& di, const mg::Option
 template <typename T>
 int launch_int8(const Int8Params& p, const int8_t* A, size_t lda, const int8_t* B, size_t ldb, int K,
                 const mg::DeviceInfo& di, cudaStream_t st) {
-  const Form f = choose_form<T>(p.M, p.N, K, di, mg::options());
+  const mg::Options opt = mg::options();
+  if (opt.int8_few != 0 && p.M <= kFewTokens)
+    return p.M == 1 ? launch_few<1, T>(p, A, lda, B, ldb, K, di.sm_count, st) : launch_few<2, T>(p, A, lda, B, ldb, K, di.sm_count, st);
+  const Form f = choose_form<T>(p.M, p.N, K, di, opt);
   CUtensorMap w, t;
   int rc;
   if ((rc = mg::make_map(&w, CU_TENSOR_MAP_DATA_TYPE_UINT8, B, K, p.N, ldb, 128, 128))) return rc;

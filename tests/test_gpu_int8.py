@@ -234,6 +234,7 @@ def test_product_against_64_bits(M, N, K, dtype):
 @pytest.mark.parametrize("tile", [32, 64, 128])
 @pytest.mark.parametrize("split", [1, 2, 4, 8])
 def test_product_of_every_tile_and_split(tile, split, mgopt):
+    mgopt.set("INT8_FEW", 0)
     mgopt.set("INT8_PAIR", 0)
     mgopt.set("INT8_TOKENS", tile)
     mgopt.set("INT8_SPLIT", split)
@@ -245,9 +246,18 @@ def test_product_of_every_tile_and_split(tile, split, mgopt):
 @pytest.mark.parametrize("tile", [128, 256])
 def test_product_of_the_pair_form(tile, dtype, mgopt):
     """One tile, many tiles to a pair (both accumulators, several turns), ragged edges, one slice of K."""
+    mgopt.set("INT8_FEW", 0)
     mgopt.set("INT8_PAIR", tile)
     for M, N, K in ((1, 1, 1), (200, 130, 1024), (140, 257, 1931), (513, 640, 128), (1000, 5000, 300), (2300, 3000, 128)):
         run_product(M, N, K, dtype, with_bias=True, seed=tile)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [1, 2, 3, 4])
+def test_product_of_single_tokens(M, dtype):
+    """Whole rows to a warp and shared ones, odd channels, tails of K shorter than a vector."""
+    for N, K in ((1, 1), (1, 15), (3, 16), (5, 17), (130, 511), (1000, 4096), (77, 14336), (5001, 1200), (2, 131071)):
+        run_product(M, N, K, dtype, with_bias=N % 2 == 0, seed=M + N)
 
 
 def test_product_does_not_depend_on_tile_or_split(mgopt):
@@ -265,6 +275,9 @@ def test_product_does_not_depend_on_tile_or_split(mgopt):
     for pair in (128, 256):
         mgopt.set("INT8_PAIR", pair)
         assert torch.equal(mg.matmul_int8(av, bv, sa, sb), ref)
+    few = mg.matmul_int8(av[:2], bv, sa[:2], sb)
+    mgopt.set("INT8_FEW", 0)
+    assert torch.equal(few, mg.matmul_int8(av[:2], bv, sa[:2], sb)) and torch.equal(few, ref[:2])
 
 
 def test_product_of_the_longest_row_does_not_overflow():
