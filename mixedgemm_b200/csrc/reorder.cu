@@ -106,6 +106,31 @@ struct RowCtx {
   uint32_t row;
 };
 
+// Two fp32 operations in one instruction, each lane rounded as the scalar form rounds it.
+__device__ __forceinline__ uint64_t f2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void un2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 // round(x * 2^e) to the nearest integer, halves away from zero, sign of x kept on a zero result.
 // `rs` is 2^e * (1 + 2^-12): the fused multiply-add forms x * rs + 1.5 * 2^23 exactly and rounds it
 // once, to nearest even, which leaves the wanted integer in the low mantissa bits.  The factor
@@ -114,10 +139,13 @@ struct RowCtx {
 // Subtracting the constant gives the integer back as a float, and or-ing the sign of x restores
 // "-0".  All three run on the FMA / ALU pipes; the conversion unit, which a round-to-integer
 // instruction would occupy for sixteen cycles per warp, stays free for the code conversions.
-__device__ __forceinline__ float scale_round(float x, float rs) {
-  const float kMagic = 12582912.0f;
-  const float r = __fadd_rn(__fmaf_rn(x, rs, kMagic), -kMagic);
-  return __uint_as_float(__float_as_uint(r) | (__float_as_uint(x) & 0x80000000u));
+// Two values at a time.
+__device__ __forceinline__ void scale_round(float& x, float& y, uint64_t rs2) {
+  const uint64_t magic = f2(12582912.0f, 12582912.0f), unmagic = f2(-12582912.0f, -12582912.0f);
+  float a, b;
+  un2(add2(fma2(f2(x, y), rs2, magic), unmagic), a, b);
+  x = __uint_as_float(__float_as_uint(a) | (__float_as_uint(x) & 0x80000000u));
+  y = __uint_as_float(__float_as_uint(b) | (__float_as_uint(y) & 0x80000000u));
 }
 
 // The 32 values of group g (already gathered) and their largest magnitude: scale, quantise, pack, store.
@@ -134,8 +162,9 @@ __device__ __forceinline__ void emit_group(const ReorderParams& p, const RowCtx&
   so.sf[rc.sf_row + (gs & 3) + (size_t)(gs >> 2) * 512 + (size_t)rc.row_blk * 512 * so.katoms] = (uint8_t)(nan ? 255 : sf);
   const float rs = __uint_as_float(((unsigned)(254 - sf) << 23) | 0x800u);  // 2^(127-sf) * (1 + 2^-12)
 
+  const uint64_t rs2 = f2(rs, rs);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) x[i] = scale_round(x[i], rs);
+  for (int i = 0; i < 32; i += 2) scale_round(x[i], x[i + 1], rs2);
 
   uint8_t* out = so.codes + (size_t)rc.row * so.pitch;
   if (fmt == 0) {
@@ -223,6 +252,12 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+__device__ __forceinline__ uint32_t add_pair(uint32_t a, uint32_t b) {
+  float lo, hi;
+  un2(add2(f2(bf16_lo(a), bf16_hi(a)), f2(bf16_lo(b), bf16_hi(b))), lo, hi);
+  return bf16_pair(lo, hi);
+}
+
 // The same behind a root-mean-square norm: the staged row holds u, and h = bf16((u w) v) is formed on the
 // way from shared memory to the codes.  wp_addr: the norm's weight in reordered order, so that a group's
 // 32 weights are one run of 64 bytes, the same for all rows that the lanes of a warp walk.
@@ -230,6 +265,7 @@ __device__ __forceinline__ void quantise_norm_group(const ReorderParams& p, cons
                                                     uint32_t wp_addr, int g, float v, bool nan_row) {
   float x[32];
   float maxv = 0.f;
+  const uint64_t v2 = f2(v, v);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const uint4 iv = lds_v4(idx2_addr + g * 64 + q * 16), wv = lds_v4(wp_addr + g * 64 + q * 16);
@@ -238,7 +274,9 @@ __device__ __forceinline__ void quantise_norm_group(const ReorderParams& p, cons
     for (int j = 0; j < 4; ++j) {
       const unsigned lo = lds_u16(rc.smem_row + (o[j] & 0xFFFFu));
       const unsigned hi = lds_u16(rc.smem_row + (o[j] >> 16));
-      const uint32_t h = bf16_pair(__uint_as_float(lo << 16) * bf16_lo(w[j]) * v, __uint_as_float(hi << 16) * bf16_hi(w[j]) * v);
+      float a, b;
+      un2(mul2(mul2(f2(__uint_as_float(lo << 16), __uint_as_float(hi << 16)), f2(bf16_lo(w[j]), bf16_hi(w[j]))), v2), a, b);
+      const uint32_t h = bf16_pair(a, b);
       x[q * 8 + j * 2] = bf16_lo(h);
       x[q * 8 + j * 2 + 1] = bf16_hi(h);
       asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(maxv) : "f"(maxv), "f"(x[q * 8 + j * 2]), "f"(x[q * 8 + j * 2 + 1]));
@@ -409,7 +447,8 @@ __device__ __forceinline__ void reorder_quantize_cta(const ReorderParams& p, int
         constexpr int kWarpsPerRow = kConsumerWarps / R;
         const int nr = warp / kWarpsPerRow, nlane = (warp % kWarpsPerRow) * 32 + lane;
         const int nrow = row_begin + it * R + nr;
-        float sum = 0.f;
+        float sum, sum_hi;
+        uint64_t sum2 = 0;  // two zeros
         if (nrow < row_end && !*stop) {
           const uint32_t xs = ptx::smem_u32(tiles + (size_t)s * stage_bytes) + nr * pitch, rs = xs + R * pitch;
           const bool add = np->R != nullptr;
@@ -420,21 +459,23 @@ __device__ __forceinline__ void reorder_quantize_cta(const ReorderParams& p, int
             uint4 a = lds_v4(xs + i * 16);
             if (add) {
               const uint4 b = np->staged ? lds_v4(rs + i * 16) : rg[i];
-              a.x = bf16_pair(bf16_lo(a.x) + bf16_lo(b.x), bf16_hi(a.x) + bf16_hi(b.x));
-              a.y = bf16_pair(bf16_lo(a.y) + bf16_lo(b.y), bf16_hi(a.y) + bf16_hi(b.y));
-              a.z = bf16_pair(bf16_lo(a.z) + bf16_lo(b.z), bf16_hi(a.z) + bf16_hi(b.z));
-              a.w = bf16_pair(bf16_lo(a.w) + bf16_lo(b.w), bf16_hi(a.w) + bf16_hi(b.w));
+              a.x = add_pair(a.x, b.x);
+              a.y = add_pair(a.y, b.y);
+              a.z = add_pair(a.z, b.z);
+              a.w = add_pair(a.w, b.w);
               ug[i] = a;
               ptx::sts_v4(xs + i * 16, a.x, a.y, a.z, a.w);
             }
             const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              sum = fmaf(bf16_lo(w[k]), bf16_lo(w[k]), sum);
-              sum = fmaf(bf16_hi(w[k]), bf16_hi(w[k]), sum);
+              const uint64_t u = f2(bf16_lo(w[k]), bf16_hi(w[k]));
+              sum2 = fma2(u, u, sum2);
             }
           }
         }
+        un2(sum2, sum, sum_hi);
+        sum += sum_hi;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) s_sum[it & 1][warp] = sum;  // (the other half may still be read)
