@@ -46,6 +46,7 @@ struct Int8Params {
   size_t ldd;
   int* status;
   long long wait_cycles;
+  int skip_load;  // fault injection for the bounded-wait test: the first CTA withholds its n-th stage load (0 = off)
 };
 
 // Instruction descriptor: 32-bit integer accumulator, signed 8-bit operands, both K-major.
@@ -210,9 +211,10 @@ __global__ void __launch_bounds__(kThreads) int8_gemm_kernel(const Int8Params p,
     const bool leader = ptx::elect_one();
     int slot = 0;
     uint32_t phase = 0;
+    int skip = (blockIdx.x | blockIdx.y | blockIdx.z) == 0 ? p.skip_load : 0;
     for (int s = s0; s < s1; ++s) {
       if (!wait_parity(empty_bar(slot), phase ^ 1u, stop, p.status, p.wait_cycles, 1)) break;
-      if (leader) {
+      if (leader && !(skip > 0 && --skip == 0)) {
         const uint32_t sbase = base + slot * C::STAGE_BYTES, fb = full_bar(slot);
         ptx::mbar_expect_tx(fb, C::STAGE_BYTES);
         ptx::tma_load_2d(sbase, &tmW, s * 128, n0, fb);
@@ -505,6 +507,7 @@ int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tm
     int slot = 0;
     uint32_t phase = 0;
     bool live = true;
+    int skip = blockIdx.x == 0 ? p.skip_load : 0;
     for (int i = 0; i < count && live; ++i) {
       int n0, m0;
       locate(i, n0, m0);
@@ -512,7 +515,7 @@ int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tm
 #pragma unroll 1
       for (int s = 0; s < p.stages; ++s) {
         if (!wait_parity(empty_bar(slot), phase ^ 1u, stop, p.status, p.wait_cycles, 1)) { live = false; break; }
-        if (leader) {
+        if (leader && !(skip > 0 && --skip == 0)) {
           const uint32_t sbase = base + slot * C::STAGE_BYTES;
           const uint32_t fb = ptx::map_to_cta(full_bar(slot), 0);
           if (rank == 0) ptx::mbar_expect_tx(full_bar(slot), 2 * C::STAGE_BYTES);
@@ -785,6 +788,7 @@ extern "C" int mg_matmul_int8(const int8_t* A, size_t lda, const int8_t* B, size
   p.D = D;
   p.ldd = ldd;
   p.wait_cycles = mg::wait_limit_cycles();
+  p.skip_load = mg::options().fault_skip_load;
   if ((rc = mg::device_status_word(&p.status)) != MG_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == MG_BF16) return launch_int8<__nv_bfloat16>(p, A, lda, B, ldb, K, di, st);

@@ -168,19 +168,18 @@ def _products_fake(x, weight_parts, fused_parts):
 
 
 # the same behind a root-mean-square norm: its last output is the stream after the residual's addition
-# (one element when there is no residual)
-@torch.library.custom_op("mixedgemm_b200::mixed_norm_linear", mutates_args=("act_scratch",))
+# (one element when there is no residual).  The quantised activation is allocated by the call.
+@torch.library.custom_op("mixedgemm_b200::mixed_norm_linear", mutates_args=())
 def mixed_norm_linear(x: torch.Tensor, residual: Optional[torch.Tensor], norm_weight: torch.Tensor, eps: float,
                       reorder_index: torch.Tensor, split: List[int], weight_parts: List[torch.Tensor],
-                      fused_parts: List[torch.Tensor], act_scratch: List[torch.Tensor]) -> List[torch.Tensor]:
+                      fused_parts: List[torch.Tensor]) -> List[torch.Tensor]:
     KN, KS, KO = split
-    A = api.rms_norm_reorder_quantize_x(x, norm_weight, reorder_index, KN, KS, KO, eps=eps, residual=residual,
-                                        out=tuple(act_scratch))
+    A = api.rms_norm_reorder_quantize_x(x, norm_weight, reorder_index, KN, KS, KO, eps=eps, residual=residual)
     return _products(A[:6], x.size(0), weight_parts, fused_parts) + [A[6] if residual is not None else x.new_empty(1)]
 
 
 @mixed_norm_linear.register_fake
-def _(x, residual, norm_weight, eps, reorder_index, split, weight_parts, fused_parts, act_scratch):
+def _(x, residual, norm_weight, eps, reorder_index, split, weight_parts, fused_parts):
     return _products_fake(x, weight_parts, fused_parts) + [x.new_empty(x.shape if residual is not None else (1,))]
 
 
@@ -261,7 +260,7 @@ class MixedLinear(torch.nn.Module):
         else:
             *outs, stream = torch.ops.mixedgemm_b200.mixed_norm_linear(
                 x2, _residual_rows(residual, x), self.norm_weight, self.eps, self.reorder_index, list(self.split),
-                self._parts, self._fused_parts, self._scratch(M, x2.device))
+                self._parts, self._fused_parts)
         if len(outs) != len(self.weights):  # the decode path: one product over the concatenated weight
             Y, outs, n0 = outs[0], [], 0
             for w in self.weights:

@@ -397,3 +397,134 @@ def test_norm_then_product_on_a_side_stream_and_in_two_graphs():
     for i in range(2):
         assert torch.equal(outs[i][0], want[2 + i][0]) and torch.equal(outs[i][1], want[2 + i][1])
     assert mg.device_status() == 0
+
+
+# ------------------------------------------------------------------------------ where calls go wrong
+
+@pytest.mark.parametrize("opts, M", [(dict(INT8_PAIR=0, INT8_TOKENS=64, INT8_SPLIT=1), 40), (dict(INT8_PAIR=0, INT8_TOKENS=32, INT8_SPLIT=4), 20),
+                                     (dict(INT8_PAIR=256), 700)])
+def test_a_wait_that_runs_out_is_reported_and_the_context_survives(opts, M, mgopt):
+    """Host-side fault injection: the first CTA withholds its second stage load.  With the wait limit at
+    1 ms the kernel gives up, stores nothing of that tile and returns; the status word says so once."""
+    import mixedgemm_b200 as mg
+    for name, v in opts.items():
+        mgopt.set(name, v)
+    N, K = 900, 2048
+    _, av = codes(M, K, 1)
+    _, bv = codes(N, K, 2)
+    sa, sb = torch.rand(M, device="cuda") + 1, torch.rand(N, device="cuda") + 1
+    want = mg.matmul_int8(av, bv, sa, sb)
+    torch.cuda.synchronize()
+    mg.set_wait_limit_us(1000)
+    mgopt.set("FAULT_SKIP_LOAD", 2)
+    out = torch.full((M, N), 7.0, dtype=torch.bfloat16, device="cuda")
+    mg.matmul_int8(av, bv, sa, sb, out=out)
+    torch.cuda.synchronize()
+    assert mg.device_status() & (1 | 2 | 8)
+    assert bool((out[:20, :128] == 7).all())  # the tile of the CTA that gave up
+    mgopt.set("FAULT_SKIP_LOAD", 0)
+    mg.set_wait_limit_us(0)
+    assert mg.device_status() == 0
+    assert torch.equal(mg.matmul_int8(av, bv, sa, sb), want)
+    assert mg.device_status() == 0
+
+
+def test_offsets_beyond_32_bits():
+    import mixedgemm_b200 as mg
+    M, K = 140001, 16384  # 2.3e9 elements, 4.6 GB
+    x = torch.empty(M, K, dtype=torch.bfloat16, device="cuda")
+    for r0 in range(0, M, 20000):
+        x[r0:r0 + 20000].normal_()
+    rows = [0, 1, 70000, 131071, 131072, M - 2, M - 1]
+    q, s = mg.quantize_int8(x)
+    part = x[rows].cpu()
+    wq, ws = want_codes(part)
+    assert np.array_equal(q[rows].cpu().numpy(), wq) and np.array_equal(s[rows].cpu().numpy(), ws)
+    w = (1 + 0.2 * torch.randn(K, generator=gen(3))).to(torch.bfloat16)
+    got = mg.rms_norm_int8(x, w.cuda(), eps=1e-5, residual=x, residual_out=x, out=(q, s))
+    check_norm([t[rows] for t in got], part, w, part, 1e-5)
+    # codes of 2.3 GB times a few channels, and a result of 2.6e9 elements
+    b, bv = codes(40, K, 1)
+    sb = torch.rand(40)
+    y = mg.matmul_int8(q, bv, s, sb.cuda(), out_dtype=torch.float32)
+    check_product(y[rows], q[rows].cpu(), b, s[rows].cpu(), sb, None)
+    del x, y, got
+    M, N, K = 65537, 40000, 48
+    a, av = codes(M, K, 2)
+    b, bv = codes(N, K, 3)
+    sa, sb = torch.rand(M) * 0.01, torch.rand(N) * 0.01
+    y = mg.matmul_int8(av, bv, sa.cuda(), sb.cuda())
+    rows = [0, 53687, 53688, M - 1]
+    check_product(y[rows], a[rows], b, sa[rows], sb, None)
+    assert mg.device_status() == 0
+
+
+def test_first_calls_inside_a_capture():
+    """A fresh process whose first call of every form is made while a graph is being captured."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+import mixedgemm_b200 as mg
+torch.manual_seed(0)
+shapes = [(1, 512, 1024), (20, 512, 4096), (60, 4096, 512), (100, 512, 1024), (700, 4096, 512), (150, 6000, 256)]
+xs = [torch.randn(M, K, device="cuda", dtype=torch.bfloat16) for M, N, K in shapes]
+ws = [torch.randn(N, K, device="cuda", dtype=torch.bfloat16) for M, N, K in shapes]
+g1 = [torch.ones(K, device="cuda", dtype=torch.bfloat16) for M, N, K in shapes]
+idx = [torch.arange(K, device="cuda").to(torch.int16) for M, N, K in shapes]
+def run():
+    outs = []
+    for x, w, g, i in zip(xs, ws, g1, idx):
+        q, s, u = mg.rms_norm_int8(x, g, residual=x)
+        b, sb = mg.quantize_int8(w)
+        K = x.shape[1]
+        outs += [mg.matmul_int8(q, b, s, sb), u] + list(mg.rms_norm_reorder_quantize_x(x, g, i, K // 2, K // 4, K // 4)[:3])
+    return outs
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = run()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, run()))
+assert mg.device_status() == 0
+print("same")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr
+
+
+def test_two_host_threads_on_their_own_streams():
+    import threading
+    import mixedgemm_b200 as mg
+    N, K = 600, 1024
+    bq, sb = mg.quantize_int8((torch.randn(N, K, generator=gen(5)) * 0.02).cuda())
+    w = torch.ones(K, dtype=torch.bfloat16, device="cuda")
+    xs = [tokens(M, K, torch.bfloat16, seed=M).cuda() for M in (1, 9, 70, 300)]
+
+    def layer(x):
+        q, s, u = mg.rms_norm_int8(x, w, residual=x)
+        return mg.matmul_int8(q, bq, s, sb), u
+
+    want = [layer(x) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for i in range(40):
+                    j = (i + k) % len(xs)
+                    got = layer(xs[j])
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[j])):
+                        bad.append((k, i))
+        except Exception as e:  # noqa: BLE001
+            bad.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(3)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad, bad
+    assert mg.device_status() == 0

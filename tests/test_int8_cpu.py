@@ -90,3 +90,49 @@ def mx_norm(lib, X=P, ldx=128, R=None, ldr=0, W=P, eps=1e-6, U=None, ldu=0, M=4,
 ])
 def test_mx_norm_refusals(lib, want, args):
     assert mx_norm(lib, **args) == want
+
+
+def test_shapes_of_the_torch_operators():
+    """What tracing sees: the operators' fake implementations return the shapes and types of the real ones."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    import mixedgemm_b200.linear  # noqa: F401
+    ops = torch.ops.mixedgemm_b200
+    with FakeTensorMode():
+        x, w = torch.empty(7, 64, dtype=torch.float16), torch.empty(64, dtype=torch.float16)
+        q, s = torch.empty(40, 64, dtype=torch.int8), torch.empty(40)
+        y = ops.int8_linear(x, q, s, None)
+        assert y.shape == (7, 40) and y.dtype == torch.float16
+        y, u = ops.int8_norm_linear(x, x, w, 1e-6, q, s, None)
+        assert y.shape == (7, 40) and u.shape == (7, 64) and u.dtype == torch.float16
+        assert ops.int8_norm_linear(x, None, w, 1e-6, q, s, None)[1].shape == (1,)
+        x, w = x.bfloat16(), w.bfloat16()
+        parts = [torch.empty(256, n, dtype=torch.uint8) for n in (16, 8, 8)] + [torch.empty(4096, dtype=torch.uint8)] * 3
+        idx = torch.empty(64, dtype=torch.int16)
+        y, u = ops.mixed_norm_linear(x, x, w, 1e-6, idx, [32, 16, 16], parts, [])
+        assert y.shape == (7, 256) and y.dtype == torch.bfloat16 and u.shape == (7, 64)
+        a, b, u = ops.mixed_norm_linear(torch.empty(200, 64, dtype=torch.bfloat16), None, w, 1e-6, idx, [32, 16, 16], parts * 2, parts)
+        assert a.shape == b.shape == (200, 256) and u.shape == (1,)
+
+
+@pytest.mark.parametrize("state", [dict(version=2), dict()])
+def test_int8_container_refuses_unknown_versions(state):
+    from mixedgemm_b200.linear import Int8Weights
+    with pytest.raises(RuntimeError, match="version"):
+        Int8Weights.from_state(dict(codes=torch.zeros(2, 32, dtype=torch.int8), scale=torch.ones(2), **state), "cpu")
+
+
+def test_int8_container_round_trip_on_the_cpu(tmp_path):
+    """The file holds dense codes; loading pads the rows to 16 bytes again."""
+    from mixedgemm_b200.linear import Int8Weights
+    q = torch.arange(3 * 37, dtype=torch.int8).view(3, 37)
+    w = Int8Weights(q, torch.tensor([1.0, 2.0, 3.0]))
+    w.save(str(tmp_path / "w.pt"))
+    back = Int8Weights.load(str(tmp_path / "w.pt"), "cpu")
+    assert torch.equal(back.codes, q) and torch.equal(back.scale, w.scale) and back.codes.stride() == (48, 1)
+    assert (back.out_features, back.in_features) == (3, 37)
+    a, b = Int8Weights(q.clone(), w.scale.clone()), Int8Weights(q.clone() + 1, w.scale * 2)
+    whole = Int8Weights.cat([a, b])
+    assert torch.equal(whole.codes, torch.cat([q, q + 1])) and torch.equal(b.scale, w.scale * 2)
+    assert b.codes.data_ptr() == whole.codes[3:].data_ptr()
+    with pytest.raises(ValueError):
+        Int8Weights.cat([a, Int8Weights(q[:, :20].contiguous(), w.scale)])
