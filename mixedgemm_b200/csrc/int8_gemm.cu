@@ -441,12 +441,15 @@ struct PairCfg {
   static constexpr uint32_t W_BYTES = 128 * 128;
   static constexpr uint32_t T_BYTES = BT / 2 * 128;
   static constexpr uint32_t STAGE_BYTES = W_BYTES + T_BYTES;
-  static constexpr uint32_t SCALE_BYTES = 4 * BT * 4;  // the tile's token scales, once per epilogue warp
+  // Eight epilogue warps, two to a quadrant of the tensor-memory lanes, each with half of the tokens: with
+  // four, a tile of 256 x 256 took 4.7 us to store, longer than its products up to K = 2000.
+  static constexpr int EPILOGUE = 8, COLS = BT / 2, THREADS = (2 + EPILOGUE) * 32;
+  static constexpr uint32_t SCALE_BYTES = EPILOGUE * COLS * 4;  // each warp's token scales
   static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + SCALE_BYTES + 256;
 };
 
 template <int BT, typename T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BT>::THREADS, 1)
 int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT) {
   using C = PairCfg<BT>;
   extern __shared__ uint8_t smem_raw[];
@@ -473,7 +476,7 @@ int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tm
     }
     for (int a = 0; a < 2; ++a) {
       ptx::mbar_init(tfull_bar(a), 1);
-      ptx::mbar_init(tempty_bar(a), 8);  // four epilogue warps in each CTA (used in the leader only)
+      ptx::mbar_init(tempty_bar(a), 2 * C::EPILOGUE);  // the epilogue warps of both CTAs (used in the leader only)
     }
     *stop = 0;
     ptx::fence_mbar_init();
@@ -559,20 +562,26 @@ int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tm
     }
   } else {
     const int quad = warp & 3;  // tensor-memory lanes this warp may read
-    const uint32_t my_scales = scales + (uint32_t)(warp - 2) * (BT * 4);
+    const int c0 = ((warp - 2) >> 2) * C::COLS;  // this warp's tokens of the tile
+    const uint32_t my_scales = scales + (uint32_t)(warp - 2) * (C::COLS * 4);
     float* g_scales = reinterpret_cast<float*>(gbase + (my_scales - base));
     for (int i = 0; i < count; ++i) {
       int n0, m0;
       locate(i, n0, m0);
+      m0 += c0;
       const int acc = i & 1;
       const Channel<T> chan(p, n0 + quad * 32 + lane, m0);
-      stage_scales<BT>(g_scales, p, m0, lane);
+      stage_scales<C::COLS>(g_scales, p, m0, lane);
       const bool store = wait_parity(tfull_bar(acc), ((uint32_t)i >> 1) & 1u, stop, p.status, p.wait_cycles, 8) &&
                          chan.real && !*stop;
       __syncwarp();
       ptx::tc_fence_after();
-      const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)acc * BT;
-      const int left = min(p.M - m0, BT);
+      const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BT + c0);
+      const int left = min(p.M - m0, C::COLS);
+      if (left <= 0) {  // none of this warp's tokens is real
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_cta(tempty_bar(acc), 0));
+      }
 #pragma unroll 1
       for (int c = 0; c < left; c += 64) {
         uint32_t r[2][32];
@@ -582,7 +591,7 @@ int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tm
         if (c + 64 >= left) {  // the accumulator is in registers: hand it back
           ptx::tc_fence_before();
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive_release_cluster(ptx::map_to_cta(tempty_bar(acc), 0));
+          if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_cta(tempty_bar(acc), 0));
         }
         if (store) {
           finish<32>(reinterpret_cast<const int*>(r[0]), my_scales, c, left - c, chan, p.ldd);
@@ -617,7 +626,7 @@ int launch_pair(const Int8Params& p, const CUtensorMap& w, const CUtensorMap& t,
   const int sms = di.sm_count;
   const int tiles = ((p.N + 255) / 256) * ((p.M + BT - 1) / BT);
   const int clusters = tiles < sms / 2 ? tiles : sms / 2;
-  MG_CUDA_TRY(mg::launch_kernel(kern, dim3(clusters * 2), dim3(kThreads), C::SMEM, st, p, w, t));
+  MG_CUDA_TRY(mg::launch_kernel(kern, dim3(clusters * 2), dim3(C::THREADS), C::SMEM, st, p, w, t));
   return MG_OK;
 }
 
