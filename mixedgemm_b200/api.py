@@ -235,6 +235,9 @@ def matmul(AN, BN, AS, BS, AO, BO, SFAN, SFBN, SFAS, SFBS, SFAO, SFBO, out=None,
     """bindings.cpp:9-67: returns a new [M,N] bfloat16 tensor = A @ B^T over the three segments.
     `out` (optional) receives the result instead; `C` (optional, bf16 [M,N]) is added before
     the single final rounding; `out_dtype=torch.float32` returns the unrounded accumulator."""
+    ops = _ops(required=False)
+    if ops is not None:  # the same checks and the same call, compiled
+        return ops.matmul(AN, BN, AS, BS, AO, BO, SFAN, SFBN, SFAS, SFBS, SFAO, SFBO, out, C, out_dtype, _workspace)
     lib = _capi.load()
     M, N, KN, KS, KO = _check_operands((AN, AS, AO, SFAN, SFAS, SFAO), (BN, BS, BO, SFBN, SFBS, SFBO), "matmul")
     dev = AN.device
@@ -402,24 +405,28 @@ def matmul_multi(problems, flags=None):
 
 # ----------------------------------------------------------------- 8-bit integers and fused norms
 
-_ops_module = None
+_ops_module = None  # False: looked for and not there
 
 
-def _ops():
-    """The compiled torch module of the operators below (csrc/int8_bindings.cpp): checks, allocation and
+def _ops(required=True):
+    """The compiled torch module of the operators below (csrc/ops_bindings.cpp): checks, allocation and
     launch in one call, because at one token the same steps in Python take longer than the kernels."""
     global _ops_module
     if _ops_module is None:
         import importlib.util
         from . import build
         path = build.ext_path("mixedgemm_ops")
-        if not os.path.exists(path):
-            raise ImportError("mixedgemm_ops is not built; run `python -m mixedgemm_b200.build --ext`.  "
-                              "There is no fallback path.")
-        spec = importlib.util.spec_from_file_location("mixedgemm_ops", path)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
-        _ops_module = module
+        _ops_module = False
+        if os.path.exists(path):
+            spec = importlib.util.spec_from_file_location("mixedgemm_ops", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            _ops_module = module
+    if _ops_module is False:
+        if not required:
+            return None
+        raise ImportError("mixedgemm_ops is not built; run `python -m mixedgemm_b200.build --ext`.  "
+                          "There is no fallback path.")
     return _ops_module
 
 

@@ -59,7 +59,7 @@ def build_lib(force=False, verbose=False):
 
 
 # torch modules under ext/ and the file each is made of
-EXT_SOURCES = {"mixedgemm": "bindings.cpp", "mixedgemm_ops": "int8_bindings.cpp"}
+EXT_SOURCES = {"mixedgemm": "bindings.cpp", "mixedgemm_ops": "ops_bindings.cpp"}
 
 
 def ext_path(name="mixedgemm"):

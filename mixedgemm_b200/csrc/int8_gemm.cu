@@ -12,7 +12,7 @@
 //   warp 0      producer: one 128-byte slice of K per stage for both operands (tiled tensor maps,
 //               128-byte swizzle)
 //   warp 1      MMA issuer: four K = 32 instructions per stage; owns the tensor memory
-//   warps 2-5   epilogue
+//   warps 2-    epilogue: four or eight
 //
 // All waits are bounded (see mg_wait.cuh); a kernel that gives up stores nothing.
 #include <cuda_bf16.h>
@@ -33,7 +33,6 @@ using mg::wait_parity;
 using mg::wait_parity_cluster;
 
 constexpr int kRows = 128;      // channels of a CTA's tile
-constexpr int kThreads = 192;
 constexpr int kMaxSplit = 8;
 
 struct Int8Params {
@@ -148,14 +147,16 @@ struct SmallCfg {
   static constexpr uint32_t STAGE_BYTES = W_BYTES + T_BYTES;
   // sums received from the other CTAs: this CTA's BT / splits columns from splits - 1 senders
   static constexpr uint32_t recv_bytes(int splits) { return (uint32_t)(splits - 1) * kRows * (BT / splits) * 4; }
-  static constexpr uint32_t SCALE_BYTES = 4 * BT * 4;  // the tile's token scales, once per epilogue warp
+  // one epilogue warp to a quadrant of the tensor-memory lanes, two from 64 tokens on (half of them each)
+  static constexpr int SIDE = BT >= 64 ? 2 : 1, EPILOGUE = 4 * SIDE, COLS = BT / SIDE, THREADS = (2 + EPILOGUE) * 32;
+  static constexpr uint32_t SCALE_BYTES = 4 * BT * 4;  // the tile's token scales, once per quadrant
   static constexpr size_t smem(int splits) {
     return 1024 + (size_t)STAGES * STAGE_BYTES + 256 + SCALE_BYTES + recv_bytes(splits);
   }
 };
 
 template <int BT, typename T>
-__global__ void __launch_bounds__(kThreads) int8_gemm_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tmW,
+__global__ void __launch_bounds__(SmallCfg<BT>::THREADS) int8_gemm_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tmW,
                                                              const __grid_constant__ CUtensorMap tmT) {
   using C = SmallCfg<BT>;
   extern __shared__ uint8_t smem_raw[];
@@ -201,6 +202,7 @@ __global__ void __launch_bounds__(kThreads) int8_gemm_kernel(const Int8Params p,
   const int n0 = blockIdx.x * kRows, m0 = blockIdx.y * BT;
   const int quad = warp & 3, row = quad * 32 + lane;  // an epilogue warp's tensor-memory lanes = channels of the tile
   const Channel<T> chan(p, warp >= 2 ? n0 + row : p.N, m0);
+  const int side = (warp - 2) >> 2;  // an epilogue warp's share of the tokens
   const uint32_t my_scales = scales + (uint32_t)((warp - 2) & 3) * (BT * 4);
   const int left = p.M - m0;     // tokens of this tile and beyond
   const int cols = BT / splits;  // columns this CTA finishes
@@ -246,13 +248,13 @@ __global__ void __launch_bounds__(kThreads) int8_gemm_kernel(const Int8Params p,
     if (leader && live) ptx::tc_commit(done_bar);
   } else {
     const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16);
-    stage_scales<BT>(reinterpret_cast<float*>(gbase + (my_scales - base)), p, m0, lane);
+    stage_scales<BT>(reinterpret_cast<float*>(gbase + (my_scales - base)), p, m0, lane);  // (the same values from either side)
     const bool store = wait_parity(done_bar, 0, stop, p.status, p.wait_cycles, 8) && chan.real && !*stop;
     __syncwarp();
     ptx::tc_fence_after();
     if (splits == 1) {
 #pragma unroll 1
-      for (int c = 0; c < BT && c < left; c += 32) {
+      for (int c = side * C::COLS; c < (side + 1) * C::COLS && c < left; c += 32) {
         uint32_t r[32];
         ptx::tmem_ld_32x32(taddr + c, r);
         ptx::tmem_ld_wait();
@@ -263,7 +265,7 @@ __global__ void __launch_bounds__(kThreads) int8_gemm_kernel(const Int8Params p,
       // theirs, 16 bytes (four columns of a channel) at a time.
       ptx::cluster_wait();  // every CTA of the cluster runs
 #pragma unroll 1
-      for (int c = 0; c < BT && c < left; c += 32) {
+      for (int c = side * C::COLS; c < (side + 1) * C::COLS && c < left; c += 32) {
         uint32_t r[32];
         ptx::tmem_ld_32x32(taddr + c, r);
         ptx::tmem_ld_wait();
@@ -292,7 +294,7 @@ __global__ void __launch_bounds__(kThreads) int8_gemm_kernel(const Int8Params p,
     if (warp >= 2 && !*stop) {
       const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16);
       const int first = rank * cols;
-      for (int c = 0; c < cols && first + c < left; c += 4) {
+      for (int c = side * 4; c < cols && first + c < left; c += 4 * C::SIDE) {
         uint32_t r[4];
         ptx::tmem_ld_32x4(taddr + first + c, r);
         ptx::tmem_ld_wait();
@@ -640,7 +642,7 @@ int launch_small(const Int8Params& p, const CUtensorMap& w, const CUtensorMap& t
   MG_CUDA_TRY(mg::allow_smem(kern, C::smem(kMaxSplit), di.device, allowed));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((p.N + kRows - 1) / kRows, (p.M + BT - 1) / BT, splits);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -670,7 +672,7 @@ int small_capacity(int splits, const mg::DeviceInfo& di) {
     int n = 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(1, 1, splits);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(C::THREADS);
     cfg.dynamicSmemBytes = C::smem(splits);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -690,20 +692,20 @@ int small_capacity(int splits, const mg::DeviceInfo& di) {
 
 // Which form takes the problem: the one with the least of
 //   T = fixed + wave * waves + sqrt(compute^2 + bytes^2)   in us,
-// compute = waves * K stages of a CTA * stage, bytes = those of the operands and the result / 7.2 MB per us,
-// waves = tiles / (clusters that run at one time).  The constants are fitted to 117 problems (M = 1 ... 2048,
-// N and K = 1024, 4096, 14336, bf16 results, cold weights) run with every form: over them the choice is
-// 1 % slower than the best form on average and 14 % at most.  What they say: a stage of the pair form runs at
+// compute = waves * K stages of a CTA * stage, bytes = those of the operands and the result / 7.1 MB per us,
+// waves = tiles / (clusters that run at one time).  The constants are fitted to 117 problems (8 to 2048
+// tokens, N and K = 1024, 4096, 14336, bf16 results, cold weights) run with every form: over them the choice is
+// 1 % slower than the best form on average and 15 % at most.  What they say: a stage of the pair form runs at
 // the tensor cores' rate (0.28 us for 256 x 256 x 128), one of the small form at the rate of its loads; a
-// pair costs a microsecond more to set up; adding sums across a cluster costs 1.6 us.  For example
-// 2048 x 4096 x 4096: pair 256 25.3 us, pair 128 26.9, small 128 41.0; 64 x 4096 x 4096: small 64 with
-// four splits 7.8, one split 9.3, pair 128 9.1; 1 x 4096 x 4096: small 32 with four splits 6.6, one 8.4.
+// pair costs two microseconds more to set up, the small form a launch's worth for every further wave; adding
+// sums across a cluster costs 1.7 us.  For example 2048 x 4096 x 4096: pair 256 25 us, pair 128 27, small 128
+// 40; 64 x 4096 x 4096: small 64 with four splits 7.8, one split 8.9, pair 128 9.1.
 struct FormCost {
   double fixed, wave, stage;
 };
-constexpr FormCost kPair256 = {3.1, 1.8, 0.281}, kPair128 = {2.75, 1.4, 0.155};
-constexpr FormCost kSmall32 = {-1.2, 3.5, 0.183}, kSmall64 = {-0.9, 3.7, 0.188}, kSmall128 = {-0.5, 4.1, 0.224};
-constexpr double kSplitCost = 1.6, kBytesPerUs = 7.2e6;
+constexpr FormCost kPair256 = {3.8, 0.55, 0.290}, kPair128 = {2.95, 0.55, 0.163};
+constexpr FormCost kSmall32 = {-1.0, 3.3, 0.179}, kSmall64 = {-1.15, 3.75, 0.184}, kSmall128 = {-0.4, 3.75, 0.215};
+constexpr double kSplitCost = 1.67, kBytesPerUs = 7.1e6;
 
 struct Form {
   bool pair;

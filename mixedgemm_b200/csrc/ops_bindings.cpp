@@ -1,7 +1,8 @@
-// pybind11 / libtorch module `mixedgemm_ops`: the 8-bit operators and the fused norms for torch tensors
-// (mixedgemm_b200/api.py documents and re-exports them).  Checks, allocation and launch in one compiled
-// call: at one token the kernels take 2 to 7 us, and the same steps in Python took 9 (quantize_int8),
-// 10 (matmul_int8), 14 (rms_norm_int8) and 31 us (rms_norm_reorder_quantize_x) of host time.
+// pybind11 / libtorch module `mixedgemm_ops`: the 8-bit operators and the fused norms for torch tensors, and
+// the mixed product that follows the norm (mixedgemm_b200/api.py documents and re-exports them).  Checks,
+// allocation and launch in one compiled call: at one token the kernels take 2 to 9 us, and the same steps in
+// Python took 9 (quantize_int8), 10 (matmul_int8), 14 (rms_norm_int8), 24 (matmul) and 31 us
+// (rms_norm_reorder_quantize_x) of host time.
 //
 // torch owns the memory and names the current stream; all work goes through the C ABI (mixedgemm_c.h).
 // Nothing is kept from one call to the next.  Inputs that a call does not take raise RuntimeError
@@ -230,6 +231,63 @@ py::tuple rms_norm_reorder_quantize_x(const Tensor& X, const Tensor& weight, con
   return py::make_tuple(o[0], o[1], o[2], o[3], o[4], o[5], n.stream);
 }
 
+// The mixed product over the tensors of the two quantisers, in the order of the reference's binding.
+// `workspace(device, bytes)` hands out scratch as (address, bytes); it is asked only when scratch is needed.
+Tensor matmul(const Tensor& AN, const Tensor& BN, const Tensor& AS, const Tensor& BS, const Tensor& AO, const Tensor& BO,
+              const Tensor& SFAN, const Tensor& SFBN, const Tensor& SFAS, const Tensor& SFBS, const Tensor& SFAO,
+              const Tensor& SFBO, const optional<Tensor>& out, const optional<Tensor>& C,
+              const optional<ScalarType>& out_dtype, const py::function& workspace) {
+  const char* what = "matmul";
+  const Tensor* codes[6] = {&AN, &BN, &AS, &BS, &AO, &BO};
+  const Tensor* scales[6] = {&SFAN, &SFBN, &SFAS, &SFBS, &SFAO, &SFBO};
+  const at::Device dev = AN.device();
+  size_t pitches[6];
+  for (int i = 0; i < 6; ++i) {
+    const Tensor& t = *codes[i];
+    TORCH_CHECK(t.is_cuda() && t.scalar_type() == ScalarType::Byte && t.dim() == 2 && (t.size(1) == 0 || t.stride(1) == 1), what,
+                ": code tensors must be 2-D CUDA uint8 with unit column stride");
+    TORCH_CHECK(t.size(0) == codes[i & 1]->size(0), what, ": the three code tensors of an operand must have the same row count");
+    pitches[i] = t.size(1) ? (size_t)t.stride(0) : 0;
+  }
+  const int M = as_int(AN.size(0), what), N = as_int(BN.size(0), what);
+  const int KN = as_int(AN.size(1) * 2, what), KS = as_int(AS.size(1) * 4 / 3, what), KO = as_int(AO.size(1), what);
+  TORCH_CHECK(AS.size(1) * 4 == (int64_t)KS * 3 && BN.size(1) * 2 == KN && BS.size(1) * 2 == KS && BO.size(1) * 2 == KO, what,
+              ": code widths of the two operands do not describe the same K split");
+  const int k[3] = {KN, KS, KO};
+  for (int i = 0; i < 6; ++i) {
+    const Tensor& t = *scales[i];
+    TORCH_CHECK(t.is_cuda() && t.scalar_type() == ScalarType::Byte && t.is_contiguous(), what,
+                ": scale tensors must be contiguous CUDA uint8 tensors");
+    const size_t need = mg_sf_bytes(i & 1 ? N : M, k[i >> 1]);
+    TORCH_CHECK((size_t)t.numel() >= need, what, ": a scale tensor holds ", t.numel(), " bytes, ", need,
+                " are read (whole 512-byte atoms)");
+    TORCH_CHECK(t.device() == dev && codes[i]->device() == dev, what, ": all operands must be on one device");
+  }
+  const ScalarType type = out ? out->scalar_type() : out_dtype ? *out_dtype : ScalarType::BFloat16;
+  TORCH_CHECK(type == ScalarType::BFloat16 || type == ScalarType::Float, what, ": output dtype must be bfloat16 or float32");
+  const Tensor D = out ? *out : new_rows(M, N, N, type, dev);
+  TORCH_CHECK(D.dim() == 2 && D.size(0) == M && D.size(1) == N && D.stride(1) == 1 && D.device() == dev, what,
+              ": out must be [M,N] on the operands' device with unit column stride");
+  TORCH_CHECK(!C || (C->scalar_type() == ScalarType::BFloat16 && C->dim() == 2 && C->size(0) == M && C->size(1) == N &&
+                     C->device() == dev && C->stride(1) == 1 && C->stride(0) == D.stride(0)),
+              what, ": C must be bf16 [M,N] on the operands' device with out's row pitch");
+  const c10::cuda::CUDAGuard guard(dev);
+  const size_t need = mg_matmul_pitched_workspace_bytes(M, N, KN, KS, KO, pitches);
+  void* ws = nullptr;
+  size_t ws_bytes = 0;
+  if (need) {
+    const py::tuple got = workspace(dev, need);
+    ws = reinterpret_cast<void*>(got[0].cast<uintptr_t>());
+    ws_bytes = got[1].cast<size_t>();
+  }
+  check(mg_matmul_pitched(bytes(AN), bytes(BN), bytes(AS), bytes(BS), bytes(AO), bytes(BO), pitches, type == ScalarType::Float, M, N,
+                          KN, KS, KO, C ? C->data_ptr() : nullptr, D.numel() ? D.data_ptr() : nullptr, as_int(D.stride(0), what),
+                          bytes(SFAN), bytes(SFBN), bytes(SFAS), bytes(SFBS), bytes(SFAO), bytes(SFBO), ws, ws_bytes,
+                          stream_of(dev)),
+        what);
+  return D;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -241,4 +299,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rms_norm_reorder_quantize_x", &rms_norm_reorder_quantize_x, py::arg("X"), py::arg("weight"), py::arg("reorder_index"),
         py::arg("KN"), py::arg("KS"), py::arg("KO"), py::arg("eps"), py::arg("residual") = py::none(),
         py::arg("residual_out") = py::none(), py::arg("out") = py::none());
+  m.def("matmul", &matmul);
 }

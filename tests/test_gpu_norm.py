@@ -270,3 +270,33 @@ def test_a_block_of_both_kinds_in_a_graph():
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(out, want2))
     assert mg.device_status() == 0
+
+
+def test_product_with_and_without_the_compiled_module(monkeypatch):
+    """api.matmul through mixedgemm_ops and through ctypes: the same bytes, the same refusals."""
+    import mixedgemm_b200 as mg
+    from mixedgemm_b200 import api
+    for M, N, split in ((9, 256, (128, 64, 64)), (300, 512, (2560, 1408, 128)), (40, 128, (256, 0, 128))):
+        K = sum(split)
+        idx = torch.randperm(K, generator=gen(1)).to(torch.int16).cuda()
+        A = mg.reorder_quantize_x(H.make_x(M, K, seed=2).cuda(), idx, *split)
+        for padded in (True, False):  # (dense buffers of 64-tails need the workspace)
+            B = mg.reorder_quantize_w(H.make_w(N, K).cuda(), idx, *split, out=api.alloc_quantized_w(N, *split, "cuda", padded=padded))
+            ops = [t for pair in zip(A, B) for t in pair]
+            C = torch.randn(M, N, generator=gen(3)).to(torch.bfloat16).cuda()
+            calls = [dict(), dict(out_dtype=torch.float32), dict(C=C), dict(out=torch.empty(M, N, device="cuda"))]
+            bad = [dict(out_dtype=torch.float16), dict(C=C.float()), dict(C=C[:, :-8]), dict(out=torch.empty(M, N + 8, dtype=torch.bfloat16, device="cuda"))]
+            got = [mg.matmul(*ops, **kw).clone() for kw in calls]
+            broken = [ops[:6] + [t[:100] for t in ops[6:]], [ops[0].cpu()] + ops[1:], ops[:2] + [ops[2][:, :-3] if split[1] else ops[2][1:]] + ops[3:], [ops[0][1:]] + ops[1:]]
+            for module in (api._ops(), False):
+                monkeypatch.setattr(api, "_ops_module", module)
+                for kw in bad:
+                    with pytest.raises(RuntimeError):
+                        mg.matmul(*ops, **kw)
+                for args in broken:
+                    with pytest.raises(RuntimeError):
+                        mg.matmul(*args)
+            want = [mg.matmul(*ops, **kw) for kw in calls]  # ctypes
+            monkeypatch.undo()
+            assert all(a.dtype == b.dtype and torch.equal(a, b) for a, b in zip(got, want))
+    assert mg.device_status() == 0
