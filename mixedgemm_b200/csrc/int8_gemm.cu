@@ -432,14 +432,15 @@ int launch_few(const Int8Params& p, const int8_t* A, size_t lda, const int8_t* B
 }
 
 // ---------------------------------------------------------------- CTA-pair form
-// Two CTAs of a cluster compute 256 channels x BT tokens with tcgen05.mma.cta_group::2: each stages
+// Two CTAs of a cluster compute 256 channels x 256 tokens with tcgen05.mma.cta_group::2: each stages
 // its own 128 channels and half of the tokens, and one instruction of the leader drives both tensor
 // cores.  The loads of both CTAs are counted on the leader's barrier.  Two accumulators alternate, so
 // the epilogue of a tile runs under the products of the next.  Persistent: cluster c takes tiles
-// c, c + clusters, ...
-template <int BT>
+// c, c + clusters, ... for as many whole rounds as there are; the tiles that are left over (4 of the 448 of
+// 2048 x 14336 on 74 clusters would take a round of their own) are cut into two or four parts of 128 or 64
+// tokens, as long as every cluster gets at most one.
 struct PairCfg {
-  static constexpr int STAGES = BT == 256 ? 6 : 8;
+  static constexpr int BT = 256, STAGES = 6;
   static constexpr uint32_t W_BYTES = 128 * 128;
   static constexpr uint32_t T_BYTES = BT / 2 * 128;
   static constexpr uint32_t STAGE_BYTES = W_BYTES + T_BYTES;
@@ -450,10 +451,13 @@ struct PairCfg {
   static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + SCALE_BYTES + 256;
 };
 
-template <int BT, typename T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BT>::THREADS, 1)
-int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT) {
-  using C = PairCfg<BT>;
+// rounds: whole rounds of tiles;  cut: parts of a tile that is left over (1, 2, 4), tmPart: their load of tokens
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
+int8_gemm_pair_kernel(const Int8Params p, int rounds, int cut, const __grid_constant__ CUtensorMap tmW,
+                      const __grid_constant__ CUtensorMap tmT, const __grid_constant__ CUtensorMap tmPart) {
+  using C = PairCfg;
+  constexpr int BT = C::BT;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = ptx::smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -499,13 +503,21 @@ int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tm
 
   const int tiles_n = (p.N + 255) / 256, tiles_m = (p.M + BT - 1) / BT;
   const int first = (int)ptx::cluster_id_x(), step = (int)ptx::nclusters_x();
-  const int count = (tiles_n * tiles_m - first + step - 1) / step;
-  auto locate = [&](int i, int& n0, int& m0) {
+  // item i of this cluster: its first channel and token, and how many tokens it has
+  auto locate = [&](int i, int& n0, int& m0, int& width) {
+    const bool whole = i < rounds;
     int m_tile, n_tile;
-    raster(first + i * step, tiles_m, tiles_n, m_tile, n_tile);
+    raster(whole ? first + i * step : rounds * step + first / cut, tiles_m, tiles_n, m_tile, n_tile);
+    width = whole ? BT : BT / cut;
     n0 = n_tile * 256 + (int)rank * 128;
-    m0 = m_tile * BT;
+    m0 = m_tile * BT + (whole ? 0 : first % cut * width);
   };
+  int count = rounds;
+  if (rounds * step + first / cut < tiles_n * tiles_m) {
+    int n0, m0, width;
+    locate(rounds, n0, m0, width);
+    if (m0 < p.M) ++count;  // (a part may lie wholly beyond the last token)
+  }
 
   if (warp == 0) {
     const bool leader = ptx::elect_one();
@@ -514,18 +526,20 @@ int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tm
     bool live = true;
     int skip = blockIdx.x == 0 ? p.skip_load : 0;
     for (int i = 0; i < count && live; ++i) {
-      int n0, m0;
-      locate(i, n0, m0);
-      m0 += (int)rank * (BT / 2);
+      int n0, m0, width;
+      locate(i, n0, m0, width);
+      m0 += (int)rank * (width / 2);
+      const CUtensorMap* tokens = width == BT ? &tmT : &tmPart;
+      const uint32_t tx = 2 * (C::W_BYTES + (uint32_t)width / 2 * 128);
 #pragma unroll 1
       for (int s = 0; s < p.stages; ++s) {
         if (!wait_parity(empty_bar(slot), phase ^ 1u, stop, p.status, p.wait_cycles, 1)) { live = false; break; }
         if (leader && !(skip > 0 && --skip == 0)) {
           const uint32_t sbase = base + slot * C::STAGE_BYTES;
           const uint32_t fb = ptx::map_to_cta(full_bar(slot), 0);
-          if (rank == 0) ptx::mbar_expect_tx(full_bar(slot), 2 * C::STAGE_BYTES);
+          if (rank == 0) ptx::mbar_expect_tx(full_bar(slot), tx);
           ptx::tma_load_2d_pair(sbase, &tmW, s * 128, n0, fb);
-          ptx::tma_load_2d_pair(sbase + C::W_BYTES, &tmT, s * 128, m0, fb);
+          ptx::tma_load_2d_pair(sbase + C::W_BYTES, tokens, s * 128, m0, fb);
         }
         if (++slot == C::STAGES) { slot = 0; phase ^= 1u; }
       }
@@ -533,7 +547,6 @@ int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tm
   } else if (warp == 1) {
     if (rank == 0) {
       const bool leader = ptx::elect_one();
-      constexpr uint32_t kIdesc = kIdescI8<256, BT>;
       int slot = 0;
       uint32_t phase = 0;
       bool live = true;
@@ -542,6 +555,7 @@ int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tm
         if (!wait_parity_cluster(tempty_bar(acc), (((uint32_t)i >> 1) & 1u) ^ 1u, stop, p.status, p.wait_cycles, 4)) break;
         ptx::tc_fence_after();
         const uint32_t d = tmem + (uint32_t)acc * BT;
+        const uint32_t idesc = i < rounds ? kIdescI8<256, BT> : cut == 1 ? kIdescI8<256, BT> : cut == 2 ? kIdescI8<256, BT / 2> : kIdescI8<256, BT / 4>;
         uint32_t accumulate = 0;
 #pragma unroll 1
         for (int s = 0; s < p.stages; ++s) {
@@ -552,7 +566,7 @@ int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tm
           if (leader) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              ptx::mma_i8_pair(d, w_lo + j * 2, t_lo + j * 2, ptx::kDescHiSw128, kIdesc, accumulate);
+              ptx::mma_i8_pair(d, w_lo + j * 2, t_lo + j * 2, ptx::kDescHiSw128, idesc, accumulate);
               accumulate = 1;
             }
             ptx::tc_commit_pair(empty_bar(slot), 3);  // frees the stage in both CTAs
@@ -564,12 +578,12 @@ int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tm
     }
   } else {
     const int quad = warp & 3;  // tensor-memory lanes this warp may read
-    const int c0 = ((warp - 2) >> 2) * C::COLS;  // this warp's tokens of the tile
     const uint32_t my_scales = scales + (uint32_t)(warp - 2) * (C::COLS * 4);
     float* g_scales = reinterpret_cast<float*>(gbase + (my_scales - base));
     for (int i = 0; i < count; ++i) {
-      int n0, m0;
-      locate(i, n0, m0);
+      int n0, m0, width;
+      locate(i, n0, m0, width);
+      const int c0 = ((warp - 2) >> 2) * (width / 2);  // this warp's tokens of the tile
       m0 += c0;
       const int acc = i & 1;
       const Channel<T> chan(p, n0 + quad * 32 + lane, m0);
@@ -579,7 +593,7 @@ int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tm
       __syncwarp();
       ptx::tc_fence_after();
       const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BT + c0);
-      const int left = min(p.M - m0, C::COLS);
+      const int left = min(p.M - m0, width / 2);
       if (left <= 0) {  // none of this warp's tokens is real
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_cta(tempty_bar(acc), 0));
@@ -619,16 +633,32 @@ int8_gemm_pair_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tm
   if (warp == 1) ptx::tmem_dealloc_pair(tmem, 2 * BT);
 }
 
-template <int BT, typename T>
-int launch_pair(const Int8Params& p, const CUtensorMap& w, const CUtensorMap& t, const mg::DeviceInfo& di, cudaStream_t st) {
-  using C = PairCfg<BT>;
-  auto kern = int8_gemm_pair_kernel<BT, T>;
+// How the tiles of a problem are dealt out to `most` clusters.
+struct PairPlan {
+  int clusters, rounds, cut;
+};
+PairPlan plan_pair(double tiles, int most) {
+  PairPlan pl;
+  pl.rounds = (int)(tiles / most);
+  const int rest = (int)(tiles - (double)pl.rounds * most);
+  pl.cut = rest == 0 || rest * 2 > most ? 1 : rest * 4 > most ? 2 : 4;
+  pl.clusters = pl.rounds > 0 ? most : rest * pl.cut;
+  return pl;
+}
+
+template <typename T>
+int launch_pair(const Int8Params& p, const int8_t* A, size_t lda, int K, const CUtensorMap& w, const mg::DeviceInfo& di,
+                cudaStream_t st) {
+  using C = PairCfg;
+  auto kern = int8_gemm_pair_kernel<T>;
   static std::atomic<unsigned long long> allowed;
   MG_CUDA_TRY(mg::allow_smem(kern, C::SMEM, di.device, allowed));
-  const int sms = di.sm_count;
-  const int tiles = ((p.N + 255) / 256) * ((p.M + BT - 1) / BT);
-  const int clusters = tiles < sms / 2 ? tiles : sms / 2;
-  MG_CUDA_TRY(mg::launch_kernel(kern, dim3(clusters * 2), dim3(C::THREADS), C::SMEM, st, p, w, t));
+  const PairPlan pl = plan_pair(std::ceil(p.N / 256.0) * std::ceil(p.M / (double)C::BT), di.sm_count / 2);
+  CUtensorMap t, part;
+  int rc;
+  if ((rc = mg::make_map(&t, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, K, p.M, lda, 128, C::BT / 2))) return rc;
+  if ((rc = mg::make_map(&part, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, K, p.M, lda, 128, C::BT / 2 / pl.cut))) return rc;
+  MG_CUDA_TRY(mg::launch_kernel(kern, dim3(pl.clusters * 2), dim3(C::THREADS), C::SMEM, st, p, pl.rounds, pl.cut, w, t, part));
   return MG_OK;
 }
 
@@ -703,7 +733,8 @@ int small_capacity(int splits, const mg::DeviceInfo& di) {
 struct FormCost {
   double fixed, wave, stage;
 };
-constexpr FormCost kPair256 = {3.8, 0.55, 0.290}, kPair128 = {2.95, 0.55, 0.163};
+constexpr FormCost kPair = {3.8, 0.55, 0.290};
+constexpr double kPairCutStage[5] = {0, 0.290, 0.163, 0, 0.12};  // of a tile in one, two, four parts
 constexpr FormCost kSmall32 = {-1.0, 3.3, 0.179}, kSmall64 = {-1.15, 3.75, 0.184}, kSmall128 = {-0.4, 3.75, 0.215};
 constexpr double kSplitCost = 1.67, kBytesPerUs = 7.1e6;
 
@@ -717,7 +748,7 @@ Form choose_form(int M, int N, int K, const mg::DeviceInfo& di, const mg::Option
   const int sms = di.sm_count;
   const double stages = (K + 127) / 128;
   const double bytes = ((double)N * K + (double)M * K + (double)sizeof(T) * M * N) / kBytesPerUs;
-  Form best = {true, 256, 1};
+  Form best = {true, 0, 1};
   double least = 1e300;
   auto offer = [&](const Form& f, const FormCost& c, double tiles, int capacity, double extra) {
     const double waves = std::ceil(tiles / capacity), compute = waves * std::ceil(stages / f.splits) * c.stage;
@@ -729,8 +760,11 @@ Form choose_form(int M, int N, int K, const mg::DeviceInfo& di, const mg::Option
   };
   auto tiles = [&](int channels, int tokens) { return std::ceil((double)N / channels) * std::ceil((double)M / tokens); };
   if (opt.int8_pair != 0) {
-    if (opt.int8_pair != 128) offer({true, 256, 1}, kPair256, tiles(256, 256), sms / 2, 0);
-    if (opt.int8_pair <= 128) offer({true, 128, 1}, kPair128, tiles(256, 128), sms / 2, 0);
+    const double all = tiles(256, 256);
+    const PairPlan pl = plan_pair(all, sms / 2);
+    const bool rest = (double)pl.rounds * pl.clusters < all;
+    const double compute = stages * (pl.rounds * kPair.stage + (rest ? kPairCutStage[pl.cut] : 0));
+    least = kPair.fixed + (pl.rounds + rest) * kPair.wave + std::sqrt(compute * compute + bytes * bytes);
   }
   if (opt.int8_pair <= 0) {
     for (int splits = 1; splits <= kMaxSplit && splits <= stages; splits *= 2) {
@@ -760,8 +794,8 @@ int launch_int8(const Int8Params& p, const int8_t* A, size_t lda, const int8_t* 
   CUtensorMap w, t;
   int rc;
   if ((rc = mg::make_map(&w, CU_TENSOR_MAP_DATA_TYPE_UINT8, B, K, p.N, ldb, 128, 128))) return rc;
-  if ((rc = mg::make_map(&t, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, K, p.M, lda, 128, f.pair ? f.tokens / 2 : f.tokens))) return rc;
-  if (f.pair) return f.tokens == 128 ? launch_pair<128, T>(p, w, t, di, st) : launch_pair<256, T>(p, w, t, di, st);
+  if (f.pair) return launch_pair<T>(p, A, lda, K, w, di, st);
+  if ((rc = mg::make_map(&t, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, K, p.M, lda, 128, f.tokens))) return rc;
   if (f.tokens == 32) return launch_small<32, T>(p, w, t, f.splits, di, st);
   if (f.tokens == 64) return launch_small<64, T>(p, w, t, f.splits, di, st);
   return launch_small<128, T>(p, w, t, f.splits, di, st);

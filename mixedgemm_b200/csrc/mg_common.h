@@ -50,7 +50,7 @@ struct Options {
                         // after the wait limit and returns normally)
   int int8_tokens;      // INT8_TOKENS: 32 / 64 / 128 forces the token tile of the 8-bit product's small form
   int int8_few;         // INT8_FEW: 0 turns the form for one or two tokens off
-  int int8_pair;        // INT8_PAIR: 0 turns the CTA-pair form off, 128 / 256 forces it with that token tile
+  int int8_pair;        // INT8_PAIR: 0 / 1 forces the CTA-pair form of the 8-bit product off / on
   int int8_split;       // INT8_SPLIT: 1 / 2 / 4 / 8 forces how many CTAs of the small form share a tile's K
 };
 Options options();

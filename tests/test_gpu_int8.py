@@ -243,13 +243,15 @@ def test_product_of_every_tile_and_split(tile, split, mgopt):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("tile", [128, 256])
-def test_product_of_the_pair_form(tile, dtype, mgopt):
-    """One tile, many tiles to a pair (both accumulators, several turns), ragged edges, one slice of K."""
+def test_product_of_the_pair_form(dtype, mgopt):
+    """No whole round of tiles or several (both accumulators), and what is left over whole, in halves and in
+    quarters (74 pairs: 1, 9 and 6 = 80 - 74 tiles in quarters, 24 and 34 in halves, 40 whole, 74 nothing),
+    parts beyond the last token, ragged edges, one slice of K."""
     mgopt.set("INT8_FEW", 0)
-    mgopt.set("INT8_PAIR", tile)
-    for M, N, K in ((1, 1, 1), (200, 130, 1024), (140, 257, 1931), (513, 640, 128), (1000, 5000, 300), (2300, 3000, 128)):
-        run_product(M, N, K, dtype, with_bias=True, seed=tile)
+    mgopt.set("INT8_PAIR", 1)
+    for M, N, K in ((1, 1, 1), (60, 200, 70), (200, 130, 1024), (140, 257, 1931), (513, 640, 128), (1000, 5000, 300), (2300, 3000, 128),
+                    (700, 2000, 640), (1280, 2000, 1000), (500, 9472, 256), (4000, 4100, 256)):
+        run_product(M, N, K, dtype, with_bias=True, seed=M)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -272,9 +274,8 @@ def test_product_does_not_depend_on_tile_or_split(mgopt):
             mgopt.set("INT8_TOKENS", tile)
             mgopt.set("INT8_SPLIT", split)
             assert torch.equal(mg.matmul_int8(av, bv, sa, sb), ref)
-    for pair in (128, 256):
-        mgopt.set("INT8_PAIR", pair)
-        assert torch.equal(mg.matmul_int8(av, bv, sa, sb), ref)
+    mgopt.set("INT8_PAIR", 1)
+    assert torch.equal(mg.matmul_int8(av, bv, sa, sb), ref)
     few = mg.matmul_int8(av[:2], bv, sa[:2], sb)
     mgopt.set("INT8_FEW", 0)
     assert torch.equal(few, mg.matmul_int8(av[:2], bv, sa[:2], sb)) and torch.equal(few, ref[:2])
@@ -402,7 +403,7 @@ def test_norm_then_product_on_a_side_stream_and_in_two_graphs():
 # ------------------------------------------------------------------------------ where calls go wrong
 
 @pytest.mark.parametrize("opts, M", [(dict(INT8_PAIR=0, INT8_TOKENS=64, INT8_SPLIT=1), 40), (dict(INT8_PAIR=0, INT8_TOKENS=32, INT8_SPLIT=4), 20),
-                                     (dict(INT8_PAIR=256), 700)])
+                                     (dict(INT8_PAIR=1), 700)])
 def test_a_wait_that_runs_out_is_reported_and_the_context_survives(opts, M, mgopt):
     """Host-side fault injection: the first CTA withholds its second stage load.  With the wait limit at
     1 ms the kernel gives up, stores nothing of that tile and returns; the status word says so once."""
