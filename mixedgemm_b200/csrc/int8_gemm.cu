@@ -722,21 +722,22 @@ int small_capacity(int splits, const mg::DeviceInfo& di) {
 
 // Which form takes the problem: the one with the least of
 //   T = fixed + wave * waves + sqrt(compute^2 + bytes^2)   in us,
-// compute = waves * K stages of a CTA * stage, bytes = those of the operands and the result / 7.1 MB per us,
-// waves = tiles / (clusters that run at one time).  The constants are fitted to 117 problems (8 to 2048
-// tokens, N and K = 1024, 4096, 14336, bf16 results, cold weights) run with every form: over them the choice is
-// 1 % slower than the best form on average and 15 % at most.  What they say: a stage of the pair form runs at
-// the tensor cores' rate (0.28 us for 256 x 256 x 128), one of the small form at the rate of its loads; a
-// pair costs two microseconds more to set up, the small form a launch's worth for every further wave; adding
-// sums across a cluster costs 1.7 us.  For example 2048 x 4096 x 4096: pair 256 25 us, pair 128 27, small 128
-// 40; 64 x 4096 x 4096: small 64 with four splits 7.8, one split 8.9, pair 128 9.1.
+// compute = waves * K stages of a CTA * stage (a part of a tile in the pair form's last round: kCutStage),
+// bytes = those of the operands and the result / 7.3 MB per us, waves = tiles / (clusters that run at one time).
+// The constants are fitted to 117 problems (8 to 2048 tokens, N and K = 1024, 4096, 14336, bf16 results, cold
+// weights) run with every form: over them the choice is 0.3 % slower than the best form on average and 11 %
+// at most.  What they say: a stage of the pair form runs at the tensor cores' rate (0.28 us for
+// 256 x 256 x 128), one of the small form at the rate of its loads; a pair costs two microseconds more to set
+// up, the small form a launch's worth for every further wave; adding sums across a cluster costs 1.7 us.  For
+// example 2048 x 4096 x 4096: pair 25 us, small 128 40; 256 x 4096 x 4096: pair 10.8, small 64 9.3;
+// 64 x 4096 x 4096: small 64 with four splits 7.8, one split 8.9, pair 10.
 struct FormCost {
   double fixed, wave, stage;
 };
-constexpr FormCost kPair = {3.8, 0.55, 0.290};
-constexpr double kPairCutStage[5] = {0, 0.290, 0.163, 0, 0.12};  // of a tile in one, two, four parts
-constexpr FormCost kSmall32 = {-1.0, 3.3, 0.179}, kSmall64 = {-1.15, 3.75, 0.184}, kSmall128 = {-0.4, 3.75, 0.215};
-constexpr double kSplitCost = 1.67, kBytesPerUs = 7.1e6;
+constexpr FormCost kPair = {3.65, 0.72, 0.290};
+constexpr double kCutStage[5] = {0, kPair.stage, 0.182, 0, 0.165};  // of a tile in one, two, four parts
+constexpr FormCost kSmall32 = {-1.07, 3.37, 0.176}, kSmall64 = {-0.85, 3.44, 0.182}, kSmall128 = {-0.11, 3.41, 0.213};
+constexpr double kSplitCost = 1.66, kBytesPerUs = 7.3e6;
 
 struct Form {
   bool pair;
@@ -763,7 +764,7 @@ Form choose_form(int M, int N, int K, const mg::DeviceInfo& di, const mg::Option
     const double all = tiles(256, 256);
     const PairPlan pl = plan_pair(all, sms / 2);
     const bool rest = (double)pl.rounds * pl.clusters < all;
-    const double compute = stages * (pl.rounds * kPair.stage + (rest ? kPairCutStage[pl.cut] : 0));
+    const double compute = stages * (pl.rounds * kPair.stage + (rest ? kCutStage[pl.cut] : 0));
     least = kPair.fixed + (pl.rounds + rest) * kPair.wave + std::sqrt(compute * compute + bytes * bytes);
   }
   if (opt.int8_pair <= 0) {
