@@ -211,8 +211,8 @@ __device__ __forceinline__ RowScale row_scale(float sum, float top, const RowQua
 }
 
 // Persistent: blockDim.x threads take a row at a time (blockDim.y rows side by side in a CTA when a row is
-// one warp's).  u w (or x) of a thread's CPT chunks stays in registers, in fp32, from the statistics to the
-// codes, and the next row's chunks are on their way while the row is reduced.
+// one warp's).  A thread's CPT chunks stay in registers from the statistics to the codes, and the next row's
+// are on their way while the row is reduced.
 // CPT = 0 is the form for rows that do not fit: it reads them twice.
 constexpr int max_threads(int cpt) { return cpt >= 4 ? 512 : 1024; }  // (registers)
 
@@ -222,6 +222,7 @@ enum { kPlain = 0, kNorm = 1, kNormAdd = 2 };
 template <typename T, int MODE, bool ALIGNED, int CPT>
 __global__ void __launch_bounds__(max_threads(CPT), MODE == kPlain && CPT == 4 ? 2 : 1) row_quant_kernel(const RowQuantParams p) {
   constexpr bool NORM = MODE != kPlain, ADD = MODE == kNormAdd;
+  constexpr bool RAW = !NORM && ALIGNED;  // a plain row is kept as it lies in memory: half the registers
   using Ck = Chunk<T, ALIGNED>;
   using Raw = typename Ck::Raw;
   constexpr int CH = Ck::CH;
@@ -278,8 +279,8 @@ __global__ void __launch_bounds__(max_threads(CPT), MODE == kPlain && CPT == 4 ?
     };
     if (row < rows) fetch(row);
     for (int turn = 0; row < rows; row += step, turn ^= 1) {
-      Ck cur[NORM ? 1 : CPT];
-      float f[NORM ? CPT : 1][CH];
+      Ck cur[RAW ? CPT : 1];
+      float f[RAW ? 1 : CPT][CH];
       sum = top = 0.f;
 #pragma unroll
       for (int i = 0; i < CPT; ++i) {
@@ -288,8 +289,8 @@ __global__ void __launch_bounds__(max_threads(CPT), MODE == kPlain && CPT == 4 ?
           next[i].add(next_r[i]);
           next[i].store(u_row(row), c * CH, K - c * CH);
         }
-        if constexpr (!NORM) cur[i] = next[i];
-        values(next[i], c, true, f[NORM ? i : 0]);
+        if constexpr (RAW) cur[i] = next[i];
+        values(next[i], c, true, f[RAW ? 0 : i]);
       }
       if (row + step < rows) fetch(row + step);
       reduce_row(sum, top, warps, sh[turn]);
@@ -299,8 +300,8 @@ __global__ void __launch_bounds__(max_threads(CPT), MODE == kPlain && CPT == 4 ?
 #pragma unroll
       for (int i = 0; i < CPT; ++i) {
         const int c = i * nt + (int)threadIdx.x;
-        if constexpr (!NORM) values(cur[i], c, false, f[0]);
-        store_codes<NORM, ALIGNED, CH>(q + c * CH, K - c * CH, f[NORM ? i : 0], rs.f, rs.bad);
+        if constexpr (RAW) values(cur[i], c, false, f[0]);
+        store_codes<NORM, ALIGNED, CH>(q + c * CH, K - c * CH, f[RAW ? 0 : i], rs.f, rs.bad);
       }
     }
   } else {
