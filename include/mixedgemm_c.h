@@ -83,7 +83,12 @@ int mg_set_wait_limit_us(long long us);
  *   PDL              0: no programmatic dependent launch
  *   REORDER_CTAS     n > 0: at most n CTAs for the quantiser (to share the GPU with another kernel)
  *   FAULT_SKIP_LOAD  n > 0: host-side fault injection for tests - the first CTA of the single-CTA
- *                    GEMM never issues its n-th stage load, so the wait for it runs out
+ *                    GEMM, or of the 8-bit product, never issues its n-th stage load, so the wait for it
+ *                    runs out
+ *   INT8_FEW         0: the 8-bit product's form for one or two tokens off
+ *   INT8_PAIR        0 / 1: its CTA-pair form off / on
+ *   INT8_TOKENS      32 / 64 / 128: token tile of its small form
+ *   INT8_SPLIT       1 / 2 / 4 / 8: CTAs of the small form that share a tile's K
  * mg_set_option returns MG_ERR_SHAPE for an unknown name; mg_reset_options re-reads the environment.
  */
 int mg_set_option(const char* name, int value);
