@@ -415,8 +415,8 @@ enum { MG_BF16 = 0, MG_FP16 = 1, MG_FP32 = 2 };
  *   X      [M,K] of `dtype`, rows `ldx` elements apart (tokens of an activation, channels of a weight)
  *   Q      [M,K] int8, rows `ldq` bytes apart; bytes beyond K are left alone
  *   scale  [M] fp32
- * A row that holds a NaN or an infinity gets the scale NaN and codes 0.  Any alignment of X and Q is
- * taken; rows that all start on 16-byte boundaries (Q: 8) with K a multiple of 8 (fp32: 4) take the
+ * A row that holds a NaN or an infinity gets the scale NaN and codes 0.  X needs the alignment of its
+ * type only and Q none; rows that all start on 16-byte boundaries (Q: 8) with K a multiple of 8 (fp32: 4) take the
  * vector form.  M may be 0.
  */
 int mg_quantize_int8(const void* X, int dtype, int M, int K, size_t ldx, int8_t* Q, size_t ldq, float* scale,
@@ -426,8 +426,9 @@ int mg_quantize_int8(const void* X, int dtype, int M, int K, size_t ldx, int8_t*
  * Root-mean-square norm with the residual's addition, quantised as above:
  *   u = X + R rounded to `dtype` (written to U; R and U are both NULL when there is no residual)
  *   h = u * W / sqrt(mean_k u^2 + eps) in fp32;   Q, scale = the 8-bit form of h
- *   W [K] of `dtype`.  U may be R or X itself.  A row whose sum of squares is not a finite fp32 number
- *   gets the scale NaN and codes 0.
+ *   W [K] of `dtype`.  U may be R or X itself, and must not overlap them in any other way.  A row whose sum
+ *   of squares or one of whose products u * W is not a finite fp32 number (with eps = 0 also one whose sum is
+ *   0) gets the scale NaN and codes 0.
  */
 int mg_rms_norm_int8(const void* X, const void* R, const void* W, float eps, int dtype, int M, int K, size_t ldx,
                      size_t ldr, void* U, size_t ldu, int8_t* Q, size_t ldq, float* scale, void* stream);
@@ -452,7 +453,7 @@ int mg_rms_norm_reorder_quantize(const void* X, size_t ldx, const void* R, size_
  *          beyond K never read into the sum (K itself may be any value up to MG_INT8_MAX_K)
  *   scale_a [M], scale_b [N] fp32;  bias [N] fp32 or NULL
  *   D      [M,N] of `dtype`, rows ldd elements apart, any alignment of its type
- * No workspace.  M, N may be 0.
+ * No workspace.  M, N may be 0.  The result is the same bytes in every form the library may choose.
  */
 int mg_matmul_int8(const int8_t* A, size_t lda, const int8_t* B, size_t ldb, const float* scale_a,
                    const float* scale_b, const float* bias, int M, int N, int K, void* D, int dtype, size_t ldd,

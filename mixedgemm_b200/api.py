@@ -416,12 +416,12 @@ def _ops(required=True):
         import importlib.util
         from . import build
         path = build.ext_path("mixedgemm_ops")
-        _ops_module = False
+        module = False
         if os.path.exists(path):
             spec = importlib.util.spec_from_file_location("mixedgemm_ops", path)
             module = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(module)
-            _ops_module = module
+        _ops_module = module  # (only now: another thread may be asking)
     if _ops_module is False:
         if not required:
             return None

@@ -18,7 +18,6 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <algorithm>
 #include <atomic>
 #include <cmath>
 
@@ -34,6 +33,7 @@ using mg::wait_parity_cluster;
 
 constexpr int kRows = 128;      // channels of a CTA's tile
 constexpr int kMaxSplit = 8;
+constexpr int kMostRows = 0x7ffffe00;  // a tile that starts below still ends in 31 bits
 
 struct Int8Params {
   int M, N;
@@ -339,9 +339,16 @@ __device__ __forceinline__ uint4 load_once(const void* p) {  // read once: not w
   return v;
 }
 
+// (volatile, so that it stays behind the wait for the kernel that wrote the tokens)
+__device__ __forceinline__ uint4 load_shared_by_warps(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 template <int MT, typename T>
-__global__ void __launch_bounds__(kFewWarps * 32) int8_few_tokens_kernel(const Int8Params p, const int8_t* __restrict__ A,
-                                                                         size_t lda, const int8_t* __restrict__ B, size_t ldb,
+__global__ void __launch_bounds__(kFewWarps * 32) int8_few_tokens_kernel(const Int8Params p, const int8_t* A,
+                                                                         size_t lda, const int8_t* B, size_t ldb,
                                                                          int K, int parts) {
   __shared__ int s_sum[kFewWarps][kFewRows * MT];
   ptx::grid_dep_launch_dependents();
@@ -372,7 +379,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) int8_few_tokens_kernel(const I
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         uint4 xv = make_uint4(0, 0, 0, 0);
-        if (c + 32 * u < c1) xv = __ldg(reinterpret_cast<const uint4*>(x[m] + (size_t)(c + 32 * u) * 16));
+        if (c + 32 * u < c1) xv = load_shared_by_warps(x[m] + (size_t)(c + 32 * u) * 16);
 #pragma unroll
         for (int r = 0; r < kFewRows; ++r) {
           sum[r][m] = __dp4a((int)wv[r][u].x, (int)xv.x, sum[r][m]);
@@ -444,9 +451,9 @@ struct PairCfg {
   static constexpr uint32_t W_BYTES = 128 * 128;
   static constexpr uint32_t T_BYTES = BT / 2 * 128;
   static constexpr uint32_t STAGE_BYTES = W_BYTES + T_BYTES;
-  // Eight epilogue warps, two to a quadrant of the tensor-memory lanes, each with half of the tokens: with
-  // four, a tile of 256 x 256 took 4.7 us to store, longer than its products up to K = 2000.
-  static constexpr int EPILOGUE = 8, COLS = BT / 2, THREADS = (2 + EPILOGUE) * 32;
+  // Eight epilogue warps, two to a quadrant of the tensor-memory lanes, each with half of the tokens: 2048 x
+  // 14336 x 512 takes 21.8 us with them and 24.9 with four; from K = 4096 on it makes no difference.
+  static constexpr int SIDE = 2, EPILOGUE = 4 * SIDE, COLS = BT / SIDE, THREADS = (2 + EPILOGUE) * 32;
   static constexpr uint32_t SCALE_BYTES = EPILOGUE * COLS * 4;  // each warp's token scales
   static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + SCALE_BYTES + 256;
 };
@@ -583,7 +590,7 @@ int8_gemm_pair_kernel(const Int8Params p, int rounds, int cut, const __grid_cons
     for (int i = 0; i < count; ++i) {
       int n0, m0, width;
       locate(i, n0, m0, width);
-      const int c0 = ((warp - 2) >> 2) * (width / 2);  // this warp's tokens of the tile
+      const int c0 = ((warp - 2) >> 2) * (width / C::SIDE);  // this warp's tokens of the tile
       m0 += c0;
       const int acc = i & 1;
       const Channel<T> chan(p, n0 + quad * 32 + lane, m0);
@@ -593,7 +600,7 @@ int8_gemm_pair_kernel(const Int8Params p, int rounds, int cut, const __grid_cons
       __syncwarp();
       ptx::tc_fence_after();
       const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BT + c0);
-      const int left = min(p.M - m0, width / 2);
+      const int left = min(p.M - m0, width / C::SIDE);
       if (left <= 0) {  // none of this warp's tokens is real
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_cta(tempty_bar(acc), 0));
@@ -808,6 +815,7 @@ extern "C" int mg_matmul_int8(const int8_t* A, size_t lda, const int8_t* B, size
                               const float* scale_b, const float* bias, int M, int N, int K, void* D, int dtype,
                               size_t ldd, void* stream) {
   if (M < 0 || N < 0 || K <= 0 || K > MG_INT8_MAX_K || dtype < 0 || dtype > 2) return MG_ERR_SHAPE;
+  if (M > kMostRows || N > kMostRows) return MG_ERR_SHAPE;
   // one row has no pitch: any value stands for the smallest that a tensor map takes
   const size_t dense = ((size_t)K + 15) / 16 * 16;
   if (M <= 1) lda = dense;

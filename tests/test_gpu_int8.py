@@ -185,6 +185,20 @@ def test_norm_rows_without_a_scale(K, dtype):
     check_norm((q[4:], s[4:]), x[4:], w, None, 1e-5)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_of_faint_rows_under_weights_of_zero(dtype):
+    """eps far below the squares and nothing left after the weight: codes 0 and the smallest scale, not NaN."""
+    import mixedgemm_b200 as mg
+    x = torch.full((3, 96), 2.0 ** -20, dtype=dtype)
+    x[1, ::2] *= -1
+    w = torch.zeros(96, dtype=dtype)
+    for eps in (0.0, 1e-30):
+        q, s = (t.cpu() for t in mg.rms_norm_int8(x.cuda(), w.cuda(), eps=eps))
+        assert (q == 0).all() and (s == np.float32(TINY) / np.float32(127)).all()
+    q, s = (t.cpu() for t in mg.rms_norm_int8(torch.zeros_like(x).cuda(), (w + 1).cuda(), eps=0.0))  # 0 / 0
+    assert (q == 0).all() and torch.isnan(s).all()
+
+
 # --------------------------------------------------------------------------------------- matmul_int8
 
 def codes(rows, K, seed, lo=-128):

@@ -54,7 +54,7 @@ def product(lib, A=P, lda=64, B=P, ldb=64, sa=P, sb=P, bias=None, M=4, N=8, K=64
     (OK, dict(M=0, A=None, D=None)), (OK, dict(N=0, B=None, D=None)),
     (SHAPE, dict(M=-1)), (SHAPE, dict(N=-1)), (SHAPE, dict(K=0)), (SHAPE, dict(K=MAX_K + 1, lda=1 << 20, ldb=1 << 20)),
     (SHAPE, dict(dtype=3)), (SHAPE, dict(lda=48)), (SHAPE, dict(ldb=48)), (SHAPE, dict(ldd=7)),
-    (SHAPE, dict(lda=1 << 40)), (SHAPE, dict(ldb=1 << 40)),
+    (SHAPE, dict(lda=1 << 40)), (SHAPE, dict(ldb=1 << 40)), (SHAPE, dict(M=0x7fffffff)), (SHAPE, dict(N=0x7fffffff, ldd=0x7fffffff)),
     (ALIGN, dict(lda=72)), (ALIGN, dict(ldb=65)), (ALIGN, dict(A=P + 8)), (ALIGN, dict(B=P + 1)), (ALIGN, dict(sa=P + 2)),
     (ALIGN, dict(sb=P + 1)), (ALIGN, dict(bias=P + 2)), (ALIGN, dict(D=P + 1)), (ALIGN, dict(D=P + 2, dtype=2)),
     (NULL, dict(A=None)), (NULL, dict(B=None)), (NULL, dict(sa=None)), (NULL, dict(sb=None)), (NULL, dict(D=None)),
