@@ -33,6 +33,7 @@ using mg::wait_parity_cluster;
 
 constexpr int kRows = 128;      // channels of a CTA's tile
 constexpr int kMaxSplit = 8;
+constexpr size_t kSmemLimit = 227 * 1024;  // of a CTA
 constexpr int kMostRows = 0x7ffffe00;  // a tile that starts below still ends in 31 bits
 
 struct Int8Params {
@@ -138,37 +139,46 @@ __device__ __forceinline__ void stage_scales(float* dst, const Int8Params& p, in
 }
 
 // A tile of 128 channels x BT tokens per cluster; the CTAs of the cluster (gridDim.z of them, along z)
-// share its K slices and add their sums through distributed shared memory.
+// share its K and add their sums through distributed shared memory.  Up to 64 tokens a stage holds two slices of
+// 128 bytes of K, so that barriers and commits are paid once for both: along K a slice takes 0.135 us in place of
+// 0.165 (32 tokens) and 0.145 in place of 0.18 (64).  With 128 tokens the ring holds too few stages of two slices
+// to keep up with memory: 128 x 4096 x 14336 took 17.3 us in place of 15.7, 2048 x 1024 x 4096 9.7 in place of 10.1.
 template <int BT>
 struct SmallCfg {
-  static constexpr int STAGES = BT == 32 ? 10 : BT == 64 ? 8 : 5;
-  static constexpr uint32_t W_BYTES = kRows * 128;
+  static constexpr int SLICES = BT <= 64 ? 2 : 1;
+  static constexpr uint32_t W_BYTES = kRows * 128;  // of a slice
   static constexpr uint32_t T_BYTES = BT * 128;
-  static constexpr uint32_t STAGE_BYTES = W_BYTES + T_BYTES;
+  static constexpr uint32_t STAGE_BYTES = SLICES * (W_BYTES + T_BYTES);
+  static constexpr int MOST_STAGES = 8;
   // sums received from the other CTAs: this CTA's BT / splits columns from splits - 1 senders
   static constexpr uint32_t recv_bytes(int splits) { return (uint32_t)(splits - 1) * kRows * (BT / splits) * 4; }
   // one epilogue warp to a quadrant of the tensor-memory lanes, two from 64 tokens on (half of them each)
   static constexpr int SIDE = BT >= 64 ? 2 : 1, EPILOGUE = 4 * SIDE, COLS = BT / SIDE, THREADS = (2 + EPILOGUE) * 32;
   static constexpr uint32_t SCALE_BYTES = 4 * BT * 4;  // the tile's token scales, once per quadrant
-  static constexpr size_t smem(int splits) {
-    return 1024 + (size_t)STAGES * STAGE_BYTES + 256 + SCALE_BYTES + recv_bytes(splits);
+  static constexpr size_t smem(int splits, int ring) {
+    return 1024 + (size_t)ring * STAGE_BYTES + 256 + SCALE_BYTES + recv_bytes(splits);
+  }
+  static constexpr int ring(int splits) {  // stages that fit
+    int n = 1;
+    while (n < MOST_STAGES && smem(splits, n + 1) <= kSmemLimit) ++n;
+    return n;
   }
 };
 
 template <int BT, typename T>
-__global__ void __launch_bounds__(SmallCfg<BT>::THREADS) int8_gemm_kernel(const Int8Params p, const __grid_constant__ CUtensorMap tmW,
-                                                             const __grid_constant__ CUtensorMap tmT) {
+__global__ void __launch_bounds__(SmallCfg<BT>::THREADS) int8_gemm_kernel(
+    const Int8Params p, int ring, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT) {
   using C = SmallCfg<BT>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = ptx::smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
-  const uint32_t bar0 = base + C::STAGES * C::STAGE_BYTES;
+  const uint32_t bar0 = base + (uint32_t)ring * C::STAGE_BYTES;
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int s) { return bar0 + 8u * (C::STAGES + s); };
-  const uint32_t done_bar = bar0 + 8u * (2 * C::STAGES);
+  auto empty_bar = [&](int s) { return bar0 + 8u * (C::MOST_STAGES + s); };
+  const uint32_t done_bar = bar0 + 8u * (2 * C::MOST_STAGES);
   volatile uint32_t* tmem_holder =
-      reinterpret_cast<volatile uint32_t*>(gbase + C::STAGES * C::STAGE_BYTES + 8 * (2 * C::STAGES + 1));
+      reinterpret_cast<volatile uint32_t*>(gbase + (bar0 - base) + 8 * (2 * C::MOST_STAGES + 1));
   volatile int* stop = reinterpret_cast<volatile int*>(tmem_holder + 1);
   const uint32_t scales = bar0 + 256u;
   const uint32_t recv = scales + C::SCALE_BYTES;  // [sender][column / 4][channel][4] sums
@@ -177,7 +187,7 @@ __global__ void __launch_bounds__(SmallCfg<BT>::THREADS) int8_gemm_kernel(const 
   const int splits = gridDim.z, rank = blockIdx.z;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::STAGES; ++s) {
+    for (int s = 0; s < ring; ++s) {
       ptx::mbar_init(full_bar(s), 1);
       ptx::mbar_init(empty_bar(s), 1);
     }
@@ -207,7 +217,8 @@ __global__ void __launch_bounds__(SmallCfg<BT>::THREADS) int8_gemm_kernel(const 
   const int left = p.M - m0;     // tokens of this tile and beyond
   const int cols = BT / splits;  // columns this CTA finishes
   const uint32_t per_sender = (uint32_t)kRows * cols * 4;
-  const int s0 = (int)((long long)p.stages * rank / splits), s1 = (int)((long long)p.stages * (rank + 1) / splits);
+  const int stages = (p.stages + C::SLICES - 1) / C::SLICES;
+  const int s0 = (int)((long long)stages * rank / splits), s1 = (int)((long long)stages * (rank + 1) / splits);
 
   if (warp == 0) {
     const bool leader = ptx::elect_one();
@@ -219,10 +230,14 @@ __global__ void __launch_bounds__(SmallCfg<BT>::THREADS) int8_gemm_kernel(const 
       if (leader && !(skip > 0 && --skip == 0)) {
         const uint32_t sbase = base + slot * C::STAGE_BYTES, fb = full_bar(slot);
         ptx::mbar_expect_tx(fb, C::STAGE_BYTES);
-        ptx::tma_load_2d(sbase, &tmW, s * 128, n0, fb);
-        ptx::tma_load_2d(sbase + C::W_BYTES, &tmT, s * 128, m0, fb);
+#pragma unroll
+        for (int i = 0; i < C::SLICES; ++i) {  // (a slice beyond K reads as zeros)
+          const int k = (s * C::SLICES + i) * 128;
+          ptx::tma_load_2d(sbase + i * C::W_BYTES, &tmW, k, n0, fb);
+          ptx::tma_load_2d(sbase + C::SLICES * C::W_BYTES + i * C::T_BYTES, &tmT, k, m0, fb);
+        }
       }
-      if (++slot == C::STAGES) { slot = 0; phase ^= 1u; }
+      if (++slot == ring) { slot = 0; phase ^= 1u; }
     }
   } else if (warp == 1) {
     const bool leader = ptx::elect_one();
@@ -234,16 +249,17 @@ __global__ void __launch_bounds__(SmallCfg<BT>::THREADS) int8_gemm_kernel(const 
       if (!wait_parity(full_bar(slot), phase, stop, p.status, p.wait_cycles, 2)) { live = false; break; }
       ptx::tc_fence_after();
       const uint32_t sbase = base + slot * C::STAGE_BYTES;
-      const uint32_t w_lo = ptx::desc_lo(sbase), t_lo = ptx::desc_lo(sbase + C::W_BYTES);
+      const uint32_t w_lo = ptx::desc_lo(sbase), t_lo = ptx::desc_lo(sbase + C::SLICES * C::W_BYTES);
       if (leader) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          ptx::mma_i8(tmem, w_lo + j * 2, t_lo + j * 2, ptx::kDescHiSw128, kIdesc, accumulate);
+        for (int j = 0; j < 4 * C::SLICES; ++j) {
+          ptx::mma_i8(tmem, w_lo + (j >> 2) * (C::W_BYTES >> 4) + (j & 3) * 2, t_lo + (j >> 2) * (C::T_BYTES >> 4) + (j & 3) * 2,
+                      ptx::kDescHiSw128, kIdesc, accumulate);
           accumulate = 1;
         }
         ptx::tc_commit(empty_bar(slot));
       }
-      if (++slot == C::STAGES) { slot = 0; phase ^= 1u; }
+      if (++slot == ring) { slot = 0; phase ^= 1u; }
     }
     if (leader && live) ptx::tc_commit(done_bar);
   } else {
@@ -674,9 +690,10 @@ int launch_small(const Int8Params& p, const CUtensorMap& w, const CUtensorMap& t
                  cudaStream_t st) {
   using C = SmallCfg<BT>;
   auto kern = int8_gemm_kernel<BT, T>;
-  const size_t smem = C::smem(splits);
+  const int ring = C::ring(splits);
+  const size_t smem = C::smem(splits, ring);
   static std::atomic<unsigned long long> allowed;
-  MG_CUDA_TRY(mg::allow_smem(kern, C::smem(kMaxSplit), di.device, allowed));
+  MG_CUDA_TRY(mg::allow_smem(kern, kSmemLimit, di.device, allowed));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((p.N + kRows - 1) / kRows, (p.M + BT - 1) / BT, splits);
   cfg.blockDim = dim3(C::THREADS);
@@ -691,7 +708,7 @@ int launch_small(const Int8Params& p, const CUtensorMap& w, const CUtensorMap& t
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = mg::pdl_enabled() ? 2 : 1;
-  MG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, w, t));
+  MG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, ring, w, t));
   return MG_OK;
 }
 
@@ -710,7 +727,7 @@ int small_capacity(int splits, const mg::DeviceInfo& di) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(1, 1, splits);
     cfg.blockDim = dim3(C::THREADS);
-    cfg.dynamicSmemBytes = C::smem(splits);
+    cfg.dynamicSmemBytes = C::smem(splits, C::ring(splits));
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 1;
@@ -718,7 +735,7 @@ int small_capacity(int splits, const mg::DeviceInfo& di) {
     attr[0].val.clusterDim.z = splits;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const bool ok = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::smem(kMaxSplit)) == cudaSuccess &&
+    const bool ok = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit) == cudaSuccess &&
                     cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n >= 1;
     if (!ok) (void)cudaGetLastError();  // the question is allowed to fail; the answer is then "none"
     k = ok ? n : -1;
@@ -730,21 +747,22 @@ int small_capacity(int splits, const mg::DeviceInfo& di) {
 // Which form takes the problem: the one with the least of
 //   T = fixed + wave * waves + sqrt(compute^2 + bytes^2)   in us,
 // compute = waves * K stages of a CTA * stage (a part of a tile in the pair form's last round: kCutStage),
-// bytes = those of the operands and the result / 7.3 MB per us, waves = tiles / (clusters that run at one time).
-// The constants are fitted to 117 problems (8 to 2048 tokens, N and K = 1024, 4096, 14336, bf16 results, cold
-// weights) run with every form: over them the choice is 0.3 % slower than the best form on average and 11 %
-// at most.  What they say: a stage of the pair form runs at the tensor cores' rate (0.28 us for
-// 256 x 256 x 128), one of the small form at the rate of its loads; a pair costs two microseconds more to set
-// up, the small form a launch's worth for every further wave; adding sums across a cluster costs 1.7 us.  For
-// example 2048 x 4096 x 4096: pair 25 us, small 128 40; 256 x 4096 x 4096: pair 10.8, small 64 9.3;
-// 64 x 4096 x 4096: small 64 with four splits 7.8, one split 8.9, pair 10.
+// bytes = those of the operands and the result / 6.5 MB per us, waves = tiles / (clusters that run at one time).
+// The constants are fitted to 137 problems (8 to 2048 tokens, N and K = 1024, 4096, 14336, and 32 to 8192 tokens
+// with K = 128 and 512; bf16 results, cold weights) run with every form: over them the choice is 0.4 % slower than
+// the best form on average and 14 % at most.  What they say: a stage of the pair form runs at the tensor cores'
+// rate (0.29 us for 256 x 256 x 128), one of the small form at the rate of its loads and barriers; a pair costs two
+// microseconds more to set up, every further wave one or two; adding sums across a cluster costs 1.4 us.  For
+// example 2048 x 4096 x 4096: pair 25 us, small 128 39; 256 x 4096 x 4096: pair 10.9, small 64 8.5;
+// 64 x 4096 x 4096: small 64 with four splits 7.3, one split 8.2; 128 x 4096 x 14336: small 128 with four splits
+// 15.6, two 19.6.
 struct FormCost {
   double fixed, wave, stage;
 };
-constexpr FormCost kPair = {3.65, 0.72, 0.290};
-constexpr double kCutStage[5] = {0, kPair.stage, 0.182, 0, 0.165};  // of a tile in one, two, four parts
-constexpr FormCost kSmall32 = {-1.07, 3.37, 0.176}, kSmall64 = {-0.85, 3.44, 0.182}, kSmall128 = {-0.11, 3.41, 0.213};
-constexpr double kSplitCost = 1.66, kBytesPerUs = 7.3e6;
+constexpr FormCost kPair = {3.26, 0.99, 0.286};
+constexpr double kCutStage[5] = {0, kPair.stage, 0.186, 0, 0.169};  // of a tile in one, two, four parts
+constexpr FormCost kSmall32 = {1.26, 1.08, 0.145}, kSmall64 = {1.14, 1.41, 0.169}, kSmall128 = {1.09, 1.98, 0.225};
+constexpr double kSplitCost = 1.44, kBytesPerUs = 6.5e6;
 
 struct Form {
   bool pair;
@@ -775,8 +793,9 @@ Form choose_form(int M, int N, int K, const mg::DeviceInfo& di, const mg::Option
     least = kPair.fixed + (pl.rounds + rest) * kPair.wave + std::sqrt(compute * compute + bytes * bytes);
   }
   if (opt.int8_pair <= 0) {
-    for (int splits = 1; splits <= kMaxSplit && splits <= stages; splits *= 2) {
-      if (opt.int8_split > 0 && opt.int8_split != splits && !(opt.int8_split > splits && splits * 2 > stages)) continue;
+    const double most_splits = std::ceil(stages / 2);  // (a stage may hold two slices)
+    for (int splits = 1; splits <= kMaxSplit && splits <= most_splits; splits *= 2) {
+      if (opt.int8_split > 0 && opt.int8_split != splits && !(opt.int8_split > splits && splits * 2 > most_splits)) continue;
       for (int tokens = 32; tokens <= 128; tokens *= 2) {
         if (opt.int8_tokens > 0 && opt.int8_tokens != tokens) continue;
         if ((double)M / tokens > 65535) continue;  // (the grid's second dimension)
