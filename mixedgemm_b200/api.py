@@ -454,7 +454,8 @@ def rms_norm_reorder_quantize_x(X, weight, reorder_index, KN, KS, KO, eps=1e-6, 
     """reorder_quantize_x of the root-mean-square norm of X [M,K] bf16 (+ residual), in one launch:
     u = bf16(X + residual), h = bf16(u * weight / sqrt(mean(u^2) + eps)).  Returns the six tensors that
     reorder_quantize_x(h, ...) returns, byte for byte, and with a residual u as a seventh.  residual_out
-    may be `residual` (or X) itself, as in rms_norm_int8; `out` the six buffers of alloc_quantized_x().
+    may be `residual` (or X) itself, as in rms_norm_int8; `out` the six buffers of alloc_quantized_x();
+    without `out` the six are parts of one allocation, which is held until the last of them is gone.
     Rows start on 16-byte boundaries.  A row with a sum of squares that is not finite gets NaN scales, and
     so does a group with such an h: that row of a product is NaN, and no other."""
     return _ops().rms_norm_reorder_quantize_x(X, weight, reorder_index, KN, KS, KO, eps, residual, residual_out, out)

@@ -198,7 +198,8 @@ class MixedLinear(torch.nn.Module):
         """weights: one QuantizedWeights or several that share an input; bias: None, or one bf16
         [N_j] tensor (or None) per weight, added to the bf16 product; max_tokens: when given, the
         buffers for the quantised activation are allocated now for that many rows (forward then
-        allocates only its outputs, which is what a captured graph needs from one call to the next)."""
+        allocates only its outputs, which is what a captured graph needs from one call to the next; with
+        norm_weight the fused quantiser allocates them in each call)."""
         super().__init__()
         self.weights = list(weights) if isinstance(weights, (list, tuple)) else [weights]
         w0 = self.weights[0]

@@ -300,3 +300,27 @@ def test_product_with_and_without_the_compiled_module(monkeypatch):
             monkeypatch.undo()
             assert all(a.dtype == b.dtype and torch.equal(a, b) for a, b in zip(got, want))
     assert mg.device_status() == 0
+
+
+@pytest.mark.parametrize("split", ((512, 256, 256), (1024, 0, 0), (576, 64, 384)))
+@pytest.mark.parametrize("M", (1, 129))
+def test_buffers_the_norm_makes_are_apart_from_one_another(M, split):
+    import mixedgemm_b200 as mg
+    g, K = gen(5), 1024
+    x, w = torch.randn(M, K, generator=g).to(torch.bfloat16).cuda(), torch.randn(K, generator=g).to(torch.bfloat16).cuda()
+    order = torch.randperm(K, generator=g).to(torch.int16).cuda()
+    got = mg.rms_norm_reorder_quantize_x(x, w, order, *split)
+    given = mg.alloc_quantized_x(M, *split, x.device)
+    for t, o in zip(got, given):
+        assert t.dtype == torch.uint8 and t.shape == o.shape and t.stride() == o.stride() and t.data_ptr() % 128 == 0
+        o.fill_(255)
+    for i, t in enumerate(got):
+        t.fill_(i + 1)
+    for i, t in enumerate(got):
+        assert (t == i + 1).all()
+    for o in got:
+        o.fill_(255)
+    mg.rms_norm_reorder_quantize_x(x, w, order, *split, out=list(got))
+    mg.rms_norm_reorder_quantize_x(x, w, order, *split, out=given)
+    for t, o in zip(got, given):
+        assert torch.equal(t, o)
