@@ -33,6 +33,10 @@ namespace {
 constexpr int kConsumerWarps = 16;
 constexpr int kConsumers = kConsumerWarps * 32;
 constexpr int kThreads = kConsumers + 32;  // + one producer warp
+constexpr int kNormWarps = 8;              // of the kernel with a norm
+constexpr int kNormThreads = kThreads + kNormWarps * 32;
+constexpr int kMostStages = 8;
+constexpr int kNormBarriers = 3 * kMostStages + 4;  // full, normed, empty; full, empty of the residual's two stages
 constexpr size_t kStaticSmem = 256;        // of the kernel with a norm: the rows' partial sums
 constexpr int kRowSkew = 16;               // bytes added to the shared-memory row pitch
 
@@ -225,7 +229,8 @@ __device__ __forceinline__ void emit_group(const ReorderParams& p, const RowCtx&
 }
 
 // One (row, group): gather, scale, quantise, pack, store.
-template <bool WEIGHTS>
+// NORM: the row may hold values that are not finite; the group's scale is then NaN.
+template <bool WEIGHTS, bool NORM = false>
 __device__ __forceinline__ void quantise_group(const ReorderParams& p, const RowCtx& rc, uint32_t idx2_addr, int g) {
   float x[32];
   float maxv = 0.f;
@@ -239,10 +244,13 @@ __device__ __forceinline__ void quantise_group(const ReorderParams& p, const Row
       const unsigned hi = lds_u16(rc.smem_row + (o[j] >> 16));
       x[q * 8 + j * 2] = __uint_as_float(lo << 16);
       x[q * 8 + j * 2 + 1] = __uint_as_float(hi << 16);
-      maxv = fmaxf(maxv, fmaxf(fabsf(x[q * 8 + j * 2]), fabsf(x[q * 8 + j * 2 + 1])));
+      if constexpr (NORM)
+        asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(maxv) : "f"(maxv), "f"(x[q * 8 + j * 2]), "f"(x[q * 8 + j * 2 + 1]));
+      else
+        maxv = fmaxf(maxv, fmaxf(fabsf(x[q * 8 + j * 2]), fabsf(x[q * 8 + j * 2 + 1])));
     }
   }
-  emit_group<WEIGHTS>(p, rc, g, x, maxv, false);
+  emit_group<WEIGHTS>(p, rc, g, x, maxv, NORM && !(maxv <= 3.4028235e38f));
 }
 
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
@@ -252,37 +260,12 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// bf16(fp32(a) + fp32(b)) of both halves.  Rounded once here; going through fp32 gives the same bits, since its 24
+// significant bits are more than twice the 8 of the result and two.
 __device__ __forceinline__ uint32_t add_pair(uint32_t a, uint32_t b) {
-  float lo, hi;
-  un2(add2(f2(bf16_lo(a), bf16_hi(a)), f2(bf16_lo(b), bf16_hi(b))), lo, hi);
-  return bf16_pair(lo, hi);
-}
-
-// The same behind a root-mean-square norm: the staged row holds u, and h = bf16((u w) v) is formed on the
-// way from shared memory to the codes.  wp_addr: the norm's weight in reordered order, so that a group's
-// 32 weights are one run of 64 bytes, the same for all rows that the lanes of a warp walk.
-__device__ __forceinline__ void quantise_norm_group(const ReorderParams& p, const RowCtx& rc, uint32_t idx2_addr,
-                                                    uint32_t wp_addr, int g, float v, bool nan_row) {
-  float x[32];
-  float maxv = 0.f;
-  const uint64_t v2 = f2(v, v);
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const uint4 iv = lds_v4(idx2_addr + g * 64 + q * 16), wv = lds_v4(wp_addr + g * 64 + q * 16);
-    const unsigned o[4] = {iv.x, iv.y, iv.z, iv.w}, w[4] = {wv.x, wv.y, wv.z, wv.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const unsigned lo = lds_u16(rc.smem_row + (o[j] & 0xFFFFu));
-      const unsigned hi = lds_u16(rc.smem_row + (o[j] >> 16));
-      float a, b;
-      un2(mul2(mul2(f2(__uint_as_float(lo << 16), __uint_as_float(hi << 16)), f2(bf16_lo(w[j]), bf16_hi(w[j]))), v2), a, b);
-      const uint32_t h = bf16_pair(a, b);
-      x[q * 8 + j * 2] = bf16_lo(h);
-      x[q * 8 + j * 2 + 1] = bf16_hi(h);
-      asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(maxv) : "f"(maxv), "f"(x[q * 8 + j * 2]), "f"(x[q * 8 + j * 2 + 1]));
-    }
-  }
-  emit_group<false>(p, rc, g, x, maxv, nan_row || !(maxv <= 3.4028235e38f));
+  uint32_t r;
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 // What a norm in front of the quantiser adds to a problem.
@@ -292,57 +275,59 @@ struct NormPart {
   const uint16_t* W;
   size_t px, pr, pu;  // row pitches in elements
   float eps, inv_k;
-  int staged;         // the residual's rows are staged beside x (otherwise the consumers read them from memory)
+  int stages;         // of the residual's ring; 0: its rows are read from memory
 };
 
-// The norm's weight into shared memory, in reordered order: read in order (2-byte loads from all over it
-// cost 10 us at K = 14336), then permuted in place through registers.
-__device__ __forceinline__ void load_reordered_weight(const uint16_t* W, int K, const uint16_t* idx2, uint16_t* wp, int tid) {
-  constexpr int kMost = (32736 / 8 + kConsumers - 1) / kConsumers;  // 16-byte vectors of the longest row, per thread
-  const int nv = K >> 3;
-  if ((reinterpret_cast<uintptr_t>(W) & 15) == 0) {
-    for (int j = tid; j < nv; j += kConsumers) reinterpret_cast<uint4*>(wp)[j] = __ldg(reinterpret_cast<const uint4*>(W) + j);
-  } else {
-    for (int j = tid; j < K; j += kConsumers) wp[j] = __ldg(W + j);
-  }
-  ptx::named_barrier_sync(1, kConsumers);  // (the index is there as well)
-  const uint32_t base = ptx::smem_u32(wp);
-  uint32_t t[kMost][4];
+// The consumers bring the index in while the producer's first rows are already in flight:
+// 16-byte loads, four in flight per thread: element-wise loads through a pointer the compiler must
+// assume may alias shared memory ran one after the other, 8 to 28 L2 round trips (4 to 15 us)
+// before the first row could be touched.
+__device__ __forceinline__ void load_index(const ReorderParams& p, uint16_t* idx2, int tid) {
+  const int K = p.K;
+  if ((reinterpret_cast<uintptr_t>(p.idx) & 15) == 0) {
+    const uint4* src = reinterpret_cast<const uint4*>(p.idx);
+    uint4* dst = reinterpret_cast<uint4*>(idx2);
+    const int nv = K >> 3;
+    const unsigned kmax = (unsigned)(K - 1);
+    for (int base = 0; base < nv; base += 4 * kConsumers) {
+      uint4 v[4];
 #pragma unroll
-  for (int u = 0; u < kMost; ++u) {
-    const int j = u * kConsumers + tid;
-    if (j < nv) {
-      const uint4 o = lds_v4(ptx::smem_u32(idx2) + j * 16);
-      t[u][0] = lds_u16(base + (o.x & 0xFFFFu)) | (lds_u16(base + (o.x >> 16)) << 16);
-      t[u][1] = lds_u16(base + (o.y & 0xFFFFu)) | (lds_u16(base + (o.y >> 16)) << 16);
-      t[u][2] = lds_u16(base + (o.z & 0xFFFFu)) | (lds_u16(base + (o.z >> 16)) << 16);
-      t[u][3] = lds_u16(base + (o.w & 0xFFFFu)) | (lds_u16(base + (o.w >> 16)) << 16);
+      for (int u = 0; u < 4; ++u) {
+        const int j = base + u * kConsumers + tid;
+        if (j < nv) v[u] = __ldg(src + j);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = base + u * kConsumers + tid;
+        if (j < nv) {
+          unsigned w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            w[k] = (min(w[k] & 0xFFFFu, kmax) * 2u) | ((min(w[k] >> 16, kmax) * 2u) << 16);
+          dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
     }
-  }
-  ptx::named_barrier_sync(1, kConsumers);
-#pragma unroll
-  for (int u = 0; u < kMost; ++u) {
-    const int j = u * kConsumers + tid;
-    if (j < nv) ptx::sts_v4(base + j * 16, t[u][0], t[u][1], t[u][2], t[u][3]);
+  } else {
+    for (int i = tid; i < K; i += kConsumers) {
+      unsigned v = (uint16_t)p.idx[i];
+      v = min(v, (unsigned)(K - 1));
+      idx2[i] = (uint16_t)(v * 2);
+    }
   }
 }
 
 // One CTA's work: block `blk` of the `nblk` blocks that share the rows of problem p.
-// With NORM every stage is first normalised: kConsumerWarps / R warps share a row, read it once in 16-byte
-// vectors, add the residual (u goes to the stream and back to the staged row) and add up u^2; after one
-// barrier of the consumers the groups are quantised as always, from h = bf16((u w) v).
-template <int R, bool WEIGHTS, bool NORM = false>
-__device__ __forceinline__ void reorder_quantize_cta(const ReorderParams& p, int blk, int nblk, const NormPart* np = nullptr) {
+template <int R, bool WEIGHTS>
+__device__ __forceinline__ void reorder_quantize_cta(const ReorderParams& p, int blk, int nblk) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int K = p.K;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int S = p.stages;
   const int pitch = 2 * K + kRowSkew;
-  const int idx_bytes = (2 * K + 15) & ~15;
   uint16_t* idx2 = reinterpret_cast<uint16_t*>(smem);
-  uint16_t* wp = reinterpret_cast<uint16_t*>(smem + idx_bytes);  // (with NORM)
-  uint8_t* tiles = smem + (NORM ? 2 : 1) * idx_bytes;
-  const int stage_bytes = (NORM && np->staged ? 2 : 1) * R * pitch;  // rows of x, then of the residual
+  uint8_t* tiles = smem + ((2 * K + 15) & ~15);
+  const int stage_bytes = R * pitch;
   uint8_t* tail = tiles + (size_t)S * stage_bytes;  // barriers: full[8], empty[8], then the stop flag
   const uint32_t bar0 = ptx::smem_u32(tail);
   volatile int* stop = reinterpret_cast<volatile int*>(tail + 16 * 8);
@@ -376,57 +361,14 @@ __device__ __forceinline__ void reorder_quantize_cta(const ReorderParams& p, int
         const int nrows = min(R, row_end - row0);
         const uint32_t fb = bar0 + 8 * s;
         const uint32_t dst = ptx::smem_u32(tiles + (size_t)s * stage_bytes);
-        if constexpr (NORM) {
-          ptx::mbar_expect_tx(fb, (uint32_t)nrows * (np->staged ? 4u : 2u) * K);
-          for (int r = 0; r < nrows; ++r) {
-            ptx::bulk_load_1d(dst + r * pitch, p.X + (size_t)(row0 + r) * np->px, 2u * K, fb);
-            if (np->staged) ptx::bulk_load_1d(dst + (R + r) * pitch, np->R + (size_t)(row0 + r) * np->pr, 2u * K, fb);
-          }
-        } else {
-          ptx::mbar_expect_tx(fb, (uint32_t)nrows * 2u * K);
-          for (int r = 0; r < nrows; ++r)
-            ptx::bulk_load_1d(dst + r * pitch, p.X + (size_t)(row0 + r) * K, 2u * K, fb);
-        }
+        ptx::mbar_expect_tx(fb, (uint32_t)nrows * 2u * K);
+        for (int r = 0; r < nrows; ++r)
+          ptx::bulk_load_1d(dst + r * pitch, p.X + (size_t)(row0 + r) * K, 2u * K, fb);
       }
     }
   } else {
     // ---------------------------------------------------------------- consumers
-    // the consumers bring the index in while the producer's first rows are already in flight
-    // 16-byte loads, four in flight per thread: element-wise loads through a pointer the compiler must
-    // assume may alias shared memory ran one after the other, 8 to 28 L2 round trips (4 to 15 us)
-    // before the first row could be touched
-    if ((reinterpret_cast<uintptr_t>(p.idx) & 15) == 0) {
-      const uint4* src = reinterpret_cast<const uint4*>(p.idx);
-      uint4* dst = reinterpret_cast<uint4*>(idx2);
-      const int nv = K >> 3;
-      const unsigned kmax = (unsigned)(K - 1);
-      for (int base = 0; base < nv; base += 4 * kConsumers) {
-        uint4 v[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int j = base + u * kConsumers + tid;
-          if (j < nv) v[u] = __ldg(src + j);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int j = base + u * kConsumers + tid;
-          if (j < nv) {
-            unsigned w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              w[k] = (min(w[k] & 0xFFFFu, kmax) * 2u) | ((min(w[k] >> 16, kmax) * 2u) << 16);
-            dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-      }
-    } else {
-      for (int i = tid; i < K; i += kConsumers) {
-        unsigned v = (uint16_t)p.idx[i];
-        v = min(v, (unsigned)(K - 1));
-        idx2[i] = (uint16_t)(v * 2);
-      }
-    }
-    if constexpr (NORM) load_reordered_weight(np->W, K, idx2, wp, tid);
+    load_index(p, idx2, tid);
     ptx::named_barrier_sync(1, kConsumers);
     // a thread keeps its row
     constexpr int kGStep = kConsumers / R;
@@ -439,69 +381,14 @@ __device__ __forceinline__ void reorder_quantize_cta(const ReorderParams& p, int
     for (int it = 0; it < nstage; ++it, s = s + 1 == S ? 0 : s + 1, ph ^= (s == 0)) {
       wait_parity(bar0 + 8 * s, ph, stop, p.status, p.wait_cycles, 32);
       const int row = row_begin + it * R + r;
-      float v = 0.f;         // 1 / root-mean-square of this thread's row
-      bool nan_row = false;
-      if constexpr (NORM) {
-        // every barrier below is reached by all consumers, also after a wait that gave up
-        __shared__ float s_sum[2][kConsumerWarps];
-        constexpr int kWarpsPerRow = kConsumerWarps / R;
-        const int nr = warp / kWarpsPerRow, nlane = (warp % kWarpsPerRow) * 32 + lane;
-        const int nrow = row_begin + it * R + nr;
-        float sum, sum_hi;
-        uint64_t sum2 = 0;  // two zeros
-        if (nrow < row_end && !*stop) {
-          const uint32_t xs = ptx::smem_u32(tiles + (size_t)s * stage_bytes) + nr * pitch, rs = xs + R * pitch;
-          const bool add = np->R != nullptr;
-          const uint4* rg = reinterpret_cast<const uint4*>(np->R + (size_t)nrow * np->pr);
-          uint4* ug = reinterpret_cast<uint4*>(np->U + (size_t)nrow * np->pu);
-#pragma unroll 4
-          for (int i = nlane; i < (K >> 3); i += kWarpsPerRow * 32) {
-            uint4 a = lds_v4(xs + i * 16);
-            if (add) {
-              const uint4 b = np->staged ? lds_v4(rs + i * 16) : rg[i];
-              a.x = add_pair(a.x, b.x);
-              a.y = add_pair(a.y, b.y);
-              a.z = add_pair(a.z, b.z);
-              a.w = add_pair(a.w, b.w);
-              ug[i] = a;
-              ptx::sts_v4(xs + i * 16, a.x, a.y, a.z, a.w);
-            }
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint64_t u = f2(bf16_lo(w[k]), bf16_hi(w[k]));
-              sum2 = fma2(u, u, sum2);
-            }
-          }
-        }
-        un2(sum2, sum, sum_hi);
-        sum += sum_hi;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) s_sum[it & 1][warp] = sum;  // (the other half may still be read)
-        __syncwarp();
-        ptx::named_barrier_sync(1, kConsumers);
-        sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < kWarpsPerRow; ++i) sum += s_sum[it & 1][r * kWarpsPerRow + i];
-        nan_row = !(sum <= 3.4028235e38f);
-        v = rsqrtf(fmaf(sum, np->inv_k, np->eps));
-      }
       if (worker && row < row_end && !*stop) {
         RowCtx rc;
         rc.smem_row = ptx::smem_u32(tiles + (size_t)s * stage_bytes) + r * pitch;
         rc.sf_row = (uint32_t)(row & 31) * 16 + (uint32_t)((row >> 5) & 3) * 4;
         rc.row_blk = (uint32_t)row >> 7;
         rc.row = (uint32_t)row;
-        if constexpr (NORM) {
-          const uint32_t wp_addr = ptx::smem_u32(wp);
-          for (int g = g0; g < G; g += kGStep) quantise_norm_group(p, rc, idx2_addr, wp_addr, g, v, nan_row);
-        } else {
-          for (int g = g0; g < G; g += kGStep) quantise_group<WEIGHTS>(p, rc, idx2_addr, g);
-        }
+        for (int g = g0; g < G; g += kGStep) quantise_group<WEIGHTS>(p, rc, idx2_addr, g);
       }
-      // (the consumers wrote into the stage that the next copy overwrites)
-      if constexpr (NORM) ptx::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar0 + 8 * (8 + s));
     }
@@ -542,15 +429,234 @@ __global__ void __launch_bounds__(kThreads, 1) reorder_quantize_multi_kernel(con
   }
 }
 
-template <int R>
-__global__ void __launch_bounds__(kThreads, 1) norm_reorder_quantize_kernel(const __grid_constant__ ReorderParams p,
-                                                                            const __grid_constant__ NormPart np) {
-  reorder_quantize_cta<R, false, true>(p, (int)blockIdx.x, (int)gridDim.x, &np);
+enum Residual { kNoResidual, kStagedResidual, kResidualInMemory };
+
+// B vectors of a staged row, kStep apart: all are read before the first is written back (one after the other, each
+// would wait for shared memory by itself).
+template <int B, int kStep, Residual RES>
+__device__ __forceinline__ uint64_t sum_squares_of(uint32_t xs, uint32_t rs, const uint4* rg, uint4* ug, int i, uint64_t sum2) {
+  uint4 a[B], b[B];
+#pragma unroll
+  for (int t = 0; t < B; ++t) {
+    a[t] = lds_v4(xs + (i + t * kStep) * 16);
+    if (RES == kStagedResidual) b[t] = lds_v4(rs + (i + t * kStep) * 16);
+    if (RES == kResidualInMemory) b[t] = rg[i + t * kStep];
+  }
+#pragma unroll
+  for (int t = 0; t < B; ++t) {
+    if (RES != kNoResidual) {
+      a[t] = make_uint4(add_pair(a[t].x, b[t].x), add_pair(a[t].y, b[t].y), add_pair(a[t].z, b[t].z), add_pair(a[t].w, b[t].w));
+      ug[i + t * kStep] = a[t];
+      ptx::sts_v4(xs + (i + t * kStep) * 16, a[t].x, a[t].y, a[t].z, a[t].w);
+    }
+    const uint32_t u[4] = {a[t].x, a[t].y, a[t].z, a[t].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint64_t u2 = f2(bf16_lo(u[k]), bf16_hi(u[k]));
+      sum2 = fma2(u2, u2, sum2);
+    }
+  }
+  return sum2;
 }
 
-// norm: 0 without, 1 with (the weight beside the index), 2 with the residual's rows staged too
-size_t smem_bytes(int K, int R, int S, int norm = 0) {
-  return (size_t)(norm ? 2 : 1) * ((2 * K + 15) & ~15) + (size_t)S * (norm == 2 ? 2 : 1) * R * (2 * K + kRowSkew) + 16 * 8 + 16;
+template <int kStep, Residual RES>
+__device__ __forceinline__ uint64_t sum_squares(uint32_t xs, uint32_t rs, const uint4* rg, uint4* ug, int first, int nv) {
+  constexpr int B = RES == kNoResidual ? 4 : 2;
+  uint64_t sum2 = 0;  // two zeros
+  int i = first;
+  for (; i + (B - 1) * kStep < nv; i += B * kStep) sum2 = sum_squares_of<B, kStep, RES>(xs, rs, rg, ug, i, sum2);
+  for (; i < nv; i += kStep) sum2 = sum_squares_of<1, kStep, RES>(xs, rs, rg, ug, i, sum2);
+  return sum2;
+}
+
+// h = bf16((u w) v) in the place of u.
+template <int B, int kStep>
+__device__ __forceinline__ void normalise_some(uint32_t xs, uint32_t wts, uint64_t v2, int i) {
+  uint4 a[B], b[B];
+#pragma unroll
+  for (int t = 0; t < B; ++t) a[t] = lds_v4(xs + (i + t * kStep) * 16), b[t] = lds_v4(wts + (i + t * kStep) * 16);
+#pragma unroll
+  for (int t = 0; t < B; ++t) {
+    const uint32_t u[4] = {a[t].x, a[t].y, a[t].z, a[t].w}, w[4] = {b[t].x, b[t].y, b[t].z, b[t].w};
+    uint32_t h[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float lo, hi;
+      un2(mul2(mul2(f2(bf16_lo(u[k]), bf16_hi(u[k])), f2(bf16_lo(w[k]), bf16_hi(w[k]))), v2), lo, hi);
+      h[k] = bf16_pair(lo, hi);
+    }
+    ptx::sts_v4(xs + (i + t * kStep) * 16, h[0], h[1], h[2], h[3]);
+  }
+}
+
+template <int kStep>
+__device__ __forceinline__ void normalise(uint32_t xs, uint32_t wts, float v, int first, int nv) {
+  const uint64_t v2 = f2(v, v);
+  int i = first;
+  for (; i + kStep < nv; i += 2 * kStep) normalise_some<2, kStep>(xs, wts, v2, i);
+  if (i < nv) normalise_some<1, kStep>(xs, wts, v2, i);
+}
+
+// Root-mean-square norm in front of the quantiser: three kinds of warps, each one stage behind the one before.
+//   * the producer copies rows of x, and of the residual into a ring of their own;
+//   * kNormWarps / R warps share a row: they read it in 16-byte vectors, add the residual (u goes to the stream
+//     and back to the staged row), add up u^2, and then write h = bf16((u w) v) over u;
+//   * the quantising warps gather from h as they do from x.  A stage of fewer groups than threads goes on where
+//     the one before left off, so that all warps get their share.
+// The sum over a row is the only thing that threads wait for one another for, and only those of the row.  (With
+// the norm as a phase of the quantising warps and two barriers of all of them in a stage: 8192 x 8192 with a
+// residual 99 us, now 88; 2048 x 14336 57.7, now 48.7; 8 x 4096 4.2, now 3.8; but 512 x 4096, one stage to a CTA,
+// 6.8, now 7.1.)  Bound: shared memory, whose pipe is 73 % busy; of its wavefronts 55 % are the gather's, three
+// quarters of those because the lanes' channels meet in a bank.
+template <int R>
+__global__ void __launch_bounds__(kNormThreads, 1) norm_reorder_quantize_kernel(const __grid_constant__ ReorderParams p,
+                                                                                const __grid_constant__ NormPart np) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float s_sum[2][kNormWarps];
+  const int K = p.K, G = K >> 5;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int S = p.stages, SR = np.stages;
+  const int pitch = 2 * K + kRowSkew;
+  const int stage_bytes = R * pitch;
+  uint16_t* idx2 = reinterpret_cast<uint16_t*>(smem);
+  const uint32_t wts = ptx::smem_u32(smem) + 2 * K;
+  const uint32_t tiles = wts + 2 * K, rtiles = tiles + S * stage_bytes, bar0 = rtiles + SR * stage_bytes;
+  volatile int* stop = reinterpret_cast<volatile int*>(smem + (bar0 - ptx::smem_u32(smem)) + kNormBarriers * 8);
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto normed = [&](int s) { return bar0 + 8u * (kMostStages + s); };
+  auto empty = [&](int s) { return bar0 + 8u * (2 * kMostStages + s); };
+  auto rfull = [&](int s) { return bar0 + 8u * (3 * kMostStages + s); };
+  auto rempty = [&](int s) { return bar0 + 8u * (3 * kMostStages + 2 + s); };
+
+  ptx::grid_dep_launch_dependents();
+  if (tid == 0) {
+    for (int s = 0; s < S; ++s) {
+      ptx::mbar_init(full(s), 1);  // one expect_tx arrival + bytes
+      ptx::mbar_init(normed(s), kNormWarps);
+      ptx::mbar_init(empty(s), kConsumerWarps);
+    }
+    for (int s = 0; s < SR; ++s) {
+      ptx::mbar_init(rfull(s), 1);
+      ptx::mbar_init(rempty(s), kNormWarps);
+    }
+    *stop = 0;
+    ptx::fence_mbar_init();
+  }
+  __syncthreads();
+  ptx::grid_dep_wait();  // nothing before this line reads or writes global memory
+
+  const int row_begin = (int)((long long)p.rows * blockIdx.x / gridDim.x);
+  const int row_end = (int)((long long)p.rows * (blockIdx.x + 1) / gridDim.x);
+  const int nstage = (row_end - row_begin + R - 1) / R;
+  int s = 0, sr = 0;
+  uint32_t ph = 0, phr = 0;
+  auto next = [&] {
+    if (++s == S) { s = 0; ph ^= 1u; }
+    if (++sr >= SR) { sr = 0; phr ^= 1u; }
+  };
+
+  if (warp == kConsumerWarps + kNormWarps) {
+    // ---------------------------------------------------------------- producer
+    if (lane == 0) {
+      for (int it = 0; it < nstage; ++it, next()) {
+        const int row0 = row_begin + it * R, nrows = min(R, row_end - row0);
+        wait_parity(empty(s), ph ^ 1u, stop, p.status, p.wait_cycles, 16);
+        ptx::mbar_expect_tx(full(s), (uint32_t)nrows * 2u * K);
+        for (int r = 0; r < nrows; ++r)
+          ptx::bulk_load_1d(tiles + s * stage_bytes + r * pitch, p.X + (size_t)(row0 + r) * np.px, 2u * K, full(s));
+        if (SR > 0) {
+          wait_parity(rempty(sr), phr ^ 1u, stop, p.status, p.wait_cycles, 16);
+          ptx::mbar_expect_tx(rfull(sr), (uint32_t)nrows * 2u * K);
+          for (int r = 0; r < nrows; ++r)
+            ptx::bulk_load_1d(rtiles + sr * stage_bytes + r * pitch, np.R + (size_t)(row0 + r) * np.pr, 2u * K, rfull(sr));
+        }
+      }
+    }
+  } else if (warp >= kConsumerWarps) {
+    // ---------------------------------------------------------------- norm
+    const int ntid = tid - kConsumers, nwarp = warp - kConsumerWarps;
+    constexpr int kWarpsPerRow = kNormWarps / R, kStep = kWarpsPerRow * 32;
+    const int nr = nwarp / kWarpsPerRow, first = ntid % kStep;
+    const int nv = K >> 3;
+    {
+      uint16_t* w = reinterpret_cast<uint16_t*>(smem + 2 * K);
+      if ((reinterpret_cast<uintptr_t>(np.W) & 15) == 0) {
+#pragma unroll 4
+        for (int j = ntid; j < nv; j += kNormWarps * 32) reinterpret_cast<uint4*>(w)[j] = __ldg(reinterpret_cast<const uint4*>(np.W) + j);
+      } else {
+        for (int j = ntid; j < K; j += kNormWarps * 32) w[j] = __ldg(np.W + j);
+      }
+      ptx::named_barrier_sync(2, kNormWarps * 32);
+    }
+    for (int it = 0; it < nstage; ++it, next()) {
+      wait_parity(full(s), ph, stop, p.status, p.wait_cycles, 32);
+      if (SR > 0) wait_parity(rfull(sr), phr, stop, p.status, p.wait_cycles, 32);
+      const int row = row_begin + it * R + nr;
+      const bool work = row < row_end && !*stop;
+      const uint32_t xs = tiles + s * stage_bytes + nr * pitch, rs = rtiles + sr * stage_bytes + nr * pitch;
+      uint64_t sum2 = 0;  // two zeros
+      if (work) {
+        const uint4* rg = reinterpret_cast<const uint4*>(np.R + (size_t)row * np.pr);
+        uint4* ug = reinterpret_cast<uint4*>(np.U + (size_t)row * np.pu);
+        if (np.R == nullptr) sum2 = sum_squares<kStep, kNoResidual>(xs, rs, rg, ug, first, nv);
+        else if (SR > 0) sum2 = sum_squares<kStep, kStagedResidual>(xs, rs, rg, ug, first, nv);
+        else sum2 = sum_squares<kStep, kResidualInMemory>(xs, rs, rg, ug, first, nv);
+      }
+      float sum, sum_hi;
+      un2(sum2, sum, sum_hi);
+      sum += sum_hi;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (SR > 0 && lane == 0) ptx::mbar_arrive(rempty(sr));  // (behind the shuffles: the whole warp has read its part)
+      if constexpr (kWarpsPerRow > 1) {  // every thread of the row comes here, also after a wait that gave up
+        if (lane == 0) s_sum[it & 1][nwarp] = sum;  // (the other half may still be read)
+        __syncwarp();
+        ptx::named_barrier_sync(3 + nr, kStep);
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kWarpsPerRow; ++i) sum += s_sum[it & 1][nr * kWarpsPerRow + i];
+      }
+      if (work) {
+        // a row whose sum is not finite: all of h is NaN
+        const float v = sum <= 3.4028235e38f ? rsqrtf(fmaf(sum, np.inv_k, np.eps)) : __uint_as_float(0x7fc00000u);
+        normalise<kStep>(xs, wts, v, first, nv);
+      }
+      ptx::fence_proxy_async_smem();  // (the next copy into the stage overwrites what was written here)
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(normed(s));
+    }
+  } else {
+    // ---------------------------------------------------------------- quantisers
+    load_index(p, idx2, tid);
+    ptx::named_barrier_sync(1, kConsumers);
+    constexpr int kGStep = kConsumers / R;
+    const uint32_t idx2_addr = ptx::smem_u32(idx2);
+    const int taken = (R * G + 31) >> 5;  // warps' worth of groups in a stage
+    int turn = warp;
+    for (int it = 0; it < nstage; ++it, next(), turn -= taken) {
+      wait_parity(normed(s), ph, stop, p.status, p.wait_cycles, 32);
+      const int t = (turn & (kConsumerWarps - 1)) * 32 + lane;
+      const int r = t % R, row = row_begin + it * R + r;
+      if (row < row_end && !*stop) {
+        RowCtx rc;
+        rc.smem_row = tiles + s * stage_bytes + r * pitch;
+        rc.sf_row = (uint32_t)(row & 31) * 16 + (uint32_t)((row >> 5) & 3) * 4;
+        rc.row_blk = (uint32_t)row >> 7;
+        rc.row = (uint32_t)row;
+        for (int g = t / R; g < G; g += kGStep) quantise_group<false, true>(p, rc, idx2_addr, g);
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(empty(s));
+    }
+  }
+  __syncthreads();
+  if (*stop) {
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);  // let copies in flight land
+  }
+}
+
+size_t smem_bytes(int K, int R, int S) {
+  return (size_t)((2 * K + 15) & ~15) + (size_t)S * R * (2 * K + kRowSkew) + 16 * 8 + 16;
 }
 
 template <int R, bool WEIGHTS>
@@ -600,20 +706,18 @@ int fill_params(bool weights, const void* X, int rows, int K, const int16_t* idx
 
 // Rows per stage and stage count of a problem whose rows are shared by `grid` CTAs; returns the
 // shared memory a CTA needs, or 0 when the problem does not fit.
-size_t stage_shape(ReorderParams* p, int grid, size_t smem_optin, int* rows_per_stage, int norm = 0) {
+size_t stage_shape(ReorderParams* p, int grid, size_t smem_optin, int* rows_per_stage) {
   const int K = p->K, rows = p->rows;
   const size_t budget = smem_optin - 1024;
-  // Behind a norm a stage costs a barrier and a reduction whatever it holds, so a CTA's rows go into as few
-  // stages as they fit (512 x 4096: 6.8 us with one stage of four rows, 10.2 with four of one).
-  const int most = norm ? (rows + grid - 1) / grid : rows / grid / 2;
+  const int rows_per_cta = rows / grid;
   static const int kRs[] = {8, 4, 2, 1};
   int R = 1;
   for (int cand : kRs)
-    if (smem_bytes(K, cand, 2, norm) <= budget && (cand <= most || cand == 1)) { R = cand; break; }
+    if (smem_bytes(K, cand, 2) <= budget && (2 * cand <= rows_per_cta || cand == 1)) { R = cand; break; }
   int S = 2;
-  while (S < 4 && smem_bytes(K, R, S + 1, norm) <= budget) ++S;
-  if (smem_bytes(K, R, 2, norm) > budget) S = 1;
-  const size_t smem = smem_bytes(K, R, S, norm);
+  while (S < 4 && smem_bytes(K, R, S + 1) <= budget) ++S;
+  if (smem_bytes(K, R, 2) > budget) S = 1;
+  const size_t smem = smem_bytes(K, R, S);
   if (smem > smem_optin) return 0;
   p->num_tiles = (rows + R - 1) / R;
   p->stages = S;
@@ -758,12 +862,34 @@ extern "C" size_t mg_code_pitch(int weights, int segment, int kseg) {
 
 namespace {
 
+// Rows per stage and stages of x and of the residual, for rows shared by `grid` CTAs; returns the shared memory a CTA
+// needs, or 0 when a row does not fit.  A stage costs 0.6 us beside what it holds, so it gets as many rows as
+// fit (8192 x 4096 without a residual: 29.6 us with eight rows, 34.5 with four, 43.2 with two).
+size_t norm_shape(ReorderParams* p, NormPart* np, int grid, size_t room, int* rows_per_stage) {
+  const int K = p->K, most = (p->rows + grid - 1) / grid;
+  const size_t row = 2 * (size_t)K + kRowSkew, fixed = 4 * (size_t)K + kNormBarriers * 8 + 16;
+  auto fits = [&](int R, int S, int SR) { return fixed + (size_t)R * (S + SR) * row <= room; };
+  int R = 1, S = 3, SR = np->R ? 2 : 0;
+  for (int cand : {8, 4, 2, 1})
+    if (cand <= most && fits(cand, S, SR)) { R = cand; break; }
+  if (!fits(R, S, SR)) S = 2, SR = SR ? 1 : 0;
+  if (!fits(R, S, SR)) SR = 0;
+  if (!fits(R, S, SR)) S = 1;
+  if (!fits(R, S, SR)) return 0;
+  while (S < kMostStages && S * R < most && fits(R, S + 1, SR)) ++S;
+  p->num_tiles = (p->rows + R - 1) / R;
+  p->stages = S;
+  np->stages = SR;
+  *rows_per_stage = R;
+  return fixed + (size_t)R * (S + SR) * row;
+}
+
 template <int R>
 int launch_norm(const ReorderParams& p, const NormPart& np, int grid, size_t smem, const mg::DeviceInfo& di, cudaStream_t st) {
   auto kern = norm_reorder_quantize_kernel<R>;
   static std::atomic<unsigned long long> allowed;
   MG_CUDA_TRY(mg::allow_smem(kern, (size_t)di.smem_optin - kStaticSmem, di.device, allowed));
-  MG_CUDA_TRY(mg::launch_kernel(kern, dim3(grid), dim3(kThreads), smem, st, p, np));
+  MG_CUDA_TRY(mg::launch_kernel(kern, dim3(grid), dim3(kNormThreads), smem, st, p, np));
   return MG_OK;
 }
 
@@ -798,11 +924,8 @@ extern "C" int mg_rms_norm_reorder_quantize(const void* X, size_t ldx, const voi
   int grid = M < di.sm_count ? M : di.sm_count;
   const int cap = mg::options().reorder_ctas;
   if (cap > 0 && grid > cap) grid = cap;
-  // the residual is staged where two stages of one row fit with it (K up to about 19000)
-  const size_t room = (size_t)di.smem_optin - kStaticSmem;
-  np.staged = R && smem_bytes(K, 1, 2, 2) <= room - 1024;
   int rows = 1;
-  const size_t smem = stage_shape(&p, grid, room, &rows, np.staged ? 2 : 1);
+  const size_t smem = norm_shape(&p, &np, grid, (size_t)di.smem_optin - kStaticSmem, &rows);
   if (smem == 0) return MG_ERR_SHAPE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (rows) {

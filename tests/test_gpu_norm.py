@@ -324,3 +324,30 @@ def test_buffers_the_norm_makes_are_apart_from_one_another(M, split):
     mg.rms_norm_reorder_quantize_x(x, w, order, *split, out=given)
     for t, o in zip(got, given):
         assert torch.equal(t, o)
+
+
+@pytest.mark.parametrize("K", (32, 1024, 4096, 8192, 14336, 17408, 20480, 32736))
+@pytest.mark.parametrize("M", (1, 150, 1333))
+def test_rows_of_every_length(M, K):
+    """Rows per stage and stages of x and of the residual depend on K: from eight rows in several stages to one row in
+    a single one with the residual read from memory.  x + r = +-2^j, so h is exact and its bytes are the quantiser's."""
+    import mixedgemm_b200 as mg
+    g = gen(M + K)
+    ko = K // 128 * 32
+    split = (K - 2 * ko, ko, ko)
+    sign = torch.randint(0, 2, (M, K), generator=g).cuda() * 2.0 - 1
+    u = (sign * torch.exp2(torch.randint(-6, 7, (M, 1), generator=g).float().cuda())).to(torch.bfloat16)
+    r = (u.float() * -0.5).to(torch.bfloat16)
+    w = (torch.randn(K, generator=g) * 3).to(torch.bfloat16).cuda()
+    order = torch.randperm(K, generator=g).to(torch.int16).cuda()
+    rows = mg.reorder_quantize_x((sign * w.float()).to(torch.bfloat16), order, *split)
+    want = [t.clone() for t in rows]
+    for x, res in ((u, None), ((u.float() * 1.5).to(torch.bfloat16), r)):
+        got = mg.rms_norm_reorder_quantize_x(x, w, order, *split, eps=0.0, residual=res)
+        if res is not None:
+            assert torch.equal(got[6], u)
+        for i in range(3):
+            assert torch.equal(got[i], want[i])
+        mg.rms_norm_reorder_quantize_x(x, w, order, *split, eps=0.0, residual=res, out=rows)
+        for i in range(3, 6):  # scale bytes behind the last row are as they were
+            assert torch.equal(rows[i], want[i])
