@@ -543,3 +543,19 @@ def test_two_host_threads_on_their_own_streams():
     [t.join() for t in threads]
     assert not bad, bad
     assert mg.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K", (8193, 10477, 16380, 16383, 16384))
+def test_long_rows_one_after_another(K, dtype):
+    """More rows than CTAs, each kept in a CTA's registers (or read twice) while the next one is fetched."""
+    import mixedgemm_b200 as mg
+    M = 333
+    x, r = tokens(M, K, dtype, seed=K), tokens(M, K, dtype, seed=K + 1)
+    w = (1 + 0.2 * torch.randn(K, generator=gen(3))).to(dtype)
+    q, s = mg.quantize_int8(x.cuda())
+    wq, ws = want_codes(x)
+    assert np.array_equal(s.cpu().numpy(), ws) and np.array_equal(q.cpu().numpy(), wq)
+    check_norm(mg.rms_norm_int8(x.cuda(), w.cuda(), eps=1e-5), x, w, None, 1e-5)
+    rd = r.cuda()
+    check_norm(mg.rms_norm_int8(x.cuda(), w.cuda(), eps=1e-5, residual=rd, residual_out=rd), x, w, r, 1e-5)
