@@ -12,12 +12,13 @@
 #include "mg_common.h"
 #include "ptx_sm100.cuh"
 
+// (The pointers are not __restrict__: these kernels are launched programmatically, so what they read may still be
+// being written when they start; see ptx::ldg_v4.)
 namespace {
 
 constexpr int kColsPerCta = 128;
 
-__global__ void __launch_bounds__(256) column_absmax_kernel(const uint16_t* __restrict__ X, int M, int K,
-                                                            uint16_t* __restrict__ keys) {
+__global__ void __launch_bounds__(256) column_absmax_kernel(const uint16_t* X, int M, int K, uint16_t* keys) {
   ptx::grid_dep_launch_dependents();
   ptx::grid_dep_wait();
   __shared__ uint32_t red[16][64];  // [row lane][channel pair]
@@ -51,8 +52,7 @@ __global__ void __launch_bounds__(256) column_absmax_kernel(const uint16_t* __re
   }
 }
 
-__global__ void __launch_bounds__(256) stable_rank_kernel(const uint16_t* __restrict__ keys, int K,
-                                                          int16_t* __restrict__ idx) {
+__global__ void __launch_bounds__(256) stable_rank_kernel(const uint16_t* keys, int K, int16_t* idx) {
   extern __shared__ uint16_t sk[];
   ptx::grid_dep_launch_dependents();
   ptx::grid_dep_wait();

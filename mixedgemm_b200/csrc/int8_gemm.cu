@@ -349,19 +349,6 @@ __global__ void __launch_bounds__(SmallCfg<BT>::THREADS) int8_gemm_kernel(
 // CTA share them when there are too few channels to keep the memory busy.
 constexpr int kFewWarps = 4, kFewRows = 4, kFewUnroll = 4, kFewTokens = 2;
 
-__device__ __forceinline__ uint4 load_once(const void* p) {  // read once: not worth a place in L1
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-
-// (volatile, so that it stays behind the wait for the kernel that wrote the tokens)
-__device__ __forceinline__ uint4 load_shared_by_warps(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-
 template <int MT, typename T>
 __global__ void __launch_bounds__(kFewWarps * 32) int8_few_tokens_kernel(const Int8Params p, const int8_t* A,
                                                                          size_t lda, const int8_t* B, size_t ldb,
@@ -369,6 +356,8 @@ __global__ void __launch_bounds__(kFewWarps * 32) int8_few_tokens_kernel(const I
   __shared__ int s_sum[kFewWarps][kFewRows * MT];
   ptx::grid_dep_launch_dependents();
   ptx::grid_dep_wait();
+  A = ptx::written_before(A);
+  B = ptx::written_before(B);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = warp / parts, part = warp - group * parts;
   const int n0 = (int)(blockIdx.x * (kFewWarps / parts) + group) * kFewRows;
@@ -389,13 +378,13 @@ __global__ void __launch_bounds__(kFewWarps * 32) int8_few_tokens_kernel(const I
     for (int u = 0; u < kFewUnroll; ++u)
 #pragma unroll
       for (int r = 0; r < kFewRows; ++r)
-        wv[r][u] = c + 32 * u < c1 ? load_once(w[r] + (size_t)(c + 32 * u) * 16) : make_uint4(0, 0, 0, 0);
+        wv[r][u] = c + 32 * u < c1 ? ptx::ldg_v4_once(w[r] + (size_t)(c + 32 * u) * 16) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int u = 0; u < kFewUnroll; ++u) {
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         uint4 xv = make_uint4(0, 0, 0, 0);
-        if (c + 32 * u < c1) xv = load_shared_by_warps(x[m] + (size_t)(c + 32 * u) * 16);
+        if (c + 32 * u < c1) xv = ptx::ldg_v4(x[m] + (size_t)(c + 32 * u) * 16);
 #pragma unroll
         for (int r = 0; r < kFewRows; ++r) {
           sum[r][m] = __dp4a((int)wv[r][u].x, (int)xv.x, sum[r][m]);

@@ -30,6 +30,37 @@ __device__ __forceinline__ void grid_dep_launch_dependents() {
 // Wait until the grids this one depends on have completed and their writes are visible.
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Loads of data that no thread of the grid writes.  A kernel launched programmatically is resident while the one
+// before it may still be writing that data, so they do not take the read-only path (ld.global.nc, what __ldg and
+// const __restrict__ pointers become): that path is for data which stays as it is for as long as the kernel is
+// resident.  The loads are pure functions of the address, free to be batched and hoisted, so the address has to
+// come through written_before, placed behind grid_dep_wait: nothing that hangs on it can move above the wait.
+template <typename T>
+__device__ __forceinline__ const T* written_before(const T* p) {
+  asm volatile("" : "+l"(p)::"memory");
+  return p;
+}
+__device__ __forceinline__ uint4 ldg_v4(const void* p) {
+  uint4 v;
+  asm("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint4 ldg_v4_once(const void* p) {  // read once: not worth a place in L1
+  uint4 v;
+  asm("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t ldg(const uint32_t* p) {
+  uint32_t v;
+  asm("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint16_t ldg(const uint16_t* p) {
+  uint16_t v;
+  asm("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p));
+  return v;
+}
+
 // ---------------------------------------------------------------- mbarrier
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");

@@ -284,8 +284,9 @@ struct NormPart {
 // before the first row could be touched.
 __device__ __forceinline__ void load_index(const ReorderParams& p, uint16_t* idx2, int tid) {
   const int K = p.K;
-  if ((reinterpret_cast<uintptr_t>(p.idx) & 15) == 0) {
-    const uint4* src = reinterpret_cast<const uint4*>(p.idx);
+  const int16_t* idx = ptx::written_before(p.idx);
+  if ((reinterpret_cast<uintptr_t>(idx) & 15) == 0) {
+    const uint4* src = reinterpret_cast<const uint4*>(idx);
     uint4* dst = reinterpret_cast<uint4*>(idx2);
     const int nv = K >> 3;
     const unsigned kmax = (unsigned)(K - 1);
@@ -294,7 +295,7 @@ __device__ __forceinline__ void load_index(const ReorderParams& p, uint16_t* idx
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int j = base + u * kConsumers + tid;
-        if (j < nv) v[u] = __ldg(src + j);
+        if (j < nv) v[u] = ptx::ldg_v4(src + j);
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -310,7 +311,7 @@ __device__ __forceinline__ void load_index(const ReorderParams& p, uint16_t* idx
     }
   } else {
     for (int i = tid; i < K; i += kConsumers) {
-      unsigned v = (uint16_t)p.idx[i];
+      unsigned v = (uint16_t)idx[i];
       v = min(v, (unsigned)(K - 1));
       idx2[i] = (uint16_t)(v * 2);
     }
@@ -580,11 +581,12 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_reorder_quantize_kernel(
     const int nv = K >> 3;
     {
       uint16_t* w = reinterpret_cast<uint16_t*>(smem + 2 * K);
-      if ((reinterpret_cast<uintptr_t>(np.W) & 15) == 0) {
+      const uint16_t* W = ptx::written_before(np.W);
+      if ((reinterpret_cast<uintptr_t>(W) & 15) == 0) {
 #pragma unroll 4
-        for (int j = ntid; j < nv; j += kNormWarps * 32) reinterpret_cast<uint4*>(w)[j] = __ldg(reinterpret_cast<const uint4*>(np.W) + j);
+        for (int j = ntid; j < nv; j += kNormWarps * 32) reinterpret_cast<uint4*>(w)[j] = ptx::ldg_v4(W + j * 8);
       } else {
-        for (int j = ntid; j < K; j += kNormWarps * 32) w[j] = __ldg(np.W + j);
+        for (int j = ntid; j < K; j += kNormWarps * 32) w[j] = ptx::ldg(W + j);
       }
       ptx::named_barrier_sync(2, kNormWarps * 32);
     }
