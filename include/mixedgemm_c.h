@@ -83,8 +83,8 @@ int mg_set_wait_limit_us(long long us);
  *   PDL              0: no programmatic dependent launch
  *   REORDER_CTAS     n > 0: at most n CTAs for the quantiser (to share the GPU with another kernel)
  *   FAULT_SKIP_LOAD  n > 0: host-side fault injection for tests - the first CTA of the single-CTA
- *                    GEMM, or of the 8-bit product, never issues its n-th stage load, so the wait for it
- *                    runs out
+ *                    GEMM, of the 8-bit product or of a quantiser into the MX formats never issues its n-th
+ *                    stage load, so the wait for it runs out
  *   INT8_FEW         0: the 8-bit product's form for one or two tokens off
  *   INT8_PAIR        0 / 1: its CTA-pair form off / on
  *   INT8_TOKENS      32 / 64 / 128: token tile of its small form

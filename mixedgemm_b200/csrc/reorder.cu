@@ -16,8 +16,9 @@
 //     computed in registers: round-half-away-from-zero is a fused multiply-add against a magic
 //     constant (FMA pipe) and the codes come from cvt.rn.satfinite.{e2m1x2,e3m2x2,e4m3x2}.f32;
 //     codes leave as 16/8-byte vector stores.
-// Waits on mbarriers are bounded; on expiry a code goes to the device status word and the
-// CTA winds down (see wait_parity).
+// Waits on mbarriers are bounded (see mg_wait.cuh): on expiry a code goes to the device status word, and a role
+// whose wait failed issues no copy, stores nothing and arrives nowhere any more, so the stage it waited for stays
+// closed to the others, whose waits then fail as well.
 #include <cuda_bf16.h>
 #include <cuda_fp4.h>
 #include <cuda_fp6.h>
@@ -26,6 +27,7 @@
 #include <atomic>
 
 #include "mg_common.h"
+#include "mg_wait.cuh"
 #include "ptx_sm100.cuh"
 
 namespace {
@@ -57,26 +59,13 @@ struct ReorderParams {
   int stages;
   long long wait_cycles;
   int* status;
+  int skip_load;  // fault injection for the bounded-wait test: the first CTA withholds its n-th stage load (0 = off)
 };
 
-// Bounded mbarrier wait; after a timeout every wait of the CTA returns at once.
-__device__ __forceinline__ void wait_parity(uint32_t bar, uint32_t parity, volatile int* stop, int* status,
-                                            long long limit, int code) {
-  if (ptx::mbar_try_wait(bar, parity)) return;
-  long long t0 = 0;
-  for (uint32_t spin = 0;; ++spin) {
-    if (ptx::mbar_try_wait(bar, parity)) return;
-    if ((spin & 63u) == 0) {
-      if (*stop) return;
-      const long long now = clock64();
-      if (spin == 0) t0 = now;
-      if (now - t0 > limit) {
-        *stop = 1;
-        atomicOr(status, code);
-        return;
-      }
-    }
-  }
+// A wait of a whole warp (see mg_wait.cuh): all lanes go on or none does.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* stop, int* status, long long limit,
+                                          int code) {
+  return __all_sync(0xffffffffu, mg::wait_parity(bar, parity, stop, status, limit, code));
 }
 
 // E8M0 byte of the smallest power of two 2^e with maxv <= fmt_max * 2^e, from the bf16
@@ -356,8 +345,10 @@ __device__ __forceinline__ void reorder_quantize_cta(const ReorderParams& p, int
     if (lane == 0) {
       int s = 0;
       uint32_t ph = 0;
+      int skip = blockIdx.x == 0 ? p.skip_load : 0;
       for (int it = 0; it < nstage; ++it, s = s + 1 == S ? 0 : s + 1, ph ^= (s == 0)) {
-        wait_parity(bar0 + 8 * (8 + s), ph ^ 1u, stop, p.status, p.wait_cycles, 16);
+        if (!mg::wait_parity(bar0 + 8 * (8 + s), ph ^ 1u, stop, p.status, p.wait_cycles, 16)) break;
+        if (skip > 0 && --skip == 0) continue;
         const int row0 = row_begin + it * R;
         const int nrows = min(R, row_end - row0);
         const uint32_t fb = bar0 + 8 * s;
@@ -380,9 +371,9 @@ __device__ __forceinline__ void reorder_quantize_cta(const ReorderParams& p, int
     int s = 0;
     uint32_t ph = 0;
     for (int it = 0; it < nstage; ++it, s = s + 1 == S ? 0 : s + 1, ph ^= (s == 0)) {
-      wait_parity(bar0 + 8 * s, ph, stop, p.status, p.wait_cycles, 32);
+      if (!warp_wait(bar0 + 8 * s, ph, stop, p.status, p.wait_cycles, 32)) break;
       const int row = row_begin + it * R + r;
-      if (worker && row < row_end && !*stop) {
+      if (worker && row < row_end) {
         RowCtx rc;
         rc.smem_row = ptx::smem_u32(tiles + (size_t)s * stage_bytes) + r * pitch;
         rc.sf_row = (uint32_t)(row & 31) * 16 + (uint32_t)((row >> 5) & 3) * 4;
@@ -559,14 +550,16 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_reorder_quantize_kernel(
   if (warp == kConsumerWarps + kNormWarps) {
     // ---------------------------------------------------------------- producer
     if (lane == 0) {
+      int skip = blockIdx.x == 0 ? p.skip_load : 0;
       for (int it = 0; it < nstage; ++it, next()) {
         const int row0 = row_begin + it * R, nrows = min(R, row_end - row0);
-        wait_parity(empty(s), ph ^ 1u, stop, p.status, p.wait_cycles, 16);
+        if (!mg::wait_parity(empty(s), ph ^ 1u, stop, p.status, p.wait_cycles, 16)) break;
+        if (skip > 0 && --skip == 0) continue;
         ptx::mbar_expect_tx(full(s), (uint32_t)nrows * 2u * K);
         for (int r = 0; r < nrows; ++r)
           ptx::bulk_load_1d(tiles + s * stage_bytes + r * pitch, p.X + (size_t)(row0 + r) * np.px, 2u * K, full(s));
         if (SR > 0) {
-          wait_parity(rempty(sr), phr ^ 1u, stop, p.status, p.wait_cycles, 16);
+          if (!mg::wait_parity(rempty(sr), phr ^ 1u, stop, p.status, p.wait_cycles, 16)) break;
           ptx::mbar_expect_tx(rfull(sr), (uint32_t)nrows * 2u * K);
           for (int r = 0; r < nrows; ++r)
             ptx::bulk_load_1d(rtiles + sr * stage_bytes + r * pitch, np.R + (size_t)(row0 + r) * np.pr, 2u * K, rfull(sr));
@@ -590,11 +583,12 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_reorder_quantize_kernel(
       }
       ptx::named_barrier_sync(2, kNormWarps * 32);
     }
+    bool live = true;  // (a warp whose wait failed still comes to the barriers of its rows)
     for (int it = 0; it < nstage; ++it, next()) {
-      wait_parity(full(s), ph, stop, p.status, p.wait_cycles, 32);
-      if (SR > 0) wait_parity(rfull(sr), phr, stop, p.status, p.wait_cycles, 32);
+      live = live && warp_wait(full(s), ph, stop, p.status, p.wait_cycles, 32) &&
+             (SR == 0 || warp_wait(rfull(sr), phr, stop, p.status, p.wait_cycles, 32));
       const int row = row_begin + it * R + nr;
-      const bool work = row < row_end && !*stop;
+      const bool work = live && row < row_end;
       const uint32_t xs = tiles + s * stage_bytes + nr * pitch, rs = rtiles + sr * stage_bytes + nr * pitch;
       uint64_t sum2 = 0;  // two zeros
       if (work) {
@@ -609,7 +603,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_reorder_quantize_kernel(
       sum += sum_hi;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (SR > 0 && lane == 0) ptx::mbar_arrive(rempty(sr));  // (behind the shuffles: the whole warp has read its part)
+      if (SR > 0 && live && lane == 0) ptx::mbar_arrive(rempty(sr));  // (behind the shuffles: the whole warp has read its part)
       if constexpr (kWarpsPerRow > 1) {  // every thread of the row comes here, also after a wait that gave up
         if (lane == 0) s_sum[it & 1][nwarp] = sum;  // (the other half may still be read)
         __syncwarp();
@@ -625,7 +619,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_reorder_quantize_kernel(
       }
       ptx::fence_proxy_async_smem();  // (the next copy into the stage overwrites what was written here)
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(normed(s));
+      if (live && lane == 0) ptx::mbar_arrive(normed(s));
     }
   } else {
     // ---------------------------------------------------------------- quantisers
@@ -636,10 +630,10 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_reorder_quantize_kernel(
     const int taken = (R * G + 31) >> 5;  // warps' worth of groups in a stage
     int turn = warp;
     for (int it = 0; it < nstage; ++it, next(), turn -= taken) {
-      wait_parity(normed(s), ph, stop, p.status, p.wait_cycles, 32);
+      if (!warp_wait(normed(s), ph, stop, p.status, p.wait_cycles, 32)) break;
       const int t = (turn & (kConsumerWarps - 1)) * 32 + lane;
       const int r = t % R, row = row_begin + it * R + r;
-      if (row < row_end && !*stop) {
+      if (row < row_end) {
         RowCtx rc;
         rc.smem_row = tiles + s * stage_bytes + r * pitch;
         rc.sf_row = (uint32_t)(row & 31) * 16 + (uint32_t)((row >> 5) & 3) * 4;
@@ -703,6 +697,7 @@ int fill_params(bool weights, const void* X, int rows, int K, const int16_t* idx
   p.seg[1] = {o6, s6, (KS + 127) / 128, (int)pitch[1]};
   p.seg[2] = {o8, s8, (KO + 127) / 128, (int)pitch[2]};
   p.wait_cycles = mg::wait_limit_cycles();
+  p.skip_load = mg::options().fault_skip_load;
   return mg::device_status_word(&p.status);
 }
 

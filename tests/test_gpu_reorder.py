@@ -243,3 +243,55 @@ def test_multi_problem_launch_of_weights_through_the_c_abi():
     assert lib.mg_reorder_quantize_multi(1, 0, None, None) == 0
     arr[1].K = 500                                                                               # K != KN + KS + KO
     assert lib.mg_reorder_quantize_multi(1, 3, ctypes.cast(arr, ctypes.c_void_p), None) == 1
+
+
+@pytest.mark.parametrize("K", [1024, 14336])
+@pytest.mark.parametrize("kind", ["x", "w", "multi", "norm", "norm and residual"])
+def test_a_quantiser_whose_load_never_comes_gives_up(kind, K, mgopt):
+    """Host-side fault injection: the first of two CTAs withholds the load of its second stage (rows 8 on at the
+    latest), with many more behind it.  With the wait limit at 1 ms every role of that CTA stops there: nothing of
+    these rows is stored, the other CTA's rows are right, the status word says so once, and the next call is
+    correct."""
+    import mixedgemm_b200 as mg
+    half = 200 if K <= 4096 else 60  # rows of a CTA
+    split = H.split_k(K)
+    x, r = H.make_x(2 * half, K, seed=1).cuda(), H.make_x(2 * half, K, seed=2).cuda()
+    w = torch.ones(K, dtype=torch.bfloat16, device="cuda")
+    idx = torch.randperm(K, generator=torch.Generator().manual_seed(3)).to(torch.int16).cuda()
+    alloc = mg.alloc_quantized_w if kind == "w" else mg.alloc_quantized_x
+    out = alloc(2 * half, *split, "cuda")
+    stream = torch.empty_like(x)
+
+    def call():
+        if kind == "x":
+            mg.reorder_quantize_x(x, idx, *split, out=out)
+        elif kind == "w":
+            mg.reorder_quantize_w(x, idx, *split, out=out)
+        elif kind == "multi":
+            mg.reorder_quantize_x_multi([(x, idx, *split, out)])
+        elif kind == "norm":
+            mg.rms_norm_reorder_quantize_x(x, w, idx, *split, out=out)
+        else:
+            mg.rms_norm_reorder_quantize_x(x, w, idx, *split, residual=r, residual_out=stream, out=out)
+        torch.cuda.synchronize()
+        return [t.clone() for t in out[:3]] + [stream.clone()]
+
+    want = call()
+    assert mg.device_status() == 0
+    mgopt.set("REORDER_CTAS", 2)
+    for t in out:
+        t.fill_(7)
+    stream.fill_(7)
+    mg.set_wait_limit_us(1000)
+    mgopt.set("FAULT_SKIP_LOAD", 2)
+    got = call()
+    assert mg.device_status() & (16 | 32)
+    for a, b in zip(got, want):
+        assert bool((a[8:half] == 7).all())
+        assert torch.equal(a[half:], b[half:]) or (a is got[3] and bool((a == 7).all()))
+    mgopt.set("FAULT_SKIP_LOAD", 0)
+    mg.set_wait_limit_us(0)
+    assert mg.device_status() == 0
+    for a, b in zip(call()[:3], want):
+        assert torch.equal(a, b)
+    assert mg.device_status() == 0
