@@ -6,7 +6,8 @@
 //
 // torch owns the memory and names the current stream; all work goes through the C ABI (mixedgemm_c.h).
 // Nothing is kept from one call to the next.  Inputs that a call does not take raise RuntimeError
-// before anything is launched.
+// before anything is launched; what the C ABI refuses is the package's MixedGemmError with the status, as on the
+// ctypes route.
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
@@ -27,13 +28,7 @@ using at::Tensor;
 using std::optional;
 
 void check(int status, const char* what) {
-  if (status == MG_OK) return;
-  static const char* names[] = {"MG_OK", "MG_ERR_SHAPE", "MG_ERR_NULL", "MG_ERR_ALIGN", "MG_ERR_WORKSPACE",
-                                "MG_ERR_CUDA", "MG_ERR_DEVICE", "MG_ERR_TIMEOUT", "MG_ERR_NCCL"};
-  std::string msg = std::string(what) + ": " + mg_strerror(status);
-  if (status >= 0 && status < 9) msg += std::string(" [") + names[status] + "]";
-  if (status == MG_ERR_CUDA) msg += " (cudaError " + std::to_string(mg_last_cuda_error()) + ")";
-  throw std::runtime_error(msg);
+  if (status != MG_OK) py::module_::import("mixedgemm_b200._capi").attr("check")(status, what);  // raises
 }
 
 int element(ScalarType t, const char* what, const char* name) {

@@ -351,3 +351,34 @@ def test_rows_of_every_length(M, K):
         mg.rms_norm_reorder_quantize_x(x, w, order, *split, eps=0.0, residual=res, out=rows)
         for i in range(3, 6):  # scale bytes behind the last row are as they were
             assert torch.equal(rows[i], want[i])
+
+
+def test_refusals_of_the_library_are_the_packages_error_on_every_route(monkeypatch):
+    """What the C ABI refuses is MixedGemmError with its status, through the compiled module as through ctypes, and
+    the same text from both."""
+    import mixedgemm_b200 as mg
+    from mixedgemm_b200 import _capi, api
+    SHAPE, ALIGN = 1, 3
+    x = torch.zeros(4, 256, dtype=torch.bfloat16, device="cuda")
+    w, q, s = x[0], torch.zeros(4, 256, dtype=torch.int8, device="cuda"), torch.ones(4, device="cuda")
+    idx = torch.arange(256, device="cuda").to(torch.int16)
+    A = mg.alloc_quantized_x(4, 128, 64, 64, "cuda")
+    narrow = [t for pair in zip(A, mg.alloc_quantized_w(100, 128, 64, 64, "cuda")) for t in pair]  # N % 128
+    crooked = [t for pair in zip(A, mg.alloc_quantized_w(128, 128, 64, 64, "cuda")) for t in pair]
+    crooked[0] = torch.zeros(4 * 64 + 4, dtype=torch.uint8, device="cuda")[4:].view(4, 64)
+    for status, call in ((SHAPE, lambda: mg.quantize_int8(x[:, :0])), (SHAPE, lambda: mg.rms_norm_int8(x, w, eps=-1.0)),
+                         (ALIGN, lambda: mg.matmul_int8(q[:, 1:33], q[:, :32], s, s)),
+                         (SHAPE, lambda: mg.rms_norm_reorder_quantize_x(x, w, idx, 144, 80, 32)),
+                         (ALIGN, lambda: mg.rms_norm_reorder_quantize_x(x[:, 1:129], w[:128], idx[:128], 64, 32, 32))):
+        with pytest.raises(_capi.MixedGemmError) as e:
+            call()
+        assert e.value.status == status
+    for status, args in ((SHAPE, narrow), (ALIGN, crooked)):
+        seen = []
+        for module in (api._ops(), False):
+            monkeypatch.setattr(api, "_ops_module", module)
+            with pytest.raises(_capi.MixedGemmError) as e:
+                mg.matmul(*args)
+            seen.append((type(e.value), e.value.status, str(e.value)))
+            monkeypatch.undo()
+        assert seen[0] == seen[1] and seen[0][1] == status
