@@ -14,6 +14,7 @@ Differences from the reference binding, all deliberate:
 import contextlib
 import ctypes
 import os
+import warnings
 
 import torch
 
@@ -405,28 +406,35 @@ def matmul_multi(problems, flags=None):
 
 # ----------------------------------------------------------------- 8-bit integers and fused norms
 
-_ops_module = None  # False: looked for and not there
+_ops_module = None  # False: looked for and not there, or it does not load
+_ops_failure = None  # why it does not load
 
 
 def _ops(required=True):
     """The compiled torch module of the operators below (csrc/ops_bindings.cpp): checks, allocation and
-    launch in one call, because at one token the same steps in Python take longer than the kernels."""
-    global _ops_module
+    launch in one call, because at one token the same steps in Python take longer than the kernels.
+    With required=False a module that is not there, or does not load (torch was replaced after the build),
+    is None: the caller has another route."""
+    global _ops_module, _ops_failure
     if _ops_module is None:
         import importlib.util
         from . import build
         path = build.ext_path("mixedgemm_ops")
         module = False
         if os.path.exists(path):
-            spec = importlib.util.spec_from_file_location("mixedgemm_ops", path)
-            module = importlib.util.module_from_spec(spec)
-            spec.loader.exec_module(module)
+            try:
+                spec = importlib.util.spec_from_file_location("mixedgemm_ops", path)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+            except ImportError as e:
+                module, _ops_failure = False, e
+                warnings.warn("mixedgemm_ops does not load, matmul goes through ctypes: %s" % e, RuntimeWarning, stacklevel=3)
         _ops_module = module  # (only now: another thread may be asking)
     if _ops_module is False:
         if not required:
             return None
-        raise ImportError("mixedgemm_ops is not built; run `python -m mixedgemm_b200.build --ext`.  "
-                          "There is no fallback path.")
+        raise ImportError("mixedgemm_ops %s; run `python -m mixedgemm_b200.build --ext`.  There is no fallback path." % (
+            "does not load (%s)" % _ops_failure if _ops_failure else "is not built")) from _ops_failure
     return _ops_module
 
 

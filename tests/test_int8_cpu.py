@@ -136,3 +136,27 @@ def test_int8_container_round_trip_on_the_cpu(tmp_path):
     assert b.codes.data_ptr() == whole.codes[3:].data_ptr()
     with pytest.raises(ValueError):
         Int8Weights.cat([a, Int8Weights(q[:, :20].contiguous(), w.scale)])
+
+
+@pytest.mark.parametrize("there", [False, True])
+def test_a_compiled_module_that_is_missing_or_does_not_load(there, monkeypatch, tmp_path):
+    """matmul then takes the ctypes route (and says once that the file does not load); the operators that have no
+    other route say why."""
+    import warnings
+    import mixedgemm_b200 as mg
+    from mixedgemm_b200 import api, build
+    path = tmp_path / "mixedgemm_ops.so"
+    if there:
+        path.write_bytes(b"not a shared object")
+    monkeypatch.setattr(build, "ext_path", lambda name="mixedgemm": str(path))
+    monkeypatch.setattr(api, "_ops_module", None)
+    monkeypatch.setattr(api, "_ops_failure", None)
+    codes, scale = torch.zeros(1, 32, dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8)
+    with warnings.catch_warnings(record=True) as seen:
+        warnings.simplefilter("always")
+        for _ in range(2):
+            with pytest.raises(RuntimeError, match="code tensors must be"):  # the ctypes route's check
+                mg.matmul(*[codes] * 6, *[scale] * 6)
+    assert len(seen) == there and all("does not load" in str(w.message) for w in seen)
+    with pytest.raises(ImportError, match="does not load" if there else "is not built"):
+        mg.quantize_int8(torch.zeros(2, 32))
