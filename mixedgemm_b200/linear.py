@@ -7,6 +7,7 @@ kind; in deployment the weight side is done once.  `QuantizedWeights` holds what
 and can be saved / loaded; `MixedLinear` owns one or several of them that share an input
 (q/k/v, gate/up) and launches them as one grouped GEMM.
 """
+import warnings
 from typing import List, Optional
 
 import torch
@@ -106,12 +107,19 @@ class QuantizedWeights:
 
 
 def _norm_weight(w, K, dtype):
-    """The weight of a module's norm: None, or a contiguous vector of K elements (in `dtype`, if given)."""
+    """The weight of a module's norm: None, or a contiguous vector of K elements (in `dtype`, if given: said aloud
+    where that takes bits from it)."""
     if w is None:
         return None
     if w.dim() != 1 or w.numel() != K:
         raise ValueError("norm_weight must be a vector of in_features elements")
-    return (w if dtype is None else w.to(dtype)).detach().contiguous()
+    w = w.detach()
+    if dtype is not None and w.dtype != dtype:
+        full, w = w, w.to(dtype)
+        if not torch.equal(w.to(full.dtype), full):
+            warnings.warn("norm_weight is rounded from %s to %s, the type the fused norm takes" % (full.dtype, dtype),
+                          UserWarning, stacklevel=3)
+    return w.contiguous()
 
 
 def _residual_rows(residual, x):
@@ -192,7 +200,8 @@ class MixedLinear(torch.nn.Module):
 
     With norm_weight the module takes the root-mean-square norm in front of the projections with it:
     forward(x, residual) normalises x + residual in the quantiser's launch and returns
-    (outputs, x + residual), forward(x) normalises x and returns the outputs."""
+    (outputs, x + residual), forward(x) normalises x and returns the outputs.  norm_weight is kept in bf16, x's type:
+    one of another type is rounded to it when the module is made, with a warning if that changes a value."""
 
     def __init__(self, weights, bias=None, max_tokens=None, norm_weight=None, eps=1e-6):
         """weights: one QuantizedWeights or several that share an input; bias: None, or one bf16
@@ -362,7 +371,8 @@ class Int8Linear(torch.nn.Module):
     """MixedLinear's counterpart with 8-bit weights and activations (a scale per channel and per token),
     for projections that 4-bit weights hurt.  Several weights that share x are one product over their
     concatenated rows, handed out as column ranges.  norm_weight, residual and what forward returns are
-    as in MixedLinear; x may be bf16, fp16 or fp32, and norm_weight has its type."""
+    as in MixedLinear; x may be bf16, fp16 or fp32, and norm_weight is kept as it is and has to have x's type (forward
+    raises otherwise: the module does not know x's type before)."""
 
     def __init__(self, weights, bias=None, norm_weight=None, eps=1e-6):
         super().__init__()

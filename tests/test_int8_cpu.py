@@ -160,3 +160,27 @@ def test_a_compiled_module_that_is_missing_or_does_not_load(there, monkeypatch, 
     assert len(seen) == there and all("does not load" in str(w.message) for w in seen)
     with pytest.raises(ImportError, match="does not load" if there else "is not built"):
         mg.quantize_int8(torch.zeros(2, 32))
+
+
+def _cpu_weights(K=64, N=128):
+    """QuantizedWeights of nothing, for what a module does when it is made."""
+    import mixedgemm_b200 as mg
+    from mixedgemm_b200.linear import QuantizedWeights
+    split = (K // 2, K // 4, K // 4)
+    return QuantizedWeights(mg.alloc_quantized_w(N, *split, "cpu"), torch.arange(K, dtype=torch.int16), split, N)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_a_norm_weight_of_another_type_is_not_rounded_without_a_word(dtype):
+    import warnings
+    from mixedgemm_b200.linear import Int8Linear, Int8Weights, MixedLinear
+    rough, fine = torch.full((64,), 1.25, dtype=dtype), torch.full((64,), 1 + 2.0 ** -9, dtype=dtype)
+    with pytest.warns(UserWarning, match="rounded"):
+        lin = MixedLinear(_cpu_weights(), norm_weight=fine)
+    assert lin.norm_weight.dtype == torch.bfloat16 and torch.equal(lin.norm_weight, fine.bfloat16())
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        assert torch.equal(MixedLinear(_cpu_weights(), norm_weight=rough).norm_weight, rough.bfloat16())
+        assert torch.equal(MixedLinear(_cpu_weights(), norm_weight=fine.bfloat16()).norm_weight, fine.bfloat16())
+        w = Int8Weights(torch.zeros(128, 64, dtype=torch.int8), torch.ones(128))
+        assert torch.equal(Int8Linear(w, norm_weight=fine).norm_weight, fine)
