@@ -207,8 +207,8 @@ class MixedLinear(torch.nn.Module):
         """weights: one QuantizedWeights or several that share an input; bias: None, or one bf16
         [N_j] tensor (or None) per weight, added to the bf16 product; max_tokens: when given, the
         buffers for the quantised activation are allocated now for that many rows (forward then
-        allocates only its outputs, which is what a captured graph needs from one call to the next; with
-        norm_weight the fused quantiser allocates them in each call)."""
+        allocates only its outputs, which is what a captured graph needs from one call to the next; it has
+        no effect with norm_weight, where the fused quantiser allocates them in each call)."""
         super().__init__()
         self.weights = list(weights) if isinstance(weights, (list, tuple)) else [weights]
         w0 = self.weights[0]
@@ -234,7 +234,7 @@ class MixedLinear(torch.nn.Module):
         self._parts = [t for w in self.weights for t in w.parts]
         self._fused_parts = list(self.fused.parts) if self.fused is not None else []
         self._a = None
-        if max_tokens is not None:
+        if max_tokens is not None and norm_weight is None:
             self._a = api.alloc_quantized_x(int(max_tokens), *self.split, self.reorder_index.device)
         self.norm_weight, self.eps = _norm_weight(norm_weight, w0.in_features, torch.bfloat16), float(eps)
 

@@ -184,3 +184,9 @@ def test_a_norm_weight_of_another_type_is_not_rounded_without_a_word(dtype):
         assert torch.equal(MixedLinear(_cpu_weights(), norm_weight=fine.bfloat16()).norm_weight, fine.bfloat16())
         w = Int8Weights(torch.zeros(128, 64, dtype=torch.int8), torch.ones(128))
         assert torch.equal(Int8Linear(w, norm_weight=fine).norm_weight, fine)
+
+
+def test_a_module_with_a_norm_keeps_no_buffers_that_it_never_uses():
+    from mixedgemm_b200.linear import MixedLinear
+    assert MixedLinear(_cpu_weights(), max_tokens=40)._a is not None
+    assert MixedLinear(_cpu_weights(), max_tokens=40, norm_weight=torch.ones(64).bfloat16())._a is None
