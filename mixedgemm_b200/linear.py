@@ -239,12 +239,13 @@ class MixedLinear(torch.nn.Module):
         self.norm_weight, self.eps = _norm_weight(norm_weight, w0.in_features, torch.bfloat16), float(eps)
 
     @classmethod
-    def from_dense(cls, Ws, calibration_x):
-        """Ws: one or several [N_j, K] bf16 weights; calibration_x: [M, K] bf16 sample whose
-        per-channel absmax orders the channels (mg_reorder_index)."""
+    def from_dense(cls, Ws, calibration_x, **kw):
+        """Ws: one or several [N_j, K] bf16 weights; calibration_x: [M, K] bf16 sample of what the
+        projections multiply (behind the norm, where the module takes one), whose per-channel absmax
+        orders the channels (mg_reorder_index); other arguments as in the constructor."""
         Ws = list(Ws) if isinstance(Ws, (list, tuple)) else [Ws]
         idx = api.reorder_index(calibration_x.contiguous())
-        return cls([QuantizedWeights.from_dense(W, idx) for W in Ws])
+        return cls([QuantizedWeights.from_dense(W, idx) for W in Ws], **kw)
 
     def _scratch(self, M, device):
         """Buffers for the quantised activation of M rows: the first M rows of the pre-allocated ones

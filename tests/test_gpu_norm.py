@@ -382,3 +382,17 @@ def test_refusals_of_the_library_are_the_packages_error_on_every_route(monkeypat
             seen.append((type(e.value), e.value.status, str(e.value)))
             monkeypatch.undo()
         assert seen[0] == seen[1] and seen[0][1] == status
+
+
+def test_mixed_linear_from_dense_takes_what_the_constructor_takes():
+    import mixedgemm_b200 as mg
+    from mixedgemm_b200.linear import MixedLinear, QuantizedWeights
+    K = 2048  # (the product takes KS and KO that are multiples of 64: 1024 channels have 32 in 8 bits)
+    X = H.make_x(300, K, seed=3).cuda()
+    Ws = [dense(N, K, N) for N in (256, 128)]
+    kw = dict(bias=[None, torch.randn(128, generator=gen(1)).cuda()], eps=1e-5,
+              norm_weight=(1 + 0.2 * torch.randn(K, generator=gen(9))).to(torch.bfloat16).cuda())
+    idx = mg.reorder_index(X)
+    want = MixedLinear([QuantizedWeights.from_dense(W, idx) for W in Ws], **kw)
+    for got, ref in zip(MixedLinear.from_dense(Ws, X, **kw)(X[:40]), want(X[:40])):
+        assert torch.equal(got, ref)
