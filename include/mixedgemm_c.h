@@ -39,7 +39,8 @@ enum {
   MG_ERR_CUDA = 5,       /* a CUDA runtime / driver call failed (see mg_last_cuda_error) */
   MG_ERR_DEVICE = 6,     /* the device is not an sm_100 part */
   MG_ERR_TIMEOUT = 7,    /* a kernel gave up on a bounded wait (see mg_device_status) */
-  MG_ERR_NCCL = 8        /* NCCL is not available in this process, or one of its calls failed */
+  MG_ERR_NCCL = 8,       /* NCCL is not available in this process, or one of its calls failed */
+  MG_ERR_OVERLAP = 9     /* an output shares memory with an input or another output where that is not allowed */
 };
 
 /* Human-readable text of a status. */
@@ -403,7 +404,9 @@ int mg_matmul_static_ws(const uint8_t* AN, const uint8_t* BN, const uint8_t* AS,
 
 /*
  * 8-bit integers with a scale for each row.  No counterpart in the reference: the form for layers
- * that 4-bit weights hurt, and the norm that stands in front of either form.
+ * that 4-bit weights hurt, and the norm that stands in front of either form.  An output of these four calls that
+ * shares a byte with an input or with another output is refused (MG_ERR_OVERLAP), but for the stream U of a norm
+ * in the place of X or R; rows that lie between one another's do not share one.
  *
  * Element types of activations and results. */
 enum { MG_BF16 = 0, MG_FP16 = 1, MG_FP32 = 2 };
@@ -426,7 +429,7 @@ int mg_quantize_int8(const void* X, int dtype, int M, int K, size_t ldx, int8_t*
  * Root-mean-square norm with the residual's addition, quantised as above:
  *   u = X + R rounded to `dtype` (written to U; R and U are both NULL when there is no residual)
  *   h = u * W / sqrt(mean_k u^2 + eps) in fp32;   Q, scale = the 8-bit form of h
- *   W [K] of `dtype`.  U may be R or X itself, and must not overlap them in any other way.  A row whose sum
+ *   W [K] of `dtype`.  U may be R or X itself (same rows, same pitch) and overlaps them in no other way.  A row whose sum
  *   of squares or one of whose products u * W is not a finite fp32 number (with eps = 0 also one whose sum is
  *   0) gets the scale NaN and codes 0.
  */

@@ -11,7 +11,7 @@ LIB_PATH = os.path.join(_PKG, "libmixedgemm_b200.so")
 
 MG_OK = 0
 STATUS_NAMES = {0: "MG_OK", 1: "MG_ERR_SHAPE", 2: "MG_ERR_NULL", 3: "MG_ERR_ALIGN", 4: "MG_ERR_WORKSPACE",
-                5: "MG_ERR_CUDA", 6: "MG_ERR_DEVICE", 7: "MG_ERR_TIMEOUT", 8: "MG_ERR_NCCL"}
+                5: "MG_ERR_CUDA", 6: "MG_ERR_DEVICE", 7: "MG_ERR_TIMEOUT", 8: "MG_ERR_NCCL", 9: "MG_ERR_OVERLAP"}
 
 # every symbol include/*.h declares, with its prototype
 _vp, _i, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t

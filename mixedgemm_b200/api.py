@@ -452,7 +452,7 @@ def rms_norm_int8(X, weight, eps=1e-6, residual=None, residual_out=None, out=Non
     u = X + residual (rounded to X's type), h = u * weight / sqrt(mean(u^2) + eps) in fp32.
     Returns (codes, scale), with a residual (codes, scale, u): u is the stream that goes on.
     weight [K] and residual [M,K] have X's type; residual_out may be `residual` (or X) itself, to
-    update the stream in place (it must not overlap them in any other way).  A row whose sum of squares
+    update the stream in place; outputs that overlap inputs in another way are refused.  A row whose sum of squares
     is not a finite fp32 number gets the scale NaN and codes 0."""
     return _ops().rms_norm_int8(X, weight, eps, residual, residual_out, out)
 

@@ -23,6 +23,7 @@
 
 #include "mg_common.h"
 #include "mg_wait.cuh"
+#include "overlap.h"
 #include "ptx_sm100.cuh"
 #include "tensor_map.h"
 
@@ -837,6 +838,11 @@ extern "C" int mg_matmul_int8(const int8_t* A, size_t lda, const int8_t* B, size
   if (!mg::aligned(A, 16) || !mg::aligned(B, 16) || !mg::aligned(scale_a, 4) || !mg::aligned(scale_b, 4) ||
       !mg::aligned(bias, 4) || !mg::aligned(D, dtype == MG_FP32 ? 4 : 2))
     return MG_ERR_ALIGN;
+  const size_t e = dtype == MG_FP32 ? 4 : 2;
+  if (mg::any_overlap({mg::Span(D, (size_t)M, (size_t)N * e, ldd * e)},
+                      {mg::Span(A, (size_t)M, (size_t)K, lda), mg::Span(B, (size_t)N, (size_t)K, ldb), mg::Span(scale_a, (size_t)M * 4),
+                       mg::Span(scale_b, (size_t)N * 4), mg::Span(bias, (size_t)N * 4)}))
+    return MG_ERR_OVERLAP;
   mg::DeviceInfo di;
   int rc = mg::device_info(&di);
   if (rc != MG_OK) return rc;

@@ -24,6 +24,7 @@
 #include <atomic>
 
 #include "mg_common.h"
+#include "overlap.h"
 #include "ptx_sm100.cuh"
 
 namespace {
@@ -407,6 +408,12 @@ int row_quant(const RowQuantParams& p, int dtype, void* stream) {
   if (!mg::aligned(p.X, e) || !mg::aligned(p.S, 4) || (NORM && !mg::aligned(p.W, e)) || !mg::aligned(p.R, e) ||
       !mg::aligned(p.U, e))
     return MG_ERR_ALIGN;
+  // a row's codes and scale are written while other rows, and in the form that reads twice its own, are still read
+  const size_t M = (size_t)p.M, bytes = (size_t)p.K * e;
+  const mg::Span x(p.X, M, bytes, p.px * e), r(p.R, M, bytes, p.pr * e), u(p.U, M, bytes, p.pu * e), w(NORM ? p.W : nullptr, bytes);
+  if (mg::any_overlap({mg::Span(p.Q, M, (size_t)p.K, p.pq), mg::Span(p.S, M * 4)}, {x, r, w, u})) return MG_ERR_OVERLAP;
+  if (p.U && (mg::overlap(u, w) || (mg::overlap(u, x) && !mg::same(u, x)) || (mg::overlap(u, r) && !mg::same(u, r))))
+    return MG_ERR_OVERLAP;
   mg::DeviceInfo di;
   const int rc = mg::device_info(&di);
   if (rc != MG_OK) return rc;

@@ -28,6 +28,7 @@
 
 #include "mg_common.h"
 #include "mg_wait.cuh"
+#include "overlap.h"
 #include "ptx_sm100.cuh"
 
 namespace {
@@ -663,8 +664,8 @@ int launch(const ReorderParams& p, int grid, size_t smem, cudaStream_t st) {
   return MG_OK;
 }
 
-// Checks one problem and fills its kernel parameters (everything but the stage shape, which depends
-// on how many CTAs the problem gets).  MG_OK with p->rows == 0 means "nothing to do".
+// Checks one problem and fills its kernel parameters (everything but the status word and the stage shape, which
+// depends on how many CTAs the problem gets).  MG_OK with p->rows == 0 means "nothing to do".
 int fill_params(bool weights, const void* X, int rows, int K, const int16_t* idx, int KN, int KS, int KO, uint8_t* o4,
                 uint8_t* o6, uint8_t* o8, const size_t* pitches, uint8_t* s4, uint8_t* s6, uint8_t* s8,
                 ReorderParams* out) {
@@ -698,7 +699,7 @@ int fill_params(bool weights, const void* X, int rows, int K, const int16_t* idx
   p.seg[2] = {o8, s8, (KO + 127) / 128, (int)pitch[2]};
   p.wait_cycles = mg::wait_limit_cycles();
   p.skip_load = mg::options().fault_skip_load;
-  return mg::device_status_word(&p.status);
+  return MG_OK;
 }
 
 // Rows per stage and stage count of a problem whose rows are shared by `grid` CTAs; returns the
@@ -729,7 +730,7 @@ int reorder_quantize(bool weights, const void* X, int rows, int K, const int16_t
   int rc = fill_params(weights, X, rows, K, idx, KN, KS, KO, o4, o6, o8, pitches, s4, s6, s8, &p);
   if (rc != MG_OK || p.rows == 0) return rc;
   mg::DeviceInfo di;
-  if ((rc = mg::device_info(&di)) != MG_OK) return rc;
+  if ((rc = mg::device_info(&di)) != MG_OK || (rc = mg::device_status_word(&p.status)) != MG_OK) return rc;
 
   // Rows per stage (8, 4, 2 or 1): as many as fit twice (double buffering) beside the index, but no more than
   // half of a CTA's share so that its last stage is not mostly empty.  Then as many stages as
@@ -782,6 +783,7 @@ extern "C" int mg_reorder_quantize_multi(int weights, int nprob, const mg_quant_
                      q.SF8, &p);
     if (rc != MG_OK) return rc;
     if (p.rows == 0) continue;
+    if ((rc = mg::device_status_word(&p.status)) != MG_OK) return rc;
     // Cost of a problem = its elements, weighted by how well its rows pipeline: a row must be whole
     // in shared memory (the index may gather from anywhere in it), so a large K leaves room for only
     // one or two rows per stage and two or three stages, and a CTA then moves 1.5x / 1.3x fewer bytes
@@ -908,6 +910,15 @@ extern "C" int mg_rms_norm_reorder_quantize(const void* X, size_t ldx, const voi
   }
   int rc = fill_params(false, X, M, K, idx, KN, KS, KO, C4, C6, C8, pitches, SF4, SF6, SF8, &p);
   if (rc != MG_OK || p.rows == 0) return rc;
+  const size_t m = (size_t)M, bytes = (size_t)K * 2;
+  const mg::Span x(X, m, bytes, ldx * 2), r(R, m, bytes, ldr * 2), u(U, m, bytes, ldu * 2), w(W, bytes), index(idx, bytes);
+  if (mg::any_overlap({mg::Span(C4, m, (size_t)KN / 2, (size_t)p.seg[0].pitch), mg::Span(C6, m, (size_t)KS / 4 * 3, (size_t)p.seg[1].pitch),
+                       mg::Span(C8, m, (size_t)KO, (size_t)p.seg[2].pitch), mg::Span(SF4, mg_sf_bytes(M, KN)),
+                       mg::Span(SF6, mg_sf_bytes(M, KS)), mg::Span(SF8, mg_sf_bytes(M, KO))},
+                      {x, r, w, index, u}))
+    return MG_ERR_OVERLAP;
+  if (U && (mg::any_overlap({u}, {w, index}) || (mg::overlap(u, x) && !mg::same(u, x)) || (mg::overlap(u, r) && !mg::same(u, r))))
+    return MG_ERR_OVERLAP;
   np.R = static_cast<const uint16_t*>(R);
   np.U = static_cast<uint16_t*>(U);
   np.W = static_cast<const uint16_t*>(W);
@@ -917,7 +928,7 @@ extern "C" int mg_rms_norm_reorder_quantize(const void* X, size_t ldx, const voi
   np.eps = eps;
   np.inv_k = 1.0f / (float)K;
   mg::DeviceInfo di;
-  if ((rc = mg::device_info(&di)) != MG_OK) return rc;
+  if ((rc = mg::device_info(&di)) != MG_OK || (rc = mg::device_status_word(&p.status)) != MG_OK) return rc;
   int grid = M < di.sm_count ? M : di.sm_count;
   const int cap = mg::options().reorder_ctas;
   if (cap > 0 && grid > cap) grid = cap;

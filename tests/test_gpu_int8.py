@@ -559,3 +559,44 @@ def test_long_rows_one_after_another(K, dtype):
     check_norm(mg.rms_norm_int8(x.cuda(), w.cuda(), eps=1e-5), x, w, None, 1e-5)
     rd = r.cuda()
     check_norm(mg.rms_norm_int8(x.cuda(), w.cuda(), eps=1e-5, residual=rd, residual_out=rd), x, w, r, 1e-5)
+
+
+def test_columns_of_one_tensor_are_apart_and_shared_bytes_are_refused():
+    """x, the residual, the stream, the codes, the scales and a result between one another's rows are taken, and give
+    what separate tensors give; a shared byte is refused, but for the stream over x or the residual."""
+    import mixedgemm_b200 as mg
+    from mixedgemm_b200 import _capi
+    M, K = 33, 64
+    x, r = tokens(M, K, torch.bfloat16, seed=1).cuda(), tokens(M, K, torch.bfloat16, seed=2).cuda()
+    w = (1 + 0.2 * torch.randn(K, generator=gen(3))).to(torch.bfloat16).cuda()
+    q0, s0, u0 = mg.rms_norm_int8(x, w, residual=r)
+    y0 = mg.matmul_int8(q0, q0, s0, s0)
+    whole = torch.zeros(M, 1024, dtype=torch.int8, device="cuda")
+    part = lambda b0, b1, t: whole[:, b0:b1].view(t)
+    xv, rv, uv = part(0, 128, torch.bfloat16), part(128, 256, torch.bfloat16), part(256, 384, torch.bfloat16)
+    qv, yv = part(384, 448, torch.int8), part(448, 448 + 2 * M, torch.bfloat16)
+    xv.copy_(x), rv.copy_(r)
+    q, s, u = mg.rms_norm_int8(xv, w, residual=rv, residual_out=uv, out=(qv, torch.empty_like(s0)))
+    assert torch.equal(q, q0) and torch.equal(s, s0) and torch.equal(u, u0)
+    assert torch.equal(mg.matmul_int8(qv, qv, s, s, out=yv), y0)
+    assert torch.equal(xv, x) and torch.equal(rv, r) and torch.equal(qv, q0) and torch.equal(uv, u0)
+    assert torch.equal(mg.quantize_int8(xv, out=(qv, s))[0], mg.quantize_int8(x)[0])
+    before = whole.clone()
+    fresh = lambda: (torch.empty_like(q0), torch.empty_like(s0))
+    bad = [
+        lambda: mg.quantize_int8(xv, out=(part(0, 64, torch.int8), s)), lambda: mg.quantize_int8(xv, out=(part(127, 191, torch.int8), s)),
+        lambda: mg.quantize_int8(part(0, 256, torch.float32)[:1], out=(qv[:1], part(252, 256, torch.float32)[0])),
+        lambda: mg.rms_norm_int8(xv, w, residual=rv, residual_out=part(2, 130, torch.bfloat16), out=fresh()),
+        lambda: mg.rms_norm_int8(xv, w, residual=rv, residual_out=part(254, 382, torch.bfloat16), out=fresh()),
+        lambda: mg.rms_norm_int8(xv[:-1], w, residual=rv[:-1], residual_out=xv[1:]), lambda: mg.rms_norm_int8(xv, xv[4], residual=rv, residual_out=xv),
+        lambda: mg.rms_norm_int8(xv, w, residual=rv, residual_out=uv, out=(part(320, 384, torch.int8), s)),
+        lambda: mg.matmul_int8(qv, qv, s, s, out=part(400, 400 + 2 * M, torch.bfloat16)),
+        lambda: mg.matmul_int8(qv, q0, s, s, out=part(384 - 2 * M + 1 + 1, 386, torch.bfloat16)),
+        lambda: mg.matmul_int8(q0[:1], q0, s[:1], s, out=s[None], out_dtype=torch.float32),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(_capi.MixedGemmError) as e:
+            call()
+            pytest.fail("case %d was not refused" % i)
+        assert e.value.status == 9, (i, str(e.value))
+    assert torch.equal(whole, before)

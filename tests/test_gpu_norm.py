@@ -396,3 +396,31 @@ def test_mixed_linear_from_dense_takes_what_the_constructor_takes():
     want = MixedLinear([QuantizedWeights.from_dense(W, idx) for W in Ws], **kw)
     for got, ref in zip(MixedLinear.from_dense(Ws, X, **kw)(X[:40]), want(X[:40])):
         assert torch.equal(got, ref)
+
+
+def test_mx_norm_between_one_anothers_rows_and_over_one_another():
+    import mixedgemm_b200 as mg
+    from mixedgemm_b200 import _capi
+    M, split = 33, (64, 32, 32)
+    x, r = H.make_x(M, 128, seed=1).cuda(), H.make_x(M, 128, seed=2).cuda()
+    w = torch.ones(128, dtype=torch.bfloat16, device="cuda")
+    idx = torch.randperm(128, generator=gen(4)).to(torch.int16).cuda()
+    ref = mg.rms_norm_reorder_quantize_x(x, w, idx, *split, residual=r)
+    whole = torch.zeros(M, 1024, dtype=torch.uint8, device="cuda")
+    part = lambda b0, b1, t: whole[:, b0:b1].view(t)
+    xv, rv, uv = part(0, 256, torch.bfloat16), part(256, 512, torch.bfloat16), part(512, 768, torch.bfloat16)
+    xv.copy_(x), rv.copy_(r)
+    out = [part(768, 800, torch.uint8), part(800, 824, torch.uint8), part(832, 864, torch.uint8)] + [torch.empty_like(t) for t in ref[3:6]]
+    got = mg.rms_norm_reorder_quantize_x(xv, w, idx, *split, residual=rv, residual_out=uv, out=out)
+    assert all(torch.equal(a, b) for a, b in zip(got[:3] + got[6:], ref[:3] + ref[6:])) and torch.equal(xv, x) and torch.equal(rv, r)
+    before = whole.clone()
+    f = lambda **kw: mg.rms_norm_reorder_quantize_x(xv, w, idx, *split, residual=rv, **kw)
+    bad = [lambda: f(residual_out=part(16, 272, torch.bfloat16)), lambda: f(residual_out=part(496, 752, torch.bfloat16)),
+           lambda: f(residual_out=uv, out=[part(752, 784, torch.uint8)] + out[1:]), lambda: f(residual_out=uv, out=out[:1] + [part(784, 808, torch.uint8)] + out[2:]),
+           lambda: f(out=out[:3] + [out[4], out[4], out[5]]), lambda: f(out=out[:2] + [part(0, 32, torch.uint8)] + out[3:])]
+    for i, call in enumerate(bad):
+        with pytest.raises(_capi.MixedGemmError) as e:
+            call()
+            pytest.fail("case %d was not refused" % i)
+        assert e.value.status == 9, (i, str(e.value))
+    assert torch.equal(whole, before)

@@ -190,3 +190,85 @@ def test_a_module_with_a_norm_keeps_no_buffers_that_it_never_uses():
     from mixedgemm_b200.linear import MixedLinear
     assert MixedLinear(_cpu_weights(), max_tokens=40)._a is not None
     assert MixedLinear(_cpu_weights(), max_tokens=40, norm_weight=torch.ones(64).bfloat16())._a is None
+
+
+# ------------------------------------------------------------------- outputs in the place of inputs
+
+OVERLAP = 9
+
+
+@pytest.fixture(scope="module")
+def overlap(tmp_path_factory):
+    """overlap.h behind a C function of two spans (start, rows, bytes, pitch)."""
+    import ctypes
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    d = tmp_path_factory.mktemp("overlap")
+    (d / "o.cpp").write_text(
+        '#include "overlap.h"\n'
+        'extern "C" int f(const size_t* v) { return mg::overlap(mg::Span((void*)v[0], v[1], v[2], v[3]), '
+        'mg::Span((void*)v[4], v[5], v[6], v[7])); }\n')
+    subprocess.check_call(["g++", "-std=c++17", "-shared", "-fPIC", "-I", os.path.join(root, "mixedgemm_b200", "csrc"),
+                           str(d / "o.cpp"), "-o", str(d / "o.so")])
+    f = ctypes.CDLL(str(d / "o.so")).f
+    return lambda a, b: bool(f((ctypes.c_size_t * 8)(*a, *b)))
+
+
+def test_overlap_of_rows_is_what_their_bytes_say(overlap):
+    import random
+    rng = random.Random(1)
+    seen = [0, 0]
+    for _ in range(20000):
+        spans = []
+        for _ in range(2):
+            size = rng.randint(0, 12)
+            spans.append((rng.randint(1, 120), rng.randint(0, 6), size, size + rng.choice([0, 1, 5, 13, 20])))
+        if rng.random() < 0.5:  # one pitch, as with columns of one tensor
+            pitch = max(s[3] for s in spans)
+            spans = [s[:3] + (pitch,) for s in spans]
+        sets = [{p + r * pitch + i for r in range(rows) for i in range(size)} for p, rows, size, pitch in spans]
+        want = bool(sets[0] & sets[1])
+        seen[want] += 1
+        assert overlap(*spans) == want, spans
+    assert min(seen) > 3000
+
+
+G = 1 << 40  # far from P
+
+
+@pytest.mark.parametrize("args", [
+    dict(Q=P), dict(Q=P + 4 * 64 * 2 - 1), dict(Q=P + 100, ldq=200), dict(Q=G, S=P + 3 * 128), dict(Q=G, S=G + 63 * 4),
+    dict(Q=P + 127, ldx=100, ldq=200, K=64),
+])
+def test_quantise_refuses_outputs_over_its_input(lib, args):
+    assert quantise(lib, **{**dict(S=2 * G), **args}) == OVERLAP
+
+
+@pytest.mark.parametrize("args", [
+    dict(Q=P), dict(S=P), dict(Q=2 * G), dict(S=2 * G + 64), dict(Q=3 * G), dict(Q=4 * G + 3), dict(S=4 * G),
+    dict(U=P + 2), dict(U=P + 128), dict(U=P, ldu=72), dict(U=3 * G + 64), dict(U=2 * G), dict(U=2 * G + 126),
+    dict(X=3 * G + 2, U=3 * G),
+])
+def test_norm_refuses_outputs_over_its_inputs(lib, args):
+    base = dict(W=2 * G, R=3 * G, ldr=64, U=4 * G, ldu=64, Q=5 * G, S=6 * G)
+    assert norm(lib, **{**base, **args}) == OVERLAP
+
+
+@pytest.mark.parametrize("args", [
+    dict(D=P), dict(D=G), dict(D=G + 7 * 64 + 62), dict(D=2 * G), dict(D=3 * G + 28), dict(D=4 * G - 2, ldd=1000), dict(D=4 * G + 28),
+])
+def test_product_refuses_a_result_over_its_operands(lib, args):
+    base = dict(B=G, sa=2 * G, sb=3 * G, bias=4 * G)
+    assert product(lib, **{**base, **args}) == OVERLAP
+
+
+@pytest.mark.parametrize("args", [
+    dict(codes=(P, G, 2 * G)), dict(codes=(G, G, 2 * G)), dict(codes=(G, G + 64, 2 * G)), dict(scales=(9 * G, 3 * G, 10 * G)),
+    dict(scales=(4 * G, 9 * G, 10 * G)), dict(scales=(9 * G, 10 * G, 9 * G + 256)), dict(codes=(G, 5 * G, 2 * G)), dict(codes=(G, 2 * G, 6 * G)),
+    dict(U=P + 16), dict(U=5 * G + 256), dict(U=3 * G), dict(U=4 * G), dict(U=P, ldu=136),
+])
+def test_mx_norm_refuses_outputs_over_its_inputs(lib, args):
+    v = {**dict(codes=(G, 2 * G, 7 * G), scales=(8 * G, 9 * G, 10 * G), W=3 * G, idx=4 * G, R=5 * G, ldr=128, U=6 * G, ldu=128), **args}
+    assert lib.mg_rms_norm_reorder_quantize(P, 128, v["R"], v["ldr"], v["W"], 1e-6, v["U"], v["ldu"], 4, 128, v["idx"], 64, 32, 32,
+                                            *v["codes"], None, *v["scales"], None) == OVERLAP
