@@ -600,3 +600,20 @@ def test_columns_of_one_tensor_are_apart_and_shared_bytes_are_refused():
             pytest.fail("case %d was not refused" % i)
         assert e.value.status == 9, (i, str(e.value))
     assert torch.equal(whole, before)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M, K", [(20011, 31), (20011, 64), (20011, 500), (20011, 512), (296, 8192), (296, 4096), (296, 4093), (5003, 1931), (5003, 4096)])
+def test_short_rows_one_after_another(M, K, dtype):
+    """More rows than threads take at once, in every form for rows up to 8192: a warp to a row, one chunk a thread
+    (8192 bf16 or fp16, 4096 fp32 and 4093 need 1024 threads, one CTA to an SM), four chunks a thread.  Each takes
+    several rows, the next on its way while one is reduced."""
+    import mixedgemm_b200 as mg
+    x, r = tokens(M, K, dtype, seed=K), tokens(M, K, dtype, seed=K + 1)
+    w = (1 + 0.2 * torch.randn(K, generator=gen(3))).to(dtype)
+    q, s = mg.quantize_int8(x.cuda())
+    wq, ws = want_codes(x)
+    assert np.array_equal(s.cpu().numpy(), ws) and np.array_equal(q.cpu().numpy(), wq)
+    check_norm(mg.rms_norm_int8(x.cuda(), w.cuda(), eps=1e-5), x, w, None, 1e-5)
+    rd = r.cuda()
+    check_norm(mg.rms_norm_int8(x.cuda(), w.cuda(), eps=1e-5, residual=rd, residual_out=rd), x, w, r, 1e-5)
