@@ -15,9 +15,11 @@
 // stream that later layers read.
 //
 // Bound: bytes, 2 + 1 per element plain in 16 bits, 6 + 1 with a residual.  14336 x 4096 bf16: plain 29.4 us
-// (6.0 TB/s), with norm and residual 63.7 us (6.5 TB/s), norm alone 34.1 us (5.2 TB/s: there the instructions
-// of the reduction show).  Rows without 16-byte alignment are moved element by element: 4096 x 1931 8.4 us
-// plain (2.8 TB/s), 17.3 us with norm and residual (3.2 TB/s).
+// (6.0 TB/s), with norm and residual 63.8 us (6.5 TB/s), norm alone 34.0 us (5.2 TB/s: one CTA to an SM, whose
+// reduction shows).  A call has a fixed part beside its bytes: 4096 elements take 2.6 us plus 1.86 us per 1000 rows
+// plain (6.6 TB/s) and 2.9 plus 2.20 behind a norm (5.6 TB/s), so 2048 rows take 6.8 and 7.1.  Rows without 16-byte
+// alignment are moved element by element: 4096 x 1931 8.5 us plain (2.8 TB/s), 17.3 us with norm and residual
+// (3.2 TB/s).  Aligned 16-bit rows beyond 16384 elements are read twice: 2048 x 28672 plain 55.5 us (bytes 27).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -216,6 +218,8 @@ __device__ __forceinline__ RowScale row_scale(float sum, float top, const RowQua
 // one warp's).  A thread's CPT chunks stay in registers from the statistics to the codes, and the next row's
 // are on their way while the row is reduced.
 // CPT = 0 is the form for rows that do not fit: it reads them twice.
+// Plain rows of four chunks a thread run two CTAs to an SM: 8192 x 16384 62 us, with one 74.  That leaves 64 registers;
+// the 16-bit aligned form is 12 bytes over, which costs 1 % at 14336 x 4096.
 constexpr int max_threads(int cpt) { return cpt >= 4 ? 512 : 1024; }  // (registers)
 
 // MODE: plain, norm, or norm behind the residual's addition
@@ -226,11 +230,12 @@ __global__ void __launch_bounds__(max_threads(CPT), MODE == kPlain && CPT == 4 ?
   constexpr bool NORM = MODE != kPlain, ADD = MODE == kNormAdd;
   constexpr bool RAW = !NORM && ALIGNED;  // a plain row is kept as it lies in memory: half the registers
   // The norm's weight is loaded wherever that suits the compiler, but in the order of the source where a thread
-  // holds 32 elements in 16-byte vectors: loaded early, it takes registers that they need (4141 x 15768 fp32 with a
-  // residual 203 us, in order 151; bf16 8192 x 16384 with one 143.7 and 141.9, 16 x 14336 without 2.57 and 2.46).
-  // Not so for fp32 without a residual (4141 x 15768 55 us, in order 78) and unaligned rows (2856 x 10477 with a
-  // residual 88 and 107).
-  constexpr bool kWeightInOrder = ALIGNED && CPT * Chunk<T, ALIGNED>::CH >= 32 && (ADD || Chunk<T, ALIGNED>::CH == 8);
+  // holds 32 elements and a weight loaded early takes registers that they need (fp32 with a residual 4141 x 15768
+  // 203 us, in order 151; fp32 unaligned 2856 x 10477 57 and 48; bf16 aligned 8192 x 16384 with a residual 143.7 and
+  // 141.9, 16 x 14336 without 2.57 and 2.46).  The other way round: fp32 aligned without a residual (4141 x 15768 55,
+  // in order 78) and 16-bit unaligned rows (2856 x 10477 with a residual 88 and 107).
+  constexpr bool kWeightInOrder =
+      CPT * Chunk<T, ALIGNED>::CH >= 32 && (sizeof(typename Chunk<T, ALIGNED>::Raw) == 4 ? ADD || !ALIGNED : ALIGNED);
   using Ck = Chunk<T, ALIGNED>;
   using Raw = typename Ck::Raw;
   constexpr int CH = Ck::CH;
@@ -377,8 +382,10 @@ int launch_rows(const RowQuantParams& p, const mg::DeviceInfo& di, cudaStream_t 
   if (chunks <= 64 && p.M > di.sm_count) return launch_form<T, MODE, ALIGNED, 2>(p, 32, 4, di, st);
   if (p.M <= 2 * di.sm_count && threads(1) <= 1024) return launch_form<T, MODE, ALIGNED, 1>(p, threads(1), 1, di, st);
   if (threads(4) <= 512) return launch_form<T, MODE, ALIGNED, 4>(p, threads(4), 1, di, st);
-  // Eight chunks of four elements (2856 x 10477 bf16 plain 28.7 us, read twice 65; 4141 x 15768 fp32 51, 115), but
-  // not where the registers do not hold them (2856 x 10477 fp32 with a residual: 201 us, read twice 146).
+  // Eight chunks of four elements (2856 x 10477 bf16 plain 28.7 us, read twice 65; 4141 x 15768 fp32 51, 115), also
+  // where the registers fall a little short (16-bit unaligned with a residual, 32 to 40 bytes spilled: 2856 x 10477
+  // 88 us, read twice 110; fp32 aligned with one, 16 bytes: 4141 x 15768 151), but not for fp32 without alignment and
+  // with a residual (2856 x 10477: 201 us, read twice 146).
   if constexpr (kChunk<T, ALIGNED> == 4 && (ALIGNED || MODE != kNormAdd || sizeof(typename Elem<T>::Raw) == 2)) {
     if (threads(8) <= 512) return launch_form<T, MODE, ALIGNED, 8>(p, threads(8), 1, di, st);
   }
