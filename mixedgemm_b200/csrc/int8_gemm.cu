@@ -143,7 +143,8 @@ __device__ __forceinline__ void stage_scales(float* dst, const Int8Params& p, in
 // share its K and add their sums through distributed shared memory.  Up to 64 tokens a stage holds two slices of
 // 128 bytes of K, so that barriers and commits are paid once for both: along K a slice takes 0.135 us in place of
 // 0.165 (32 tokens) and 0.145 in place of 0.18 (64).  With 128 tokens the ring holds too few stages of two slices
-// to keep up with memory: 128 x 4096 x 14336 took 17.3 us in place of 15.7, 2048 x 1024 x 4096 9.7 in place of 10.1.
+// to keep up with memory along a long K: 128 x 4096 x 14336 took 17.3 us in place of 15.7 (a shorter one gained:
+// 2048 x 1024 x 4096 9.7 in place of 10.1).
 template <int BT>
 struct SmallCfg {
   static constexpr int SLICES = BT <= 64 ? 2 : 1;
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) int8_few_tokens_kernel(const I
 template <int MT, typename T>
 int launch_few(const Int8Params& p, const int8_t* A, size_t lda, const int8_t* B, size_t ldb, int K, int sms, cudaStream_t st) {
   const int groups = (p.N + kFewRows - 1) / kFewRows;
-  // 16 warps an SM at least, but no part of a row shorter than one turn of its warp
+  // 16 warps an SM at least, but no part of a row shorter than a 16-byte vector for every lane
   int parts = 1;
   while (parts < kFewWarps && (long long)groups * parts < 16ll * sms && K >= parts * 2 * 32 * 16) parts *= 2;
   const int per_cta = kFewWarps / parts;
@@ -736,7 +737,8 @@ int small_capacity(int splits, const mg::DeviceInfo& di) {
 
 // Which form takes the problem: the one with the least of
 //   T = fixed + wave * waves + sqrt(compute^2 + bytes^2)   in us,
-// compute = waves * K stages of a CTA * stage (a part of a tile in the pair form's last round: kCutStage),
+// compute = waves * 128-byte slices of K of a CTA * stage (a part of a tile in the pair form's last round: kCutStage;
+// a stage of the small form that is half empty, an odd slice at 32 or 64 tokens, counts as one slice, in the fit too),
 // bytes = those of the operands and the result / 6.5 MB per us, waves = tiles / (clusters that run at one time).
 // The constants are fitted to 137 problems (8 to 2048 tokens, N and K = 1024, 4096, 14336, and 32 to 8192 tokens
 // with K = 128 and 512; bf16 results, cold weights) run with every form: over them the choice is 0.4 % slower than

@@ -7,8 +7,8 @@ namespace mg {
 // Bounded mbarrier wait: true once the phase has completed.  When the limit expires the lane
 // records `code`, raises the CTA's stop flag and returns false; from then on every wait of the CTA
 // that does not find its phase complete at the first probe returns false at once.  A role whose
-// wait failed issues nothing more (no copies, no MMAs, no arrivals) and leaves its loops; the
-// kernel then ends normally, with nothing stored.
+// wait failed issues no copy and no MMA any more and leaves its loops (an epilogue may walk its remaining
+// tiles, storing nothing); the kernel then ends normally.
 __device__ __forceinline__ bool wait_parity(uint32_t bar, uint32_t parity, volatile int* stop, int* status,
                                             long long limit, int code) {
   if (ptx::mbar_try_wait(bar, parity)) return true;

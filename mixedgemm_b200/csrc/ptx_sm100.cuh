@@ -1,6 +1,6 @@
 // Thin inline-PTX wrappers for the sm_100a features the GEMM uses: mbarrier, TMA (tiled and
 // 1-D bulk copies, no cluster broadcast forms), tensor memory and tcgen05 MMA / copy / load.
-// Every wait is bounded by the caller (see wait_parity in gemm.cu).
+// Every wait is bounded by the caller (see mg_wait.cuh).
 #pragma once
 #include <stdint.h>
 
