@@ -443,7 +443,8 @@ def quantize_int8(X, out=None):
     8 bits: returns (codes int8 [M,K], scale fp32 [M]) with X ~ codes * scale[:, None], scale = largest
     magnitude of the row / 127, codes rounded to nearest even.  The rows of X may be any distance
     apart; those of the codes start on 16-byte boundaries, as matmul_int8 needs them.  A row with a
-    value that is not finite gets the scale NaN and codes 0.  `out` = (codes, scale) to write into."""
+    value that is not finite gets the scale NaN and codes 0.  `out` = (codes, scale) to write into (not over X or one
+    another: refused)."""
     return _ops().quantize_int8(X, out)
 
 
@@ -474,7 +475,8 @@ def matmul_int8(A, B, scale_a, scale_b, bias=None, out=None, out_dtype=None):
     (A @ B^T, exact in 32-bit integers) * scale_a[:, None] * scale_b[None, :] + bias, rounded once to
     `out_dtype` (bfloat16 unless given; float16 or float32).  scale_a [M], scale_b [N] and bias [N]
     are fp32.  Rows of A and B start on 16-byte boundaries (those of quantize_int8 do); K is at most
-    131071.  `out` [M,N] receives the result instead of a new tensor; its rows may be any distance apart."""
+    131071.  `out` [M,N] receives the result instead of a new tensor; its rows may be any distance apart, but may not share
+    memory with an operand (refused)."""
     return _ops().matmul_int8(A, B, scale_a, scale_b, bias, out, out_dtype)
 
 
